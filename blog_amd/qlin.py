@@ -28,6 +28,26 @@ class GgufTensorInfo(C.Structure):
     _fields_ = [("name", C.c_char_p), ("type", C.c_int), ("n_dims", C.c_int), ("shape", C.c_int64 * 4),
                 ("nbytes", C.c_uint64), ("offset", C.c_uint64), ("data", C.c_void_p)]
 
+
+class QkRopeArgs(C.Structure):
+    """struct qlin_qk_rope (include/qlin_decoder.h)."""
+    _fields_ = [("q_norm", P), ("k_norm", P), ("norm_type", I), ("eps", F), ("one_plus", I), ("table", P),
+                ("table_len", I), ("rotary_dim", I), ("pairing", I)]
+
+
+class Kv8CacheArgs(C.Structure):
+    """struct qlin_kv8_cache (include/qlin_decoder.h)."""
+    _fields_ = [("pages", P), ("recent", P), ("block_table", P), ("n_pages", I), ("n_seqs", I), ("blocks_per_seq", I),
+                ("kv_heads", I), ("head_dim", I)]
+
+
+class LogitsControlsArgs(C.Structure):
+    """struct qlin_logits_controls (include/qlin_decoder.h)."""
+    _fields_ = [("history", P), ("history_lens", P), ("repetition", P), ("frequency", P), ("presence", P),
+                ("bias_ids", P), ("bias_values", P), ("mask", P), ("mask_stride", SZ), ("max_history", I),
+                ("max_bias", I)]
+
+
 # name -> (restype, argtypes); every symbol of include/qlin.h
 SIGNATURES = {
     "qlin_status_string": (C.c_char_p, [I]),
@@ -87,6 +107,14 @@ SIGNATURES = {
     "qlin_launch_rms_norm_quant_gemv_multi": (I, [I, I, P, SZ, P, P, I, F, I, P, P, I]),
     "qlin_launch_rms_norm_quant_swiglu": (I, [I, P, P, SZ, P, P, I, F, I, P, I, I]),
     "qlin_launch_quant_gemv_argmax": (I, [I, P, SZ, P, P, I, F, I, P, I, I, P, P]),
+    "qlin_launch_rope_table": (I, [P, I, I, F]),
+    "qlin_launch_qk_norm_rope_store_kv": (I, [P, P, SZ, P, SZ, P, SZ, P, P, P, I, I, I, I, I, P]),
+    "qlin_launch_qk_norm_rope_store_kv8": (I, [P, P, P, SZ, P, SZ, P, SZ, P, I, I, P, P]),
+    "qlin_launch_kv8_read": (I, [P, P, P, I, P, P]),
+    "qlin_attend_kv8_workspace_bytes": (SZ, [I, I, I, I, I, I]),
+    "qlin_launch_attend_kv8": (I, [P, P, P, I, I, P, P, F, P, SZ]),
+    "qlin_logits_controls_scratch_bytes": (SZ, [I, I]),
+    "qlin_launch_logits_controls": (I, [P, P, SZ, P, SZ, I, I, P, P, SZ]),
     "qlin_launch_quant_embedding": (I, [I, P, P, P, SZ, I, I]),
     "qlin_launch_mla_absorb_q_nope": (I, [I, P, P, SZ, P, I, I, I, I, I]),
     "qlin_launch_mla_absorb_q4_xsum_delta": (I, [P, P, SZ, P, I, I, I, I, I]),
@@ -246,3 +274,103 @@ def dequantize(qtype, src, out, n, f16=True):
         call("qlin_launch_dequantize_to_f16", qtype, src, out, n)
     else:
         call("qlin_launch_dequantize_to_f32", qtype, src, out, n)
+
+
+# ---- head norms with the rotation, the 8-bit attention cache, controls on logits (qlin_decoder.h) ---
+
+KV8_BLOCK, KV8_RECENT = 32, 64
+
+
+def kv8_record_bytes(head_dim):
+    """Bytes of one block of one key head in a page."""
+    return 64 * head_dim + 16
+
+
+def rope_table(table, theta):
+    """Fills table ([n_pos, rotary_dim] f32) with the cosines and sines of every position."""
+    call("qlin_launch_rope_table", table, table.shape[0], table.shape[1], theta)
+
+
+class QkRope:
+    """How heads are normed and rotated (struct qlin_qk_rope): norm weights (bf16 or f16 bits, or None) and the
+    rotation table [positions, rotary_dim] (None: no rotation).  Holds on to the tensors."""
+
+    def __init__(self, q_norm, k_norm, norm_type, eps, one_plus, table, rotary_dim, pairing=0):
+        self.tensors = (q_norm, k_norm, table)
+        self.args = QkRopeArgs(ptr(q_norm), ptr(k_norm), norm_type, eps, int(one_plus), ptr(table),
+                               table.shape[0] if table is not None else 0, rotary_dim, pairing)
+        self.address = C.addressof(self.args)
+
+
+class Kv8Cache:
+    """One layer's 8-bit cache (struct qlin_kv8_cache): pages [n_pages, kv_heads, kv8_record_bytes(head_dim)] uint8,
+    recent [n_seqs, kv_heads, 2, 64, head_dim] f32, and the block table [n_seqs, blocks_per_seq] int32, or None with
+    blocks_per_seq given.  Holds on to the tensors."""
+
+    def __init__(self, pages, recent, block_table=None, blocks_per_seq=0):
+        n_seqs, kv_heads, _, ring, head_dim = recent.shape
+        if ring != KV8_RECENT or tuple(pages.shape[1:]) != (kv_heads, kv8_record_bytes(head_dim)):
+            raise ValueError(f"pages {tuple(pages.shape)} and recent {tuple(recent.shape)} are not one cache's")
+        for name, t in (("pages", pages), ("recent", recent), ("block_table", block_table)):
+            if t is not None and not t.is_contiguous():
+                raise ValueError(f"{name} is not contiguous")
+        if block_table is not None:
+            if block_table.shape[0] != n_seqs:
+                raise ValueError(f"a block table of {block_table.shape[0]} sequences for {n_seqs}")
+            blocks_per_seq = block_table.shape[1]
+        self.pages, self.recent, self.block_table = pages, recent, block_table
+        self.n_seqs, self.kv_heads, self.head_dim, self.blocks_per_seq = n_seqs, kv_heads, head_dim, blocks_per_seq
+        self.args = Kv8CacheArgs(ptr(pages), ptr(recent), ptr(block_table), pages.shape[0], n_seqs, blocks_per_seq,
+                                 kv_heads, head_dim)
+        self.address = C.addressof(self.args)
+
+    @classmethod
+    def empty(cls, torch, n_seqs, kv_heads, head_dim, max_seq, device="cuda"):
+        """A cache of max_seq positions (in whole blocks) for each sequence, its pages in order."""
+        blocks = (max_seq + KV8_BLOCK - 1) // KV8_BLOCK
+        pages = torch.zeros(n_seqs * blocks, kv_heads, kv8_record_bytes(head_dim), dtype=torch.uint8, device=device)
+        recent = torch.zeros(n_seqs, kv_heads, 2, KV8_RECENT, head_dim, device=device)
+        return cls(pages, recent, None, blocks)
+
+
+def qk_norm_rope_store_kv(how, q, q_stride, k, k_stride, v, v_stride, q_out, kc, vc, rows, n_heads, kv_heads, head_dim,
+                          max_seq, start_pos):
+    call("qlin_launch_qk_norm_rope_store_kv", how.address, q, q_stride, k, k_stride, v, v_stride, q_out, kc, vc, rows,
+         n_heads, kv_heads, head_dim, max_seq, start_pos)
+
+
+def qk_norm_rope_store_kv8(how, cache, q, q_stride, k, k_stride, v, v_stride, q_out, rows, n_heads, start_pos,
+                           n_rows=None):
+    call("qlin_launch_qk_norm_rope_store_kv8", how.address, cache.address, q, q_stride, k, k_stride, v, v_stride, q_out,
+         rows, n_heads, start_pos, n_rows)
+
+
+def kv8_read(cache, first, lens, count, k_out, v_out):
+    call("qlin_launch_kv8_read", cache.address, first, lens, count, k_out, v_out)
+
+
+def attend_kv8_workspace_bytes(n_seqs, rows, n_heads, kv_heads, head_dim, blocks_per_seq):
+    return int(lib().qlin_attend_kv8_workspace_bytes(n_seqs, rows, n_heads, kv_heads, head_dim, blocks_per_seq))
+
+
+def attend_kv8(cache, q, attn, rows, n_heads, start_pos, n_rows, softmax_scale, workspace):
+    """workspace: a uint8 tensor of at least attend_kv8_workspace_bytes(...) (None where that is 0)."""
+    call("qlin_launch_attend_kv8", cache.address, q, attn, rows, n_heads, start_pos, n_rows, softmax_scale, workspace,
+         0 if workspace is None else workspace.numel())
+
+
+def logits_controls_scratch_bytes(rows, vocab):
+    return int(lib().qlin_logits_controls_scratch_bytes(rows, vocab))
+
+
+def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None, repetition=None, frequency=None,
+                    presence=None, bias_ids=None, bias_values=None, mask=None, picks=None, scratch=None):
+    """Penalties, biases and a mask on logits [rows, >= vocab] into out (which may be logits), and the greedy picks.
+    history [rows, max_history], bias_ids / bias_values [rows, max_bias] and mask [rows, words] (32 tokens a word) are
+    2-D and contiguous; scratch: a uint8 tensor of logits_controls_scratch_bytes(...), needed with picks."""
+    a = LogitsControlsArgs(ptr(history), ptr(history_lens), ptr(repetition), ptr(frequency), ptr(presence),
+                           ptr(bias_ids), ptr(bias_values), ptr(mask), mask.shape[1] if mask is not None else 0,
+                           history.shape[1] if history is not None else 0,
+                           bias_ids.shape[1] if bias_ids is not None else 0)
+    call("qlin_launch_logits_controls", C.addressof(a), logits, logits.stride(0), out, out.stride(0), rows, vocab, picks,
+         scratch, 0 if scratch is None else scratch.numel())
