@@ -310,8 +310,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
         k_top = block_max_bits(k_top, red);
         v_top = block_max_bits(v_top, red);
         const bool k_fin = k_top < 0x7f800000u, v_fin = v_top < 0x7f800000u;
-        const float k_scale = k_fin ? __builtin_bit_cast(float, k_top) / 127.0f : NAN;
-        const float v_scale = v_fin ? __builtin_bit_cast(float, v_top) / 127.0f : NAN;
+        const float k_scale = k_fin ? __builtin_bit_cast(float, k_top) * (1.0f / 127.0f) : NAN;
+        const float v_scale = v_fin ? __builtin_bit_cast(float, v_top) * (1.0f / 127.0f) : NAN;
 #pragma unroll
         for (int p = 0; p < kPass; ++p) {
             if (!in_head) break;

@@ -80,8 +80,8 @@ extern "C" {
  *     position t and dim 4 e + j (j < 4), with w = e + (t % 2) * head_dim / 4, at byte 1024 (w / 16) + 256 (t / 4 % 4) +
  *     16 (w % 16) + 8 (t / 16) + 4 (t / 2 % 2) + j.  Then the two f32 scales, the keys' and the values', and 8 bytes
  *     that nothing reads or writes.
- *     scale = amax / 127 over the 32 x head_dim values, code = clamp(round-to-even(x / scale), -127, 127), 0 where
- *     the scale is 0; a block with a value that is not finite has scale NaN and codes 0.
+ *     scale = amax * (1.0f / 127.0f) over the 32 x head_dim values, code = clamp(round-to-even(x / scale), -127, 127),
+ *     0 where the scale is 0; a block with a value that is not finite has scale NaN and codes 0.
  *   - recent holds the last positions in f32: [seq][key head][keys, values][64][head_dim], position p in row p % 64.
  *     The open block (the positions after the last complete block) is read from there.
  * So what a position's code is does not depend on whether its block came as a prompt or token by token, and

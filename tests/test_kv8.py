@@ -55,7 +55,7 @@ def quantize(x):
     top = np.abs(x).max()
     if not np.isfinite(top):
         return np.zeros(x.shape, np.int8), np.float32(np.nan)
-    s = np.float32(top) / np.float32(127)
+    s = np.float32(top) * (np.float32(1) / np.float32(127))
     if s == 0:
         return np.zeros(x.shape, np.int8), s
     return np.clip(np.rint(x / s), -127, 127).astype(np.int8), s
