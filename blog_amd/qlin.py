@@ -281,6 +281,20 @@ def dequantize(qtype, src, out, n, f16=True):
 KV8_BLOCK, KV8_RECENT = 32, 64
 
 
+# (call() looks at every argument twice: 2 to 4 us of a launch of 5)
+def _at(t):
+    return t if t is None or t.__class__ is int else t.data_ptr()
+
+
+def _lib_of():
+    return _lib or lib()
+
+
+def _done(name, rc):
+    if rc != 0:
+        raise QlinError(name, rc)
+
+
 def kv8_record_bytes(head_dim):
     """Bytes of one block of one key head in a page."""
     return 64 * head_dim + 16
@@ -335,18 +349,21 @@ class Kv8Cache:
 
 def qk_norm_rope_store_kv(how, q, q_stride, k, k_stride, v, v_stride, q_out, kc, vc, rows, n_heads, kv_heads, head_dim,
                           max_seq, start_pos):
-    call("qlin_launch_qk_norm_rope_store_kv", how.address, q, q_stride, k, k_stride, v, v_stride, q_out, kc, vc, rows,
-         n_heads, kv_heads, head_dim, max_seq, start_pos)
+    _done("qlin_launch_qk_norm_rope_store_kv", _lib_of().qlin_launch_qk_norm_rope_store_kv(
+        how.address, _at(q), q_stride, _at(k), k_stride, _at(v), v_stride, _at(q_out), _at(kc), _at(vc), rows, n_heads,
+        kv_heads, head_dim, max_seq, _at(start_pos)))
 
 
 def qk_norm_rope_store_kv8(how, cache, q, q_stride, k, k_stride, v, v_stride, q_out, rows, n_heads, start_pos,
                            n_rows=None):
-    call("qlin_launch_qk_norm_rope_store_kv8", how.address, cache.address, q, q_stride, k, k_stride, v, v_stride, q_out,
-         rows, n_heads, start_pos, n_rows)
+    _done("qlin_launch_qk_norm_rope_store_kv8", _lib_of().qlin_launch_qk_norm_rope_store_kv8(
+        how.address, cache.address, _at(q), q_stride, _at(k), k_stride, _at(v), v_stride, _at(q_out), rows, n_heads,
+        _at(start_pos), _at(n_rows)))
 
 
 def kv8_read(cache, first, lens, count, k_out, v_out):
-    call("qlin_launch_kv8_read", cache.address, first, lens, count, k_out, v_out)
+    _done("qlin_launch_kv8_read", _lib_of().qlin_launch_kv8_read(cache.address, _at(first), _at(lens), count, _at(k_out),
+                                                                 _at(v_out)))
 
 
 def attend_kv8_workspace_bytes(n_seqs, rows, n_heads, kv_heads, head_dim, blocks_per_seq):
@@ -355,8 +372,9 @@ def attend_kv8_workspace_bytes(n_seqs, rows, n_heads, kv_heads, head_dim, blocks
 
 def attend_kv8(cache, q, attn, rows, n_heads, start_pos, n_rows, softmax_scale, workspace):
     """workspace: a uint8 tensor of at least attend_kv8_workspace_bytes(...) (None where that is 0)."""
-    call("qlin_launch_attend_kv8", cache.address, q, attn, rows, n_heads, start_pos, n_rows, softmax_scale, workspace,
-         0 if workspace is None else workspace.numel())
+    _done("qlin_launch_attend_kv8", _lib_of().qlin_launch_attend_kv8(
+        cache.address, _at(q), _at(attn), rows, n_heads, _at(start_pos), _at(n_rows), softmax_scale, _at(workspace),
+        0 if workspace is None else workspace.numel()))
 
 
 def logits_controls_scratch_bytes(rows, vocab):
@@ -368,9 +386,10 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
     """Penalties, biases and a mask on logits [rows, >= vocab] into out (which may be logits), and the greedy picks.
     history [rows, max_history], bias_ids / bias_values [rows, max_bias] and mask [rows, words] (32 tokens a word) are
     2-D and contiguous; scratch: a uint8 tensor of logits_controls_scratch_bytes(...), needed with picks."""
-    a = LogitsControlsArgs(ptr(history), ptr(history_lens), ptr(repetition), ptr(frequency), ptr(presence),
-                           ptr(bias_ids), ptr(bias_values), ptr(mask), mask.shape[1] if mask is not None else 0,
+    a = LogitsControlsArgs(_at(history), _at(history_lens), _at(repetition), _at(frequency), _at(presence),
+                           _at(bias_ids), _at(bias_values), _at(mask), mask.shape[1] if mask is not None else 0,
                            history.shape[1] if history is not None else 0,
                            bias_ids.shape[1] if bias_ids is not None else 0)
-    call("qlin_launch_logits_controls", C.addressof(a), logits, logits.stride(0), out, out.stride(0), rows, vocab, picks,
-         scratch, 0 if scratch is None else scratch.numel())
+    _done("qlin_launch_logits_controls", _lib_of().qlin_launch_logits_controls(
+        C.addressof(a), logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, _at(picks),
+        _at(scratch), 0 if scratch is None else scratch.numel()))
