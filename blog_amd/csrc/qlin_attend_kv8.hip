@@ -4,20 +4,28 @@
 // over the positions: m is the largest score so far, and the sums are scaled down when it grows.
 //
 // The 16 query rows of a tile are (row, head of the key head's group) pairs, so that every code is read once for all
-// of a group's heads.  Scores are taken as S^T = K q^T and outputs as O^T = V^T P^T on v_mfma_f32_16x16x32_bf16: lane
+// of a group's heads.  Scores are taken as S^T = K q^T and outputs as O^T = V^T P^T on v_mfma_f32_16x16x32_f16: lane
 // (n, g) then holds, of query row n, the probabilities of positions 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3 of a block,
-// which is what it supplies as the second product's operand (the value codes are stored in that order), so that
-// probabilities go from one product to the next without leaving their lane.  Codes are exact in bf16; q (times
-// softmax_scale log2(e), one rounding) and p are taken in three exact bf16 parts (qlin_bf16x3.hpp).  A block's own sum
-// joins the output by one fma with its scale: a chain through the MFMA's C would be cut off downwards each time.
+// which is what it supplies as the second product's operand, so that probabilities go from one product to the next
+// without leaving their lane.
+//
+// Operands: a code is exact in fp16 (one v_cvt_f16_i16 with byte and half selects).  q (times
+// softmax_scale log2(e), one rounding, and a power of two that brings its row's largest value to 2^14 .. 2^15) and p
+// (times 2^11) are fp16 pairs hi + lo, 22 bits and a sign, so their products with a code are exact and a score is off by
+// 2^-23 of its terms.  What is lost besides lies below 2^-39 of a row's largest q, or 2^-36 of its largest p: a
+// position of less weight than that adds nothing.  (Three bf16 parts, which lose nothing, took 3 products instead of 2.)
+// A block's own sum joins the output by one fma with the block's scale: a chain of blocks through the MFMA's C would be
+// cut off downwards each time.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "qlin.h"
-#include "qlin_bf16x3.hpp"
 #include "qlin_internal.hpp"
 #include "qlin_kv8.hpp"
+#include "qlin_mfma.hpp"
 
 namespace qlin {
 
@@ -28,6 +36,74 @@ namespace {
 
 constexpr int kWaves = 4, kTile = 16;
 constexpr int kMinItems = 8;  // blocks of a split, at least
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4 mfma16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// The fp16 values of 4 codes, as two pairs (a's byte LA and b's LB, then c's LC and d's LD).  A half written by itself may
+// not be read by the next instruction (one wait state): the two pairs alternate, and a wait ends them.
+#define QLIN_CODES4(NAME, LA, LB, LC, LD)                                                                            \
+    __device__ __forceinline__ void NAME(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t &x, uint32_t &y) { \
+        asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_" #LA "\n\t"         \
+            "v_cvt_f16_i16_sdwa %1, sext(%4) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_" #LC "\n\t"         \
+            "v_cvt_f16_i16_sdwa %0, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_" #LB "\n\t"    \
+            "v_cvt_f16_i16_sdwa %1, sext(%5) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_" #LD "\n\t"    \
+            "s_nop 0"                                                                                                \
+            : "=&v"(x), "=&v"(y)                                                                                     \
+            : "v"(a), "v"(b), "v"(c), "v"(d));                                                                       \
+    }
+QLIN_CODES4(codes_0123, 0, 1, 2, 3)
+QLIN_CODES4(codes_0, 0, 0, 0, 0)
+QLIN_CODES4(codes_1, 1, 1, 1, 1)
+QLIN_CODES4(codes_2, 2, 2, 2, 2)
+QLIN_CODES4(codes_3, 3, 3, 3, 3)
+#undef QLIN_CODES4
+// the 8 codes of two dwords, in order
+__device__ __forceinline__ u32x4 f16_of_8(uint32_t a, uint32_t b) {
+    uint32_t v[4];
+    codes_0123(a, a, a, a, v[0], v[1]);
+    codes_0123(b, b, b, b, v[2], v[3]);
+    return u32x4{v[0], v[1], v[2], v[3]};
+}
+// byte J of a and b, then of c and d
+template <int J>
+__device__ __forceinline__ uint2 f16_of_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    uint2 v;
+    if constexpr (J == 0) codes_0(a, b, c, d, v.x, v.y);
+    else if constexpr (J == 1) codes_1(a, b, c, d, v.x, v.y);
+    else if constexpr (J == 2) codes_2(a, b, c, d, v.x, v.y);
+    else codes_3(a, b, c, d, v.x, v.y);
+    return v;
+}
+// hi + lo of two values, each an fp16 pair
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const f32x2 v = {a, b};
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+    f32x2 r;
+    float r0, r1;  // v - hi, exact
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(b));
+    r = f32x2{r0, r1};
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, f16x2));
+}
+__device__ __forceinline__ void split2(const f32x4 &a, const f32x4 &b, u32x4 &hi, u32x4 &lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 &v = i < 2 ? a : b;
+        uint32_t h, l;
+        split2(v[2 * (i & 1)], v[2 * (i & 1) + 1], h, l);
+        hi[i] = h;
+        lo[i] = l;
+    }
+}
+// value j of 8 packed fp16 values
+__device__ __forceinline__ float f16_at(const u32x4 &v, int j) {
+    const uint32_t w = v[j >> 1];
+    return f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xffffu);
+}
 
 // over the four lane groups of a query row
 __device__ __forceinline__ float groups_max(float v) {
@@ -42,20 +118,18 @@ __device__ __forceinline__ float groups_sum(float v) {
     const auto b = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
     return __builtin_bit_cast(float, static_cast<uint32_t>(b[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(b[1]));
 }
-// byte j of a dword of codes
-__device__ __forceinline__ float code_at(uint32_t w, int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// What a tile of query rows sees: blocks [0, blocks) and `tails` 16-position tiles of the open block.
+// What `count` query rows from p0 on see: blocks [0, blocks) and `tails` 16-position tiles of the open block.
 struct Span {
-    int first, last;  // last position seen by the tile's first and last rows (-1: none)
+    int first, last;  // last position seen by the first and the last of the rows (-1: none)
     int done;         // the cache's complete blocks
     int blocks, tails;
     __device__ __forceinline__ int items() const { return blocks + tails; }
 };
-__device__ __forceinline__ Span span_of(const Kv8Rows &w, int p0, int group) {
+__device__ __forceinline__ Span span_of(const Kv8Rows &w, int p0, int count, int group) {
     Span s;
-    const int r0 = p0 / group, r1 = min((p0 + kTile - 1) / group, w.rows - 1);
+    const int r0 = p0 / group, r1 = min((p0 + count - 1) / group, w.rows - 1);
     s.first = min(w.start + r0, w.len - 1);
     s.last = min(w.start + r1, w.len - 1);
     s.done = w.len / kKv8Block;
@@ -64,10 +138,49 @@ __device__ __forceinline__ Span span_of(const Kv8Rows &w, int p0, int group) {
     s.tails = s.last >= open ? (s.last - open) / 16 + 1 : 0;
     return s;
 }
-// items of a split, and how many splits have some
+// items of a split
 __device__ __forceinline__ int items_per_split(int items, int splits) { return max(kMinItems, (items + splits - 1) / splits); }
 
+// A tile's queries as operands: value j of slot i is dim 32 i + 8 g + j of query row n, times 1 / inv.
+template <int HD>
+struct Queries {
+    u32x4 hi[HD / 32], lo[HD / 32];
+    float inv;
+    int seen;  // the last position that query row n sees
+    __device__ __forceinline__ void load(const float *row, float q_scale) {
+        f32x4 v[HD / 32][2];
+        uint32_t top = 0;  // (integers: a value that is not finite is above all others)
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v[i][h] = *reinterpret_cast<const f32x4 *>(row + 32 * i + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[i][h][e] *= q_scale;
+                    top = max(top, __float_as_uint(v[i][h][e]) & 0x7fffffffu);
+                }
+            }
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
+        const int up = min(127 + 14 - static_cast<int>(top >> 23), 100);  // at most 2^100
+        const float scale = top < 0x7f800000u ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : NAN;
+        inv = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][h][e] *= scale;
+            split2(v[i][0], v[i][1], hi[i], lo[i]);
+        }
+    }
+};
+
 // One wave's running sums of a tile.
+// Probabilities are 2^(s - m + kUp), and m is left as it is until a score is kSlack above it: after the first few blocks
+// it rarely changes, where the exact maximum of one row in 16 changes in most of a prompt's blocks (47 instructions).
+constexpr float kUp = 11.0f, kSlack = 4.0f;  // (2^15 at most, in fp16)
 template <int HD>
 struct Sums {
     static constexpr int NT = (HD + 63) / 64;
@@ -81,10 +194,10 @@ struct Sums {
         m = -INFINITY;
         l = 0.0f;
     }
-    // the maximum becomes that of the tile's scores too; returns what is subtracted
+    // the maximum becomes at least that of the tile's scores; returns what is added to the scores
     __device__ __forceinline__ float raise(float mx) {
         mx = fmaxf(m, groups_max(mx));
-        if (__any(mx > m)) {  // uniform
+        if (__any(mx > m + kSlack)) {  // uniform
             const float al = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
             l *= al;
 #pragma unroll
@@ -95,179 +208,93 @@ struct Sums {
                     for (int r = 0; r < 4; ++r) o[i][j][r] *= al;
             m = mx;
         }
-        return m == -INFINITY ? 0.0f : m;
+        return m == -INFINITY ? 0.0f : kUp - m;
     }
-};
-
-// A workgroup of 4 waves per (tile, sequence, key head, split of the positions); its waves take the split's blocks
-// in turn, each with sums of its own, which meet in LDS.
-template <int HD>
-__global__ __launch_bounds__(64 * kWaves) void attend_kv8_kernel(Kv8View c, const float *__restrict__ q,
-                                                                 float *__restrict__ out, int rows, int n_heads,
-                                                                 const int *__restrict__ start_pos,
-                                                                 const int *__restrict__ n_rows, float q_scale, int tiles,
-                                                                 int splits, float *__restrict__ part) {
-    constexpr int NC = HD / 32, NT = Sums<HD>::NT;
-    __shared__ float s_o[kWaves][kTile][HD + 4];
-    __shared__ float s_m[kWaves][kTile], s_l[kWaves][kTile];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % splits;
-    id /= splits;
-    const int kh = id % c.kv;
-    id /= c.kv;
-    const int tile = id % tiles, seq = id / tiles;
-    const int group = n_heads / c.kv, p0 = tile * kTile;
-    const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, c.per * kKv8Block);
-    const int pairs = w.rows * group;
-    if (p0 >= pairs) return;
-    const Span sp = span_of(w, p0, group);
-    const int per = items_per_split(sp.items(), splits), used = max(1, (sp.items() + per - 1) / per);
-    if (split >= used) return;
-
-    const int pair = min(p0 + n, pairs - 1);
-    const int seen = min(w.start + pair / group, w.len - 1);  // the last position of this lane's query row
-    u32x4 qp[3][NC];
-    {
-        const float *src = q + ((static_cast<size_t>(seq) * rows + pair / group) * n_heads + kh * group + pair % group) * HD + 8 * g;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            f32x4 a = *reinterpret_cast<const f32x4 *>(src + 32 * i), b = *reinterpret_cast<const f32x4 *>(src + 32 * i + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[e] *= q_scale;
-                b[e] *= q_scale;
-            }
-            split3(a, b, qp[0][i], qp[1][i], qp[2][i]);
-        }
-    }
-    Sums<HD> t;
-    t.clear();
-    const int end = min((split + 1) * per, sp.items());
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-
-    for (int it = split * per + wave; it < min(end, sp.blocks); it += kWaves) {  // uniform
-        const int page = c.page(seq, it);
-        if (page < 0) continue;
-        const uint8_t *rec = c.record(page, kh, kv8_record_bytes(HD));
-        const float2 scale = *reinterpret_cast<const float2 *>(rec + 64 * HD);
-        u32x4 kc[NC], vc[NT][2];
-#pragma unroll
-        for (int i = 0; i < NC; ++i) kc[i] = *reinterpret_cast<const u32x4 *>(rec + 1024 * i + 16 * lane);
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int odd = 0; odd < 2; ++odd)  // dims 64 i + 4n .. + 3 of positions 4g + odd, + 2, 16 + 4g + odd, + 2
-                vc[i][odd] = 64 * (i + 1) <= HD || 64 * i + 4 * n < HD
-                                 ? *reinterpret_cast<const u32x4 *>(rec + kv8_value_byte(4 * g + odd, 64 * i + 4 * n, HD))
-                                 : u32x4{0u, 0u, 0u, 0u};
-        f32x4 hi[2] = {zero, zero}, lo[2] = {zero, zero};
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const u32x4 a = bf16_of_i8(kc[i][2 * u], kc[i][2 * u + 1]);
-                hi[u] = mfma(a, qp[0][i], hi[u]);
-                lo[u] = mfma(a, qp[1][i], lo[u]);
-                lo[u] = mfma(a, qp[2][i], lo[u]);
-            }
-        }
-        f32x4 s[2];
+    // a block's sums S (positions block * 32 + 16 u + 4 g + r) to probabilities, as operands
+    __device__ __forceinline__ void weigh(f32x4 (&s)[2], float f, bool edge, int block, int g, int seen, u32x4 &hi, u32x4 &lo) {
         float mx = -INFINITY;
-        const int at = it * kKv8Block + 4 * g;
-        const bool edge = it * kKv8Block + kKv8Block - 1 > sp.first;  // uniform
+        if (edge) {  // uniform
+            asm volatile("");  // (a branch: as selects these 30 instructions would go with every block)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float v = s[u][r] * f;
+                    s[u][r] = block * kKv8Block + 16 * u + 4 * g + r > seen ? -INFINITY : v;
+                    mx = fmaxf(mx, s[u][r]);
+                }
+            f = 1.0f;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][r]);
+            mx *= f;  // (f > 0, 0 with sums of 0, or NaN)
+        }
+        const float add = raise(mx);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float v = (hi[u][r] + lo[u][r]) * scale.x;
-                if (edge && at + 16 * u + r > seen) v = -INFINITY;
-                s[u][r] = v;
-                mx = fmaxf(mx, v);
+                s[u][r] = exp2_fast(fmaf(s[u][r], f, add));
+                l += s[u][r];
             }
-        const float m = t.raise(mx);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[u][r] = exp2_fast(s[u][r] - m);
-                t.l += s[u][r];
-            }
-        u32x4 ph, pm, pl;
-        split3(s[0], s[1], ph, pm, pl);
-        // a scale that is not finite meets only the rows that see one of the block's positions
-        const float vs = edge && it * kKv8Block > seen ? 0.0f : scale.y;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 a;
-#pragma unroll
-                for (int h = 0; h < 4; ++h)  // positions 4g, 4g + 1; 4g + 2, + 3; 16 + 4g, + 1; 16 + 4g + 2, + 3
-                    a[h] = bf16_tops(code_at(vc[i][0][h], j), code_at(vc[i][1][h], j));
-                const f32x4 x = mfma(a, ph, zero);
-                f32x4 y = mfma(a, pm, zero);
-                y = mfma(a, pl, y);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) t.o[i][j][r] = fmaf(x[r] + y[r], vs, t.o[i][j][r]);
-            }
+        split2(s[0], s[1], hi, lo);
     }
-
-    // The open block, 16 positions at a time, from the ring: f32 on v_mfma_f32_16x16x4_f32, dims and positions in the
-    // same lanes as above.
-    for (int it = max(split * per, sp.blocks); it < end; ++it) {
-        if ((it - split * per) % kWaves != wave) continue;  // uniform
-        if (c.page(seq, sp.done) < 0) continue;
-        const int base = sp.done * kKv8Block + 16 * (it - sp.blocks);
-        const float *kr = c.ring(seq, kh, 0, HD), *vr = c.ring(seq, kh, 1, HD);
+    __device__ __forceinline__ void join(int i, int j, const f32x4 &t, float vs) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[i][j][r] = fmaf(t[r], vs, o[i][j][r]);
+    }
+    // 16 positions of the open block from base on, from the ring: f32 on v_mfma_f32_16x16x4_f32, dims and positions in
+    // the same lanes as above.  kr, vr: the ring's keys and values; first: the last position that every row sees.
+    __device__ __forceinline__ void tail(const Queries<HD> &q, const float *kr, const float *vr, int base, int len, int first,
+                                         int n, int g) {
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
         const int mine = base + n;
         const float *krow = kr + static_cast<size_t>(mine % kKv8Recent) * HD + 8 * g;
         f32x4 acc[4] = {zero, zero, zero, zero};
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
+        for (int i = 0; i < HD / 32; ++i) {
             f32x4 x[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) x[h] = mine < w.len ? *reinterpret_cast<const f32x4 *>(krow + 32 * i + 4 * h) : zero;
+            for (int h = 0; h < 2; ++h) x[h] = mine < len ? *reinterpret_cast<const f32x4 *>(krow + 32 * i + 4 * h) : zero;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float qv = (bf16_at(qp[0][i], j) + bf16_at(qp[1][i], j)) + bf16_at(qp[2][i], j);  // exact
-                acc[j % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j / 4][j % 4], qv, acc[j % 4], 0, 0, 0);
-            }
+            for (int e = 0; e < 8; ++e)
+                acc[e % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e / 4][e % 4], f16_at(q.hi[i], e) + f16_at(q.lo[i], e), acc[e % 4], 0, 0, 0);
         }
         f32x4 s;
         float mx = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float v = (acc[0][r] + acc[1][r]) + (acc[2][r] + acc[3][r]);
-            s[r] = base + 4 * g + r > seen ? -INFINITY : v;
+            const float v = ((acc[0][r] + acc[1][r]) + (acc[2][r] + acc[3][r])) * q.inv;
+            s[r] = base + 4 * g + r > q.seen ? -INFINITY : v;
             mx = fmaxf(mx, s[r]);
         }
-        const float m = t.raise(mx);
+        const float add = raise(mx);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[r] = exp2_fast(s[r] - m);
-            t.l += s[r];
+            s[r] = exp2_fast(s[r] + add);
+            l += s[r];
         }
-        bool odd = false;  // a value that is not finite, at a position that some row does not see
-        f32x4 v[4][NT];  // dims 64 i + 4n .. + 3 of position 4g + r
+        bool odd = false;  // a value that is not finite
+        f32x4 v[4][NT];    // dims 64 i + 4n .. + 3 of position 4g + r
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int pos = base + 4 * g + r;
             const float *vrow = vr + static_cast<size_t>(pos % kKv8Recent) * HD + 4 * n;
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                v[r][i] = pos < w.len && 64 * i + 4 * n < HD ? *reinterpret_cast<const f32x4 *>(vrow + 64 * i) : zero;
+                v[r][i] = pos < len && 64 * i + 4 * n < HD ? *reinterpret_cast<const f32x4 *>(vrow + 64 * i) : zero;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) odd |= !isfinite(v[r][i][j]);
             }
         }
-        if (base + 15 > sp.first && __any(odd)) {  // uniform: 0 times that value would be NaN
-            for (int j = 0; j < 16 && base + j < w.len; ++j) {
-                const int from = 16 * (j / 4) + n;
-                float p = j % 4 == 0 ? s[0] : j % 4 == 1 ? s[1] : j % 4 == 2 ? s[2] : s[3];
-                p = __shfl(p, from, 64);
-                if (base + j <= seen) {
-                    const float *vrow = vr + static_cast<size_t>((base + j) % kKv8Recent) * HD;
+        if (base + 15 > first && __any(odd)) {  // uniform: 0 times that value, for a row that does not see it, would be NaN
+            for (int e = 0; e < 16 && base + e < len; ++e) {
+                float p = e % 4 == 0 ? s[0] : e % 4 == 1 ? s[1] : e % 4 == 2 ? s[2] : s[3];
+                p = __shfl(p, 16 * (e / 4) + n, 64);
+                if (base + e <= q.seen) {
+                    const float *vrow = vr + static_cast<size_t>((base + e) % kKv8Recent) * HD;
 #pragma unroll
                     for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -275,7 +302,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kv8_kernel(Kv8View c, cons
                             const int d = 64 * i + 16 * g + 4 * r;
                             const f32x4 y = d < HD ? *reinterpret_cast<const f32x4 *>(vrow + d) : zero;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) t.o[i][e][r] = fmaf(p, y[e], t.o[i][e][r]);
+                            for (int j = 0; j < 4; ++j) o[i][j][r] = fmaf(p, y[j], o[i][j][r]);
                         }
                 }
             }
@@ -288,72 +315,230 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kv8_kernel(Kv8View c, cons
 #pragma unroll
                     for (int r = 0; r < 4; ++r) x = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i][j], s[r], x, 0, 0, 0);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) t.o[i][j][r] += x[r];
+                    for (int r = 0; r < 4; ++r) o[i][j][r] += x[r];
                 }
         }
     }
+};
 
-    t.l = groups_sum(t.l);
-    if (g == 0) {
-        s_m[wave][n] = t.m;
-        s_l[wave][n] = t.l;
+// A workgroup of 4 waves per (RT tiles of 16 query rows, sequence, key head, split of the positions); its waves take the
+// split's blocks in turn, each with sums of its own, which meet in LDS.  A wave knows the pages of its next 64 blocks,
+// requests a block's keys while it weighs the values of the one before, and turns codes into operands for its RT tiles
+// in registers: there is no barrier before the end.
+// Few rows (RT = 1): bound by the latency of a wave's few blocks, and by the codes' bytes.  Many (RT = 2): bound by the
+// VALU; of a tile's 32 x 16 scores, 8 a lane, each costs an fma, an exp, a sum and 2 instructions for its operands,
+// then 4 fmas for 64 of its values, and half of the codes' 128.  (A workgroup that turned a block's codes once, into
+// LDS, for 64 rows took half of these, but one block after the other: the longest row's time, 86 us for 2011 rows of 28
+// heads, was all of it.)
+template <int HD, int RT>
+__global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, const float *__restrict__ q,
+                                                                    float *__restrict__ out, int rows, int n_heads,
+                                                                    const int *__restrict__ start_pos,
+                                                                    const int *__restrict__ n_rows, float q_scale, int macros,
+                                                                    int splits, float *__restrict__ part) {
+    constexpr int NC = HD / 32, NT = Sums<HD>::NT, kRows = RT * kTile;
+    __shared__ float s_o[kWaves][kTile][HD + 4];
+    __shared__ float s_m[kWaves][kTile], s_l[kWaves][kTile];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    // (neighbours in the grid: splits, then the key heads, whose codes so stay in their XCD's L2; the longest rows first)
+    int id = blockIdx.x;
+    const int split = id % splits;
+    id /= splits;
+    const int kh = id % c.kv;
+    id /= c.kv;
+    const int macro = macros - 1 - id % macros, seq = id / macros;
+    const int group = n_heads / c.kv, p0 = macro * kRows;
+    const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, c.per * kKv8Block);
+    const int pairs = w.rows * group;
+    if (p0 >= pairs) return;
+    const Span sp = span_of(w, p0, kRows, group);
+    const int per = items_per_split(sp.items(), splits), used = max(1, (sp.items() + per - 1) / per);
+    if (split >= used) return;
+    const int end = min((split + 1) * per, sp.items());
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr size_t kRec = kv8_record_bytes(HD);
+
+    // this wave's blocks: b0, b0 + kWaves, ...; lane i holds the page of the i-th of the next 64
+    const int b0 = split * per + wave, b1 = min(end, sp.blocks);
+    const int mine = b0 < b1 ? (b1 - b0 + kWaves - 1) / kWaves : 0;  // uniform
+    int pages = lane < mine ? c.page(seq, b0 + kWaves * lane) : -1;
+
+    u32x4 kc[NC], vc[NT][2];
+    float2 scale;
+    auto load_k = [&](int page) {
+        if (page < 0) return;
+        const uint8_t *rec = c.record(page, kh, kRec);
+        scale = *reinterpret_cast<const float2 *>(rec + 64 * HD);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) kc[i] = *reinterpret_cast<const u32x4 *>(rec + 1024 * i + 16 * lane);
+    };
+    auto load_v = [&](int page) {
+        if (page < 0) return;
+        const uint8_t *rec = c.record(page, kh, kRec);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd)  // dims 64 i + 4n .. + 3 of positions 4g + odd, + 2, 16 + 4g + odd, + 2
+                vc[i][odd] = 64 * (i + 1) <= HD || 64 * i + 4 * n < HD
+                                 ? *reinterpret_cast<const u32x4 *>(rec + kv8_value_byte(4 * g + odd, 64 * i + 4 * n, HD))
+                                 : u32x4{0u, 0u, 0u, 0u};
+    };
+    int page = __builtin_amdgcn_readlane(pages, 0);
+    load_k(page);
+    load_v(page);
+    Queries<HD> qs[RT];
+    Sums<HD> t[RT];
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const int pair = min(p0 + k * kTile + n, pairs - 1);
+        qs[k].seen = min(w.start + pair / group, w.len - 1);
+        qs[k].load(q + ((static_cast<size_t>(seq) * rows + pair / group) * n_heads + kh * group + pair % group) * HD + 8 * g, q_scale);
+        t[k].clear();
     }
+
+    for (int i0 = 0; i0 < mine; ++i0) {  // uniform
+        const int block = b0 + kWaves * i0;
+        if ((i0 + 1) % 64 == 0) pages = i0 + 1 + lane < mine ? c.page(seq, block + kWaves * (1 + lane)) : -1;
+        const int next = i0 + 1 < mine ? __builtin_amdgcn_readlane(pages, (i0 + 1) % 64) : -1;
+        if (page >= 0) {
+            const float ks = scale.x, vscale = scale.y;
+            f32x4 s[RT][2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+            for (int k = 0; k < RT; ++k) s[k][0] = s[k][1] = zero;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = 64 * i + 16 * g + 4 * r;
-            if (d < HD) *reinterpret_cast<f32x4 *>(&s_o[wave][n][d]) = f32x4{t.o[i][0][r], t.o[i][1][r], t.o[i][2][r], t.o[i][3][r]};
-        }
-    __syncthreads();
-    for (int e = threadIdx.x; e < kTile * (HD / 4); e += 64 * kWaves) {
-        const int row = e / (HD / 4), d = 4 * (e % (HD / 4));
-        if (p0 + row >= pairs) continue;
-        float mx = -INFINITY;
+            for (int i = 0; i < NC; ++i) {
+                const u32x4 a0 = f16_of_8(kc[i][0], kc[i][1]), a1 = f16_of_8(kc[i][2], kc[i][3]);
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, s_m[i][row]);
-        f32x4 num = zero;
-        float den = 0.0f;
+                for (int k = 0; k < RT; ++k) {
+                    s[k][0] = mfma16(a0, qs[k].hi[i], s[k][0]);
+                    s[k][1] = mfma16(a1, qs[k].hi[i], s[k][1]);
+                }
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            const float mi = s_m[i][row], li = s_l[i][row];
-            if (mi == -INFINITY && li == 0.0f) continue;                    // no position of this row
-            const float f = mi == -INFINITY ? 1.0f : exp2_fast(mi - mx);  // (-inf: then li is NaN)
-            const f32x4 o = *reinterpret_cast<const f32x4 *>(&s_o[i][row][d]);
+                for (int k = 0; k < RT; ++k) {
+                    s[k][0] = mfma16(a0, qs[k].lo[i], s[k][0]);
+                    s[k][1] = mfma16(a1, qs[k].lo[i], s[k][1]);
+                }
+            }
+            load_k(next);
+            const bool edge = block * kKv8Block + kKv8Block - 1 > sp.first;  // uniform
+            u32x4 hi[RT], lo[RT];
+            float vs[RT];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) num[r] = fmaf(o[r], f, num[r]);
-            den = fmaf(li, f, den);
-        }
-        if (used == 1) {
-            const int pr = p0 + row;
-            f32x4 o = zero;
-            if (den != 0.0f)
+            for (int k = 0; k < RT; ++k) {
+                t[k].weigh(s[k], ks * qs[k].inv, edge, block, g, qs[k].seen, hi[k], lo[k]);
+                // a scale that is not finite meets only the rows that see one of the block's positions
+                vs[k] = edge && block * kKv8Block > qs[k].seen ? 0.0f : vscale;
+            }
+            auto values = [&](int i, auto jc) {  // two operands, whose chains are independent
+                constexpr int J = decltype(jc)::value;
+                // positions 4g, 4g + 1; 4g + 2, + 3; 16 + 4g, + 1; 16 + 4g + 2, + 3
+                const uint2 a0 = f16_of_bytes<J>(vc[i][0][0], vc[i][1][0], vc[i][0][1], vc[i][1][1]);
+                const uint2 a1 = f16_of_bytes<J>(vc[i][0][2], vc[i][1][2], vc[i][0][3], vc[i][1][3]);
+                const uint2 b0 = f16_of_bytes<J + 1>(vc[i][0][0], vc[i][1][0], vc[i][0][1], vc[i][1][1]);
+                const uint2 b1 = f16_of_bytes<J + 1>(vc[i][0][2], vc[i][1][2], vc[i][0][3], vc[i][1][3]);
+                const u32x4 a = {a0.x, a0.y, a1.x, a1.y}, b = {b0.x, b0.y, b1.x, b1.y};
+                f32x4 x[RT][2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] = num[r] / den;
-            *reinterpret_cast<f32x4 *>(out + ((static_cast<size_t>(seq) * rows + pr / group) * n_heads + kh * group + pr % group) * HD + d) = o;
+                for (int k = 0; k < RT; ++k) {
+                    x[k][0] = mfma16(a, hi[k], zero);
+                    x[k][1] = mfma16(b, hi[k], zero);
+                }
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+                    x[k][0] = mfma16(a, lo[k], x[k][0]);
+                    x[k][1] = mfma16(b, lo[k], x[k][1]);
+                }
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+                    t[k].join(i, J, x[k][0], vs[k]);
+                    t[k].join(i, J + 1, x[k][1], vs[k]);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                values(i, std::integral_constant<int, 0>());
+                values(i, std::integral_constant<int, 2>());
+            }
+            load_v(next);
         } else {
-            // [tile of this launch][split][row]: HD sums, the maximum, the denominator
-            float *dst = part + ((static_cast<size_t>(blockIdx.x / splits) * splits + split) * kTile + row) * (HD + 4);
-            *reinterpret_cast<f32x4 *>(dst + d) = num;
-            if (d == 0) {
-                dst[HD] = mx;
-                dst[HD + 1] = den;
+            load_k(next);
+            load_v(next);
+        }
+        page = next;
+    }
+    for (int it = max(split * per, sp.blocks); it < end; ++it)
+        if ((it - split * per) % kWaves == wave && c.page(seq, sp.done) >= 0)  // uniform
+#pragma unroll
+            for (int k = 0; k < RT; ++k)
+                t[k].tail(qs[k], c.ring(seq, kh, 0, HD), c.ring(seq, kh, 1, HD), sp.done * kKv8Block + 16 * (it - sp.blocks), w.len, sp.first, n, g);
+
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const int pk = p0 + k * kTile;
+        if (k > 0) __syncthreads();  // (the tile before is read)
+        t[k].l = groups_sum(t[k].l);
+        if (g == 0) {
+            s_m[wave][n] = t[k].m;
+            s_l[wave][n] = t[k].l;
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = 64 * i + 16 * g + 4 * r;
+                if (d < HD) *reinterpret_cast<f32x4 *>(&s_o[wave][n][d]) = f32x4{t[k].o[i][0][r], t[k].o[i][1][r], t[k].o[i][2][r], t[k].o[i][3][r]};
+            }
+        __syncthreads();
+        for (int e = threadIdx.x; e < kTile * (HD / 4); e += 64 * kWaves) {
+            const int row = e / (HD / 4), d = 4 * (e % (HD / 4));
+            if (pk + row >= pairs) continue;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, s_m[i][row]);
+            f32x4 num = zero;
+            float den = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                const float mi = s_m[i][row], li = s_l[i][row];
+                if (mi == -INFINITY && li == 0.0f) continue;                    // no position of this row
+                const float f = mi == -INFINITY ? 1.0f : exp2_fast(mi - mx);  // (-inf: then li is NaN)
+                const f32x4 o = *reinterpret_cast<const f32x4 *>(&s_o[i][row][d]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) num[r] = fmaf(o[r], f, num[r]);
+                den = fmaf(li, f, den);
+            }
+            if (used == 1) {
+                const int pr = pk + row;
+                f32x4 o = zero;
+                if (den != 0.0f)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = num[r] / den;
+                *reinterpret_cast<f32x4 *>(out + ((static_cast<size_t>(seq) * rows + pr / group) * n_heads + kh * group + pr % group) * HD + d) = o;
+            } else {
+                // [tile of this launch][split][row]: HD sums, the maximum, the denominator
+                const size_t tile = (static_cast<size_t>(seq) * (macros * RT) + macro * RT + k) * c.kv + kh;
+                float *dst = part + ((tile * splits + split) * kTile + row) * (HD + 4);
+                *reinterpret_cast<f32x4 *>(dst + d) = num;
+                if (d == 0) *reinterpret_cast<float2 *>(dst + HD) = make_float2(mx, den);
             }
         }
     }
 }
 
-// A workgroup per query row: the splits' sums joined.
+// A workgroup per query row: the splits' sums joined.  Each wave finds the splits' weights (a split a lane), and each
+// thread adds four dims of every C-th split, eight in flight.
 constexpr int kJoinThreads = 256;
+constexpr int kMaxSplits = 128;
 template <int HD>
 __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c, float *__restrict__ out, int rows,
                                                                        int n_heads, const int *__restrict__ start_pos,
                                                                        const int *__restrict__ n_rows, int tiles,
-                                                                       int splits, const float *__restrict__ part) {
-    constexpr int D4 = HD / 4, C = kJoinThreads / D4;
+                                                                       int macro, int splits,
+                                                                       const float *__restrict__ part) {
+    constexpr int D4 = HD / 4, C = kJoinThreads / D4, kSlots = kMaxSplits / 64;
     __shared__ f32x4 s_num[C][D4];
-    __shared__ float s_den[C];
-    const int row = blockIdx.x % kTile;
+    __shared__ float s_f[kJoinThreads / 64][kMaxSplits];
+    const int row = blockIdx.x % kTile, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned group_id = blockIdx.x / kTile;
     int id = group_id;
     const int kh = id % c.kv;
@@ -363,58 +548,93 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c
     const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, c.per * kKv8Block);
     const int pr = p0 + row;
     if (pr >= w.rows * group) return;
-    const Span sp = span_of(w, p0, group);
+    // of the rows that one workgroup took
+    const Span sp = span_of(w, p0 / macro * macro, macro, group);
     const int per = items_per_split(sp.items(), splits), used = (sp.items() + per - 1) / per;
     if (used <= 1) return;  // written already
     const float *src = part + (static_cast<size_t>(group_id) * splits * kTile + row) * (HD + 4);
     const size_t step = static_cast<size_t>(kTile) * (HD + 4);
-    float mx = -INFINITY;
-    for (int i = threadIdx.x & 63; i < used; i += 64) mx = fmaxf(mx, src[i * step + HD]);
-    mx = wave_max_dpp(mx);
     const int cls = threadIdx.x / D4, d4 = threadIdx.x % D4;
-    f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
-    float den = 0.0f;
-    if (cls < C) {
-        for (int i = cls; i < used; i += C) {
-            const float mi = src[i * step + HD], li = src[i * step + HD + 1];
-            const f32x4 o = *reinterpret_cast<const f32x4 *>(src + i * step + 4 * d4);
-            if (mi == -INFINITY && li == 0.0f) continue;
-            const float f = mi == -INFINITY ? 1.0f : exp2_fast(mi - mx);
+    f32x4 first[4];  // (requested before the weights are known)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) num[r] = fmaf(o[r], f, num[r]);
-            den = fmaf(li, f, den);
+    for (int u = 0; u < 4; ++u)
+        first[u] = cls < C && cls + u * C < used ? *reinterpret_cast<const f32x4 *>(src + (cls + u * C) * step + 4 * d4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float mi[kSlots], li[kSlots], mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+        const int i = lane + 64 * k;
+        const float2 ml = i < used ? *reinterpret_cast<const float2 *>(src + i * step + HD) : make_float2(-INFINITY, 0.0f);
+        mi[k] = ml.x;
+        li[k] = ml.y;
+        mx = fmaxf(mx, ml.x);
+    }
+    mx = wave_max_dpp(mx);
+    float den = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+        // no position of this row: nothing; a maximum of -inf otherwise: li is NaN
+        const float f = mi[k] == -INFINITY ? (li[k] == 0.0f ? 0.0f : 1.0f) : exp2_fast(mi[k] - mx);
+        s_f[wave][lane + 64 * k] = f;
+        den = fmaf(li[k], f, den);
+    }
+    den = wave_sum(den);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the wave's own row of s_f)
+    __builtin_amdgcn_wave_barrier();
+    f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (cls < C) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (cls + u * C < used) {
+                const float f = s_f[wave][cls + u * C];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) num[r] = fmaf(first[u][r], f, num[r]);
+            }
+        for (int i0 = cls + 4 * C; i0 < used; i0 += 4 * C) {
+            f32x4 o[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                o[u] = i0 + u * C < used ? *reinterpret_cast<const f32x4 *>(src + (i0 + u * C) * step + 4 * d4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float f = i0 + u * C < used ? s_f[wave][i0 + u * C] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) num[r] = fmaf(o[u][r], f, num[r]);
+            }
         }
         s_num[cls][d4] = num;
-        if (d4 == 0) s_den[cls] = den;
     }
     __syncthreads();
     if (threadIdx.x < D4) {
         f32x4 o = s_num[0][d4];
-        float l = s_den[0];
 #pragma unroll
-        for (int i = 1; i < C; ++i) {
+        for (int i = 1; i < C; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] += s_num[i][d4][r];
-            l += s_den[i];
-        }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = l != 0.0f ? o[r] / l : 0.0f;
+        for (int r = 0; r < 4; ++r) o[r] = den != 0.0f ? o[r] / den : 0.0f;
         *reinterpret_cast<f32x4 *>(out + ((static_cast<size_t>(seq) * rows + pr / group) * n_heads + kh * group + pr % group) * HD + 4 * d4) = o;
     }
 }
 
 struct Plan {
-    int64_t tiles, groups;  // tiles of a (sequence, key head), of the launch
+    int rt;                 // tiles of a wave
+    int64_t tiles, groups;  // tiles of a (sequence, key head), of the launch (padded to whole workgroups)
+    int64_t work;           // workgroups of a split
     int splits;
 };
-Plan plan_of(int n_seqs, int rows, int n_heads, int kv, int blocks) {
+Plan plan_of(int n_seqs, int rows, int n_heads, int kv, int head_dim, int blocks) {
     Plan p;
-    p.tiles = (static_cast<int64_t>(rows) * (n_heads / kv) + kTile - 1) / kTile;
-    p.groups = p.tiles * kv * n_seqs;
+    const int64_t pairs = static_cast<int64_t>(rows) * (n_heads / kv);
+    p.rt = pairs > kTile && head_dim <= 128 ? 2 : 1;  // (at 192 two tiles' sums and queries do not fit a wave's registers)
+    const int64_t macros = (pairs + p.rt * kTile - 1) / (p.rt * kTile);
+    p.tiles = macros * p.rt;
+    p.work = macros * kv * n_seqs;
+    p.groups = p.work * p.rt;
     // two workgroups for every CU, but no split of less than kMinItems blocks of the longest sequence
-    const int64_t want = p.groups > 0 ? (512 + p.groups - 1) / p.groups : 1;
+    const int64_t want = p.work > 0 ? (512 + p.work - 1) / p.work : 1;
     const int64_t most = (blocks + kMinItems) / kMinItems;
     p.splits = static_cast<int>(want < most ? want : most);
+    if (p.splits > kMaxSplits) p.splits = kMaxSplits;
     return p;
 }
 
@@ -430,7 +650,7 @@ size_t qlin_attend_kv8_workspace_bytes(int n_seqs, int rows, int n_heads, int kv
                                        int blocks_per_seq) {
     if (n_seqs <= 0 || rows <= 0 || n_heads <= 0 || kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || blocks_per_seq <= 0)
         return 0;
-    const qlin::Plan p = qlin::plan_of(n_seqs, rows, n_heads, kv_heads, blocks_per_seq);
+    const qlin::Plan p = qlin::plan_of(n_seqs, rows, n_heads, kv_heads, head_dim, blocks_per_seq);
     if (p.splits <= 1) return 0;
     return static_cast<size_t>(p.groups) * p.splits * qlin::kTile * (static_cast<size_t>(head_dim) + 4) * sizeof(float);
 }
@@ -448,8 +668,8 @@ int qlin_launch_attend_kv8(const qlin_kv8_cache *cache, const float *q, float *a
         !qlin::aligned_to(n_rows_dev, 4) || !qlin::aligned_to(workspace, 16))
         return QLIN_ERR_ALIGN;
     if (static_cast<int64_t>(rows) * (n_heads / kv) > 1 << 30) return QLIN_ERR_LIMIT;
-    const qlin::Plan p = qlin::plan_of(cache->n_seqs, rows, n_heads, kv, cache->blocks_per_seq);
-    const int64_t grid = p.groups * p.splits;
+    const qlin::Plan p = qlin::plan_of(cache->n_seqs, rows, n_heads, kv, hd, cache->blocks_per_seq);
+    const int64_t grid = p.work * p.splits;
     if (grid > (1 << 23) || p.groups * qlin::kTile > (1 << 23)) return QLIN_ERR_LIMIT;
     const size_t need = qlin_attend_kv8_workspace_bytes(cache->n_seqs, rows, n_heads, kv, hd, cache->blocks_per_seq);
     if (need > 0 && !workspace) return QLIN_ERR_NULL;
@@ -459,23 +679,23 @@ int qlin_launch_attend_kv8(const qlin_kv8_cache *cache, const float *q, float *a
     const qlin::Kv8View view = qlin::kv8_view(cache);
     auto go = [&](auto attend, auto join) {
         hipLaunchKernelGGL(attend, dim3(static_cast<unsigned>(grid)), dim3(64 * qlin::kWaves), 0, qlin::current_stream(),
-                           view, q, attn, rows, n_heads, start_pos_dev, n_rows_dev, q_scale, static_cast<int>(p.tiles),
-                           p.splits, part);
+                           view, q, attn, rows, n_heads, start_pos_dev, n_rows_dev, q_scale,
+                           static_cast<int>(p.tiles / p.rt), p.splits, part);
         if (hipGetLastError() != hipSuccess) return QLIN_ERR_LAUNCH;
         if (p.splits > 1) {
             hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(p.groups * qlin::kTile)), dim3(qlin::kJoinThreads), 0,
                                qlin::current_stream(), view, attn, rows, n_heads, start_pos_dev, n_rows_dev,
-                               static_cast<int>(p.tiles), p.splits, part);
+                               static_cast<int>(p.tiles), p.rt * qlin::kTile, p.splits, part);
             if (hipGetLastError() != hipSuccess) return QLIN_ERR_LAUNCH;
         }
         return QLIN_OK;
     };
     switch (hd) {
-        case 64: return go(qlin::attend_kv8_kernel<64>, qlin::attend_kv8_join_kernel<64>);
-        case 96: return go(qlin::attend_kv8_kernel<96>, qlin::attend_kv8_join_kernel<96>);
-        case 128: return go(qlin::attend_kv8_kernel<128>, qlin::attend_kv8_join_kernel<128>);
-        case 192: return go(qlin::attend_kv8_kernel<192>, qlin::attend_kv8_join_kernel<192>);
-        default: return go(qlin::attend_kv8_kernel<256>, qlin::attend_kv8_join_kernel<256>);
+        case 64: return go(p.rt == 2 ? qlin::attend_kv8_kernel<64, 2> : qlin::attend_kv8_kernel<64, 1>, qlin::attend_kv8_join_kernel<64>);
+        case 96: return go(p.rt == 2 ? qlin::attend_kv8_kernel<96, 2> : qlin::attend_kv8_kernel<96, 1>, qlin::attend_kv8_join_kernel<96>);
+        case 128: return go(p.rt == 2 ? qlin::attend_kv8_kernel<128, 2> : qlin::attend_kv8_kernel<128, 1>, qlin::attend_kv8_join_kernel<128>);
+        case 192: return go(qlin::attend_kv8_kernel<192, 1>, qlin::attend_kv8_join_kernel<192>);
+        default: return go(qlin::attend_kv8_kernel<256, 1>, qlin::attend_kv8_join_kernel<256>);
     }
 }
 
