@@ -68,8 +68,14 @@ struct Runs {
     }
 };
 
-__device__ __forceinline__ double weight_of(const uint16_t *w, int j, int type, int one_plus) {
-    const uint32_t u = w[j];
+// The 4 weights from w + j (j a multiple of 4) as 16-bit patterns: one load where w is 8-byte aligned (four loads of 2
+// bytes for each run of each head kept a prompt's kernel at 28 us where the bytes take 14).
+__device__ __forceinline__ uint2 weights_at(const uint16_t *w, int j) {
+    if ((reinterpret_cast<uintptr_t>(w) & 7u) == 0) return *reinterpret_cast<const uint2 *>(w + j);  // uniform
+    return make_uint2(w[j] | static_cast<uint32_t>(w[j + 1]) << 16, w[j + 2] | static_cast<uint32_t>(w[j + 3]) << 16);
+}
+__device__ __forceinline__ double weight_of(uint2 w, int e, int type, int one_plus) {
+    const uint32_t u = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
     const float v = type == 0 ? __builtin_bit_cast(float, u << 16)
                               : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u)));
     return one_plus ? static_cast<double>(v) + 1.0 : static_cast<double>(v);
@@ -87,14 +93,11 @@ __device__ __forceinline__ void norm_and_turn(f32x4v &va, f32x4v &vb, const Runs
         b[e] = vb[e];
     }
     // (requested before the sum needs them)
-    double wa[4], wb[4];
     const bool normed = w != nullptr;
+    uint2 wa = make_uint2(0u, 0u), wb = make_uint2(0u, 0u);
     if (normed && live) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            wa[e] = weight_of(w, r.a + e, how.norm_type, how.one_plus);
-            wb[e] = weight_of(w, r.b + e, how.norm_type, how.one_plus);
-        }
+        wa = weights_at(w, r.a);
+        wb = weights_at(w, r.b);
     }
     const int half = how.rotary_dim / 2;
     f32x4v c0, s0;  // halves: the pairs' cosines and sines; neighbours: (cos, cos, sin, sin) of run a's and b's pairs
@@ -116,8 +119,8 @@ __device__ __forceinline__ void norm_and_turn(f32x4v &va, f32x4v &vb, const Runs
         if (live) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                a[e] = a[e] * inv * wa[e];
-                b[e] = b[e] * inv * wb[e];
+                a[e] = a[e] * inv * weight_of(wa, e, how.norm_type, how.one_plus);
+                b[e] = b[e] * inv * weight_of(wb, e, how.norm_type, how.one_plus);
             }
         }
     }
@@ -160,9 +163,10 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kernel(qlin_qk_rope 
                                                                    float *__restrict__ vc, int rows, int n_heads, int kv,
                                                                    int hd, int max_seq, const int *__restrict__ start_pos) {
     const int t = threadIdx.x % T, heads = n_heads + 2 * kv;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / T) + threadIdx.x / T;
-    const bool there = unit < static_cast<int64_t>(rows) * heads;
-    const int row = there ? static_cast<int>(unit / heads) : 0, head = there ? static_cast<int>(unit % heads) : 0;
+    const unsigned unit = blockIdx.x * (kThreads / T) + threadIdx.x / T;  // (the launch has fewer than 2^31)
+    const unsigned line = unit / static_cast<unsigned>(heads);
+    const bool there = line < static_cast<unsigned>(rows);
+    const int row = there ? static_cast<int>(line) : 0, head = there ? static_cast<int>(unit - line * heads) : 0;
     const int64_t at = static_cast<int64_t>(*start_pos) + row;
     const int pos = static_cast<int>(at < 0 ? 0 : at < max_seq ? at : max_seq - 1);
     const Runs r(t, how.rotary_dim);
@@ -175,13 +179,18 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kernel(qlin_qk_rope 
                  : is_k ? kc + (static_cast<size_t>(pos) * kv + (head - n_heads)) * hd
                         : vc + (static_cast<size_t>(pos) * kv + (head - n_heads - kv)) * hd;
     f32x4v a = live ? ld4(src + r.a) : kZero4, b = live ? ld4(src + r.b) : kZero4;
-    const f32x4v a0 = a, b0 = b;
+    f32x4v x = a, y = b;
     Runs rr = r;
     rr.turned = rr.turned && live && (is_q || is_k);
-    norm_and_turn<T>(a, b, rr, live, hd, is_q ? how.q_norm : how.k_norm, how, pos);
+    norm_and_turn<T>(x, y, rr, live, hd, is_q ? how.q_norm : how.k_norm, how, pos);
     if (live) {
-        st4(dst + r.a, is_q || is_k ? a : a0);
-        st4(dst + r.b, is_q || is_k ? b : b0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // (by value: a choice between vectors goes through memory)
+            a[e] = is_q || is_k ? x[e] : a[e];
+            b[e] = is_q || is_k ? y[e] : b[e];
+        }
+        st4(dst + r.a, a);
+        st4(dst + r.b, b);
     }
 }
 
@@ -190,15 +199,18 @@ constexpr int lanes_of() {
     return HD <= 64 ? 8 : HD <= 128 ? 16 : 32;
 }
 
-// The largest over the workgroup (kThreads), of the magnitudes' bits: NaN is above infinity, which is above the rest.
-__device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t *red) {
+// The largest over the workgroup (kThreads), of the bits of two magnitudes: NaN is above infinity, which is above the
+// rest.  A barrier lies between two calls' uses of red.
+__device__ __forceinline__ uint2 block_max_bits(uint2 v, uint2 *red) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)));
-    __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) {
+        v.x = max(v.x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v.x), o, 64)));
+        v.y = max(v.y, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v.y), o, 64)));
+    }
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) v = max(v, red[w]);
+    for (int w = 0; w < kThreads / 64; ++w) v = make_uint2(max(v.x, red[w].x), max(v.y, red[w].y));
     return v;
 }
 
@@ -223,16 +235,17 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
                                                                        const int *__restrict__ n_rows) {
     constexpr int T = lanes_of<HD>(), kTok = kThreads / T, kPass = kKv8Block / kTok;
     const int t = threadIdx.x % T;
-    const int64_t kv_groups = static_cast<int64_t>(n_seqs) * c.kv * slots;
+    const unsigned kv_groups = static_cast<unsigned>(n_seqs) * c.kv * slots;
     const int cap = c.per * kKv8Block;
     const Runs r(t, how.rotary_dim);
     const bool in_head = 8 * t < HD;
     if (blockIdx.x >= kv_groups) {
-        const int64_t unit = (blockIdx.x - kv_groups) * kTok + threadIdx.x / T;
-        const bool there = unit < static_cast<int64_t>(n_seqs) * rows * n_heads;
-        const int64_t line = there ? unit / n_heads : 0;
-        const int head = there ? static_cast<int>(unit % n_heads) : 0;
-        const int seq = static_cast<int>(line / rows), row = static_cast<int>(line % rows);
+        const unsigned unit = (blockIdx.x - kv_groups) * kTok + threadIdx.x / T;  // (the launch has fewer than 2^31)
+        const unsigned at = unit / static_cast<unsigned>(n_heads);
+        const bool there = at < static_cast<unsigned>(n_seqs) * static_cast<unsigned>(rows);
+        const unsigned line = there ? at : 0;
+        const int head = there ? static_cast<int>(unit - at * n_heads) : 0;
+        const int seq = static_cast<int>(line / static_cast<unsigned>(rows)), row = static_cast<int>(line - seq * static_cast<unsigned>(rows));
         const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, cap);
         const bool live = there && in_head && row < w.rows;
         const float *src = q + static_cast<size_t>(line) * q_stride + static_cast<size_t>(head) * HD;
@@ -248,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
         return;
     }
     __shared__ __attribute__((aligned(16))) uint8_t s_rec[64 * HD];
-    __shared__ uint32_t red[kThreads / 64];
+    __shared__ uint2 red[kThreads / 64];
     const int slot = static_cast<int>(blockIdx.x % slots);
     const int head = static_cast<int>(blockIdx.x / slots % c.kv), seq = static_cast<int>(blockIdx.x / slots / c.kv);
     const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, cap);
@@ -261,6 +274,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
 
     auto block = [&](int b) {
         const bool complete = (b + 1) * kKv8Block <= w.len;
+        const int page = c.page(seq, b);
         f32x4v ka[kPass], kb[kPass], va[kPass], vb[kPass];
 #pragma unroll
         for (int p = 0; p < kPass; ++p) {
@@ -305,10 +319,10 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
                 v_top = max(max(v_top, __float_as_uint(va[p][e]) & 0x7fffffffu), __float_as_uint(vb[p][e]) & 0x7fffffffu);
             }
         }
-        const int page = c.page(seq, b);
         if (!complete || page < 0) return;  // uniform
-        k_top = block_max_bits(k_top, red);
-        v_top = block_max_bits(v_top, red);
+        const uint2 top = block_max_bits(make_uint2(k_top, v_top), red);
+        k_top = top.x;
+        v_top = top.y;
         const bool k_fin = k_top < 0x7f800000u, v_fin = v_top < 0x7f800000u;
         const float k_scale = k_fin ? __builtin_bit_cast(float, k_top) * (1.0f / 127.0f) : NAN;
         const float v_scale = v_fin ? __builtin_bit_cast(float, v_top) * (1.0f / 127.0f) : NAN;
@@ -347,21 +361,25 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
     }
 }
 
-// A workgroup per (sequence, key head, 32 rows): a thread per 4 dims of a row.
+// A workgroup per (sequence, key head, 32 rows): a thread per 4 dims of a row.  Its rows lie in two blocks at most, whose
+// pages are requested first.
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(Kv8View c, int hd, const int *__restrict__ first,
                                                             const int *__restrict__ lens, int count, int parts,
                                                             float *__restrict__ k_out, float *__restrict__ v_out) {
     const int part = static_cast<int>(blockIdx.x % parts);
     const int head = static_cast<int>(blockIdx.x / parts % c.kv), seq = static_cast<int>(blockIdx.x / parts / c.kv);
     const int len = min(max(lens[seq], 0), c.per * kKv8Block);
-    const int64_t from = first[seq];
-    const int n4 = hd / 4;
+    const int64_t from = static_cast<int64_t>(first[seq]) + part * 32;
+    if (from >= len || from + 31 < 0) return;  // uniform
+    const int n4 = hd / 4, b0 = from < 0 ? 0 : static_cast<int>(from / kKv8Block);
+    const int page0 = c.page(seq, b0), page1 = (b0 + 1) * kKv8Block < len ? c.page(seq, b0 + 1) : -1;
+#pragma unroll 4
     for (int i = threadIdx.x; i < 32 * n4; i += kThreads) {
         const int row = part * 32 + i / n4, d = 4 * (i % n4);
-        const int64_t at = from + row;
+        const int64_t at = from + i / n4;
         if (row >= count || at < 0 || at >= len) continue;
         const int pos = static_cast<int>(at), b = pos / kKv8Block, tok = pos % kKv8Block;
-        const int page = c.page(seq, b);
+        const int page = b == b0 ? page0 : page1;
         if (page < 0) continue;
         f32x4v kx, vx;
         if ((b + 1) * kKv8Block <= len) {
