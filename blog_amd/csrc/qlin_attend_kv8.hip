@@ -147,14 +147,22 @@ struct Queries {
     u32x4 hi[HD / 32], lo[HD / 32];
     float inv;
     int seen;  // the last position that query row n sees
-    __device__ __forceinline__ void load(const float *row, float q_scale) {
+    struct Raw {
         f32x4 v[HD / 32][2];
+        __device__ __forceinline__ void load(const float *row) {
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[i][h] = *reinterpret_cast<const f32x4 *>(row + 32 * i + 4 * h);
+        }
+    };
+    __device__ __forceinline__ void take(Raw &raw, float q_scale) {
+        auto &v = raw.v;
         uint32_t top = 0;  // (integers: a value that is not finite is above all others)
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                v[i][h] = *reinterpret_cast<const f32x4 *>(row + 32 * i + 4 * h);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[i][h][e] *= q_scale;
@@ -348,6 +356,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
     id /= c.kv;
     const int macro = macros - 1 - id % macros, seq = id / macros;
     const int group = n_heads / c.kv, p0 = macro * kRows;
+    typename Queries<HD>::Raw raw[RT];  // (requested first: nothing that is read has to be known)
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const int pair = min(p0 + k * kTile + n, rows * group - 1);
+        raw[k].load(q + ((static_cast<size_t>(seq) * rows + pair / group) * n_heads + kh * group + pair % group) * HD + 8 * g);
+    }
     const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, c.per * kKv8Block);
     const int pairs = w.rows * group;
     if (p0 >= pairs) return;
@@ -392,7 +406,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
     for (int k = 0; k < RT; ++k) {
         const int pair = min(p0 + k * kTile + n, pairs - 1);
         qs[k].seen = min(w.start + pair / group, w.len - 1);
-        qs[k].load(q + ((static_cast<size_t>(seq) * rows + pair / group) * n_heads + kh * group + pair % group) * HD + 8 * g, q_scale);
+        qs[k].take(raw[k], q_scale);
         t[k].clear();
     }
 
@@ -540,6 +554,18 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c
     __shared__ float s_f[kJoinThreads / 64][kMaxSplits];
     const int row = blockIdx.x % kTile, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned group_id = blockIdx.x / kTile;
+    const float *src = part + (static_cast<size_t>(group_id) * splits * kTile + row) * (HD + 4);
+    const size_t step = static_cast<size_t>(kTile) * (HD + 4);
+    const int cls = threadIdx.x / D4, d4 = threadIdx.x % D4;
+    // requested before it is known how many splits there are; what the others hold is not used
+    f32x4 first[4];
+    float2 ml[kSlots];
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k)
+        ml[k] = lane + 64 * k < splits ? *reinterpret_cast<const float2 *>(src + (lane + 64 * k) * step + HD) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        first[u] = cls < C && cls + u * C < splits ? *reinterpret_cast<const f32x4 *>(src + (cls + u * C) * step + 4 * d4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int id = group_id;
     const int kh = id % c.kv;
     id /= c.kv;
@@ -552,21 +578,12 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c
     const Span sp = span_of(w, p0 / macro * macro, macro, group);
     const int per = items_per_split(sp.items(), splits), used = (sp.items() + per - 1) / per;
     if (used <= 1) return;  // written already
-    const float *src = part + (static_cast<size_t>(group_id) * splits * kTile + row) * (HD + 4);
-    const size_t step = static_cast<size_t>(kTile) * (HD + 4);
-    const int cls = threadIdx.x / D4, d4 = threadIdx.x % D4;
-    f32x4 first[4];  // (requested before the weights are known)
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-        first[u] = cls < C && cls + u * C < used ? *reinterpret_cast<const f32x4 *>(src + (cls + u * C) * step + 4 * d4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float mi[kSlots], li[kSlots], mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kSlots; ++k) {
-        const int i = lane + 64 * k;
-        const float2 ml = i < used ? *reinterpret_cast<const float2 *>(src + i * step + HD) : make_float2(-INFINITY, 0.0f);
-        mi[k] = ml.x;
-        li[k] = ml.y;
-        mx = fmaxf(mx, ml.x);
+        mi[k] = lane + 64 * k < used ? ml[k].x : -INFINITY;
+        li[k] = lane + 64 * k < used ? ml[k].y : 0.0f;
+        mx = fmaxf(mx, mi[k]);
     }
     mx = wave_max_dpp(mx);
     float den = 0.0f;

@@ -92,8 +92,8 @@ extern "C" {
  * of them is storing to.
  *
  * Rows come as [n_seqs, rows, heads, head_dim], row r of sequence s at position start_pos_dev[s] + r; with n_rows_dev
- * only the first n_rows_dev[s] (clamped to 0 .. rows) of them count: the others are neither read nor stored,
- * and their outputs stay as they were.  *_stride is the distance of a row's first head from the next row's, in
+ * only the first n_rows_dev[s] (clamped to 0 .. rows) of them count: the others are not stored, and their outputs
+ * stay as they were.  *_stride is the distance of a row's first head from the next row's, in
  * floats (>= heads * head_dim, so that q, k and v may be parts of one tensor); outputs are packed.
  * head_dim 64, 96, 128, 192 or 256 (else QLIN_ERR_LIMIT), pages and recent 16-byte aligned, blocks_per_seq <= 32768.
  *
