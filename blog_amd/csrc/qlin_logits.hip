@@ -27,10 +27,14 @@ __device__ __forceinline__ void better(float &v, int &i, float w, int j) {
     v = take ? w : v;
     i = take ? j : i;
 }
-// over the workgroup, in thread 0
-__device__ __forceinline__ void block_best(float &v, int &i, float *s_v, int *s_i) {
+// over the wave, in every lane
+__device__ __forceinline__ void wave_best(float &v, int &i) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) better(v, i, __shfl_xor(v, o, 64), __shfl_xor(i, o, 64));
+}
+// over the workgroup, in thread 0
+__device__ __forceinline__ void block_best(float &v, int &i, float *s_v, int *s_i) {
+    wave_best(v, i);
     if ((threadIdx.x & 63) == 0) {
         s_v[threadIdx.x >> 6] = v;
         s_i[threadIdx.x >> 6] = i;
@@ -40,7 +44,22 @@ __device__ __forceinline__ void block_best(float &v, int &i, float *s_v, int *s_
         for (int w = 1; w < kThreads / 64; ++w) better(v, i, s_v[w], s_i[w]);
 }
 
-// U runs of 4 tokens a thread: slices of 1024 U tokens.
+// entries i .. i + 3 of the n at p, -1 past them
+__device__ __forceinline__ int4 ids_at(const int *p, int i, int n) {
+    int4 v = make_int4(-1, -1, -1, -1);
+    if (i + 4 <= n) {
+        __builtin_memcpy(&v, __builtin_assume_aligned(p + i, 4), 16);
+    } else {
+        if (i < n) v.x = p[i];
+        if (i + 1 < n) v.y = p[i + 1];
+        if (i + 2 < n) v.z = p[i + 2];
+    }
+    return v;
+}
+
+// U runs of 4 tokens a thread: slices of 1024 U tokens.  Everything that does not wait for another load is requested
+// before the first barrier: the logits, the mask, the first 2048 tokens of the history (whose length is then not known
+// yet) and the first 256 biases.
 template <int U>
 __global__ __launch_bounds__(kThreads) void logits_controls_kernel(qlin_logits_controls c, const float *logits,
                                                                    size_t logits_stride, float *out, size_t out_stride,
@@ -73,12 +92,18 @@ __global__ __launch_bounds__(kThreads) void logits_controls_kernel(qlin_logits_c
         }
         if (mask && i < n) allow[u] = mask[i / 32] >> (i % 32);
     }
+    const int *hist = c.history ? c.history + static_cast<size_t>(row) * c.max_history : nullptr;
+    const int most = hist ? c.max_history : 0;
+    int4 h0 = ids_at(hist, 4 * tid, most), h1 = ids_at(hist, 4 * (kThreads + tid), most);
+    const bool biased = c.bias_ids != nullptr && c.max_bias > 0;
+    const int *ids = c.bias_ids + static_cast<size_t>(row) * c.max_bias;
+    const float *add = c.bias_values + static_cast<size_t>(row) * c.max_bias;
+    const int id0 = biased && tid < c.max_bias ? ids[tid] : -1;
+    const float add0 = biased && tid < c.max_bias ? add[tid] : 0.0f;
     const float rep = c.repetition ? c.repetition[row] : 1.0f;
     const float freq = c.frequency ? c.frequency[row] : 0.0f, pres = c.presence ? c.presence[row] : 0.0f;
-    int h = c.history ? c.max_history : 0;
-    if (h && c.history_lens) h = min(max(c.history_lens[row], 0), h);
+    const int h = most && c.history_lens ? min(max(c.history_lens[row], 0), most) : most;
     const bool counted = h > 0 && !(rep == 1.0f && freq == 0.0f && pres == 0.0f);  // uniform
-    const bool biased = c.bias_ids != nullptr && c.max_bias > 0;
     if (counted) {
 #pragma unroll
         for (int u = 0; u < U; ++u) reinterpret_cast<int4 *>(s_count)[u * kThreads + tid] = make_int4(0, 0, 0, 0);
@@ -89,23 +114,34 @@ __global__ __launch_bounds__(kThreads) void logits_controls_kernel(qlin_logits_c
     }
     __syncthreads();
     if (counted) {
-        const int *hist = c.history + static_cast<size_t>(row) * c.max_history;
-        for (int i0 = tid; i0 < h; i0 += 8 * kThreads) {
-            int t[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = i0 + k * kThreads < h ? hist[i0 + k * kThreads] : -1;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const unsigned at = static_cast<unsigned>(t[k]) - static_cast<unsigned>(v0);
-                if (t[k] >= 0 && at < static_cast<unsigned>(n)) atomicAdd(&s_count[at], 1);
-            }
+        auto count = [&](int t) {  // (as unsigned, what is below the slice is above it too: ids < 0 among them)
+            const unsigned at = static_cast<unsigned>(t) - static_cast<unsigned>(v0);
+            if (at < static_cast<unsigned>(n)) atomicAdd(&s_count[at], 1);
+        };
+        auto count4 = [&](int4 t, int i) {
+            count(i < h ? t.x : -1);
+            count(i + 1 < h ? t.y : -1);
+            count(i + 2 < h ? t.z : -1);
+            count(i + 3 < h ? t.w : -1);
+        };
+        count4(h0, 4 * tid);
+        count4(h1, 4 * (kThreads + tid));
+        for (int i0 = 8 * kThreads; i0 < h; i0 += 8 * kThreads) {
+            h0 = ids_at(hist, i0 + 4 * tid, h);
+            h1 = ids_at(hist, i0 + 4 * (kThreads + tid), h);
+            count(h0.x);
+            count(h0.y);
+            count(h0.z);
+            count(h0.w);
+            count(h1.x);
+            count(h1.y);
+            count(h1.z);
+            count(h1.w);
         }
     }
-    const int *ids = c.bias_ids + static_cast<size_t>(row) * c.max_bias;
-    const float *add = c.bias_values + static_cast<size_t>(row) * c.max_bias;
     if (biased) {
         for (int e = tid; e < c.max_bias; e += kThreads) {
-            const int t = ids[e];
+            const int t = e == tid ? id0 : ids[e];
             const unsigned at = static_cast<unsigned>(t) - static_cast<unsigned>(v0);
             if (t >= 0 && at < static_cast<unsigned>(n)) {
                 const uint32_t bit = 1u << (at % 32);
@@ -156,10 +192,10 @@ __global__ __launch_bounds__(kThreads) void logits_controls_kernel(qlin_logits_c
     if (biased) {
         const bool twice = s_twice != 0;  // uniform
         for (int e = tid; e < c.max_bias; e += kThreads) {
-            const int t = ids[e];
+            const int t = e == tid ? id0 : ids[e];
             const unsigned at = static_cast<unsigned>(t) - static_cast<unsigned>(v0);
             if (t < 0 || at >= static_cast<unsigned>(n)) continue;
-            float sum = add[e];
+            float sum = e == tid ? add0 : add[e];
             if (twice) {
                 bool first = true;
                 for (int k = 0; k < e; ++k) first &= ids[k] != t;
@@ -185,17 +221,15 @@ __global__ __launch_bounds__(kThreads) void logits_controls_kernel(qlin_logits_c
     }
 }
 
-// A workgroup per row: the best of its slices'.
-__global__ __launch_bounds__(kThreads) void logits_pick_kernel(const float *__restrict__ best_v,
-                                                               const int *__restrict__ best_i, int slices,
-                                                               int *__restrict__ picks) {
-    __shared__ float s_v[kThreads / 64];
-    __shared__ int s_i[kThreads / 64];
+// A wave per row: the best of its slices'.
+__global__ __launch_bounds__(64) void logits_pick_kernel(const float *__restrict__ best_v, const int *__restrict__ best_i,
+                                                         int slices, int *__restrict__ picks) {
     const size_t at = static_cast<size_t>(blockIdx.x) * slices;
     float v = -INFINITY;
     int i = 0;
-    for (int k = threadIdx.x; k < slices; k += kThreads) better(v, i, best_v[at + k], best_i[at + k]);
-    block_best(v, i, s_v, s_i);
+#pragma unroll 4
+    for (int k = threadIdx.x; k < slices; k += 64) better(v, i, best_v[at + k], best_i[at + k]);
+    wave_best(v, i);
     if (threadIdx.x == 0) picks[blockIdx.x] = i;
 }
 
@@ -253,7 +287,7 @@ int qlin_launch_logits_controls(const qlin_logits_controls *controls, const floa
                            logits, logits_stride, out, out_stride, vocab, slices, bv, bi, picks);
         if (hipGetLastError() != hipSuccess) return QLIN_ERR_LAUNCH;
         if (!picks || slices == 1) return QLIN_OK;
-        hipLaunchKernelGGL(qlin::logits_pick_kernel, dim3(rows), dim3(qlin::kThreads), 0, qlin::current_stream(), bv, bi,
+        hipLaunchKernelGGL(qlin::logits_pick_kernel, dim3(rows), dim3(64), 0, qlin::current_stream(), bv, bi,
                            slices, picks);
         return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
     };
