@@ -27,9 +27,10 @@ __device__ __forceinline__ f32x4v ld4(const float *p) {
     __builtin_memcpy(&v, __builtin_assume_aligned(p, 4), 16);
     return v;
 }
-__device__ __forceinline__ void st4(float *p, const f32x4v &v) {
-    __builtin_memcpy(__builtin_assume_aligned(p, 4), &v, 16);
-}
+// Streaming stores: what lies dirty in the L2s at the kernel's end is written back then (a 2011-row prompt's store and
+// read back 26.0 us, so 22.2; 1877 rows into the f32 cache 18.3 and 16.5).
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void st4(float *p, const f32x4v &v) { __builtin_nontemporal_store(v, reinterpret_cast<f32x4u *>(p)); }
 
 template <int CTRL>
 __device__ __forceinline__ double dpp_move64(double x) {
