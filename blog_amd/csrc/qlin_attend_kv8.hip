@@ -9,7 +9,7 @@
 // which is what it supplies as the second product's operand, so that probabilities go from one product to the next
 // without leaving their lane.
 //
-// Operands: a code is exact in fp16 (one v_cvt_f16_i16 with byte and half selects).  q (times
+// Operands: a code is exact in fp16 (1024 + 128 + code by byte permutes, less 1152).  q (times
 // softmax_scale log2(e), one rounding, and a power of two that brings its row's largest value to 2^14 .. 2^15) and p
 // (times 2^11) are fp16 pairs hi + lo, 22 bits and a sign, so their products with a code are exact and a score is off by
 // 2^-23 of its terms.  What is lost besides lies below 2^-39 of a row's largest q, or 2^-36 of its largest p: a
@@ -43,50 +43,31 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ f32x4 mfma16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// The fp16 values of 4 codes, as two pairs (a's byte LA and b's LB, then c's LC and d's LD).  A half written by itself may
-// not be read by the next instruction (one wait state): the two pairs alternate, and a wait ends them.
-#define QLIN_CODES4(NAME, LA, LB, LC, LD)                                                                            \
-    __device__ __forceinline__ void NAME(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t &x, uint32_t &y) { \
-        asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_" #LA "\n\t"         \
-            "v_cvt_f16_i16_sdwa %1, sext(%4) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_" #LC "\n\t"         \
-            "v_cvt_f16_i16_sdwa %0, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_" #LB "\n\t"    \
-            "v_cvt_f16_i16_sdwa %1, sext(%5) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_" #LD "\n\t"    \
-            "s_nop 0"                                                                                                \
-            : "=&v"(x), "=&v"(y)                                                                                     \
-            : "v"(a), "v"(b), "v"(c), "v"(d));                                                                       \
-    }
-QLIN_CODES4(codes_0123, 0, 1, 2, 3)
-QLIN_CODES4(codes_0, 0, 0, 0, 0)
-QLIN_CODES4(codes_1, 1, 1, 1, 1)
-QLIN_CODES4(codes_2, 2, 2, 2, 2)
-QLIN_CODES4(codes_3, 3, 3, 3, 3)
-#undef QLIN_CODES4
-// the 8 codes of two dwords, in order
-__device__ __forceinline__ u32x4 f16_of_8(uint32_t a, uint32_t b) {
-    uint32_t v[4];
-    codes_0123(a, a, a, a, v[0], v[1]);
-    codes_0123(b, b, b, b, v[2], v[3]);
-    return u32x4{v[0], v[1], v[2], v[3]};
+// No instructions in inline assembly here: the compiler does not see what it does to registers that an MFMA is still writing (byte-select
+// conversions, 1 instruction a code, wrote such a register before its MFMA's unused lanes did).
+// 1024 + 128 + code, in fp16, less 1152
+__device__ __forceinline__ uint32_t less_1152(uint32_t biased) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, biased) + f16x2{-1152.0f16, -1152.0f16});
 }
-// byte J of a and b, then of c and d
+// the 8 codes of two dwords, in order: a byte code ^ 0x80 is code + 128, under the byte 0x64 it is that plus 1024
+__device__ __forceinline__ u32x4 f16_of_8(uint32_t a, uint32_t b) {
+    const uint32_t u = a ^ 0x80808080u, v = b ^ 0x80808080u, k64 = 0x64646464u;
+    return u32x4{less_1152(__builtin_amdgcn_perm(k64, u, 0x04010400u)), less_1152(__builtin_amdgcn_perm(k64, u, 0x04030402u)),
+                 less_1152(__builtin_amdgcn_perm(k64, v, 0x04010400u)), less_1152(__builtin_amdgcn_perm(k64, v, 0x04030402u))};
+}
+// byte J of a and of b
 template <int J>
-__device__ __forceinline__ uint2 f16_of_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    uint2 v;
-    if constexpr (J == 0) codes_0(a, b, c, d, v.x, v.y);
-    else if constexpr (J == 1) codes_1(a, b, c, d, v.x, v.y);
-    else if constexpr (J == 2) codes_2(a, b, c, d, v.x, v.y);
-    else codes_3(a, b, c, d, v.x, v.y);
-    return v;
+__device__ __forceinline__ uint32_t f16_of_bytes(uint32_t a, uint32_t b) {
+    return less_1152(__builtin_amdgcn_perm(b, a, 0x0c000c00u | ((4u + J) << 16) | J) ^ 0x64806480u);
 }
 // hi + lo of two values, each an fp16 pair
 __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
     const f32x2 v = {a, b};
-    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-    f32x2 r;
-    float r0, r1;  // v - hi, exact
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(a));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(b));
-    r = f32x2{r0, r1};
+    const f16x2 h = __builtin_convertvector(v, f16x2);
+    float minus = -1.0f;
+    asm("" : "+s"(minus));  // (unknown to the compiler: one v_fma_mix_f32 a value, where it makes two of a difference)
+    const f32x2 r = {__builtin_fmaf(static_cast<float>(h[0]), minus, a), __builtin_fmaf(static_cast<float>(h[1]), minus, b)};  // exact
+    hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, f16x2));
 }
 __device__ __forceinline__ void split2(const f32x4 &a, const f32x4 &b, u32x4 &hi, u32x4 &lo) {
@@ -158,21 +139,18 @@ struct Queries {
     };
     __device__ __forceinline__ void take(Raw &raw, float q_scale) {
         auto &v = raw.v;
-        uint32_t top = 0;  // (integers: a value that is not finite is above all others)
+        float most = 0.0f;  // (a NaN is not seen here, and is one in its parts)
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[i][h][e] *= q_scale;
-                    top = max(top, __float_as_uint(v[i][h][e]) & 0x7fffffffu);
-                }
+                most = fmaxf(fmaxf(most, fabsf(v[i][h][0])), fabsf(v[i][h][1]));
+                most = fmaxf(fmaxf(most, fabsf(v[i][h][2])), fabsf(v[i][h][3]));
             }
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
+        const uint32_t top = __float_as_uint(groups_max(most) * fabsf(q_scale));
         const int up = min(127 + 14 - static_cast<int>(top >> 23), 100);  // at most 2^100
-        const float scale = top < 0x7f800000u ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : NAN;
+        // (a power of two times q_scale: one rounding a value; NaN for a row whose largest is not finite)
+        const float scale = top < 0x7f800000u ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) * q_scale : NAN;
         inv = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
@@ -193,7 +171,7 @@ template <int HD>
 struct Sums {
     static constexpr int NT = (HD + 63) / 64;
     f32x4 o[NT][4];    // of query row n: [i][j][r] is dim 64 i + 16 g + 4 r + j (past HD: zeros)
-    float m, l;        // l: of this lane's positions
+    float m, l;
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -202,10 +180,11 @@ struct Sums {
         m = -INFINITY;
         l = 0.0f;
     }
-    // the maximum becomes at least that of the tile's scores; returns what is added to the scores
+    // the maximum becomes the tile's where one is kSlack above it; mx: of this lane's scores.  Returns what is added to
+    // the scores.
     __device__ __forceinline__ float raise(float mx) {
-        mx = fmaxf(m, groups_max(mx));
         if (__any(mx > m + kSlack)) {  // uniform
+            mx = fmaxf(m, groups_max(mx));
             const float al = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
             l *= al;
 #pragma unroll
@@ -245,9 +224,13 @@ struct Sums {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 s[u][r] = exp2_fast(fmaf(s[u][r], f, add));
-                l += s[u][r];
             }
         split2(s[0], s[1], hi, lo);
+        // the sum of the operands that the values meet, by products with ones (8 additions took as long as 5 MFMAs)
+        const uint32_t one = 0x3c003c00u;
+        const u32x4 ones = {one, one, one, one};
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        l += mfma16(ones, lo, mfma16(ones, hi, zero))[0];
     }
     __device__ __forceinline__ void join(int i, int j, const f32x4 &t, float vs) {
 #pragma unroll
@@ -282,8 +265,8 @@ struct Sums {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             s[r] = exp2_fast(s[r] + add);
-            l += s[r];
         }
+        l += groups_sum((s[0] + s[1]) + (s[2] + s[3]));
         bool odd = false;  // a value that is not finite
         f32x4 v[4][NT];    // dims 64 i + 4n .. + 3 of position 4g + r
 #pragma unroll
@@ -446,11 +429,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
             auto values = [&](int i, auto jc) {  // two operands, whose chains are independent
                 constexpr int J = decltype(jc)::value;
                 // positions 4g, 4g + 1; 4g + 2, + 3; 16 + 4g, + 1; 16 + 4g + 2, + 3
-                const uint2 a0 = f16_of_bytes<J>(vc[i][0][0], vc[i][1][0], vc[i][0][1], vc[i][1][1]);
-                const uint2 a1 = f16_of_bytes<J>(vc[i][0][2], vc[i][1][2], vc[i][0][3], vc[i][1][3]);
-                const uint2 b0 = f16_of_bytes<J + 1>(vc[i][0][0], vc[i][1][0], vc[i][0][1], vc[i][1][1]);
-                const uint2 b1 = f16_of_bytes<J + 1>(vc[i][0][2], vc[i][1][2], vc[i][0][3], vc[i][1][3]);
-                const u32x4 a = {a0.x, a0.y, a1.x, a1.y}, b = {b0.x, b0.y, b1.x, b1.y};
+                u32x4 a, b;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    a[h] = f16_of_bytes<J>(vc[i][0][h], vc[i][1][h]);
+                    b[h] = f16_of_bytes<J + 1>(vc[i][0][h], vc[i][1][h]);
+                }
                 f32x4 x[RT][2];
 #pragma unroll
                 for (int k = 0; k < RT; ++k) {
@@ -490,7 +474,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
     for (int k = 0; k < RT; ++k) {
         const int pk = p0 + k * kTile;
         if (k > 0) __syncthreads();  // (the tile before is read)
-        t[k].l = groups_sum(t[k].l);
         if (g == 0) {
             s_m[wave][n] = t[k].m;
             s_l[wave][n] = t[k].l;
@@ -523,10 +506,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
             }
             if (used == 1) {
                 const int pr = pk + row;
-                f32x4 o = zero;
-                if (den != 0.0f)
+                const float inv = den != 0.0f ? 1.0f / den : 0.0f;  // (no position: num is 0 too)
+                f32x4 o;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] = num[r] / den;
+                for (int r = 0; r < 4; ++r) o[r] = num[r] * inv;
                 *reinterpret_cast<f32x4 *>(out + ((static_cast<size_t>(seq) * rows + pr / group) * n_heads + kh * group + pr % group) * HD + d) = o;
             } else {
                 // [tile of this launch][split][row]: HD sums, the maximum, the denominator
@@ -627,8 +610,9 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c
         for (int i = 1; i < C; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] += s_num[i][d4][r];
+        const float inv = den != 0.0f ? 1.0f / den : 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = den != 0.0f ? o[r] / den : 0.0f;
+        for (int r = 0; r < 4; ++r) o[r] *= inv;
         *reinterpret_cast<f32x4 *>(out + ((static_cast<size_t>(seq) * rows + pr / group) * n_heads + kh * group + pr % group) * HD + 4 * d4) = o;
     }
 }
