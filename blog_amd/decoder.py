@@ -12,6 +12,10 @@ with the KV-cache store and attention are qlin_decoder.h's.  The prompt runs as 
 m > 1 matmuls); each decode step is one token at a position held in device memory, so a step can be
 captured into a HIP graph and replayed, the argmax writing the next step's token id on the device.
 torch provides the device memory and the streams.
+
+Two variations of the architecture: ``qk_norm`` norms every query and key head before the rotation (weights ``q_norm``
+and ``k_norm`` [head_dim] in each layer), and ``kv8`` keeps keys and values in the 8-bit cache of blocks.  With
+``set_controls`` the pick goes by the logits after penalties for repeated tokens, biases and a mask.
 """
 from __future__ import annotations
 
@@ -35,6 +39,8 @@ class Qwen2Config:
     eps: float = 1e-6
     theta: float = 1e6
     wtype: int = Q8_0
+    qk_norm: bool = False  # norms of query and key heads
+    kv8: bool = False      # the cache in 8 bits (head_dim 64, 96, 128, 192 or 256)
 
     @property
     def q_dim(self) -> int:
@@ -63,8 +69,8 @@ def quantize_q8_0(torch, x):
 
 def make_weights(torch, cfg: Qwen2Config, seed: int) -> dict:
     """Random-init weights on the GPU: {'layers': [{wq, wk, wv, wo, wg, wu, wd, attn_norm,
-    ffn_norm}], 'final_norm', 'table'}; linears packed Q8_0 (uint8), norms as bf16 bit patterns
-    (int16 tensors)."""
+    ffn_norm}], 'final_norm', 'table'}, with cfg.qk_norm also q_norm and k_norm in each layer; linears packed
+    Q8_0 (uint8), norms as bf16 bit patterns (int16 tensors)."""
     assert cfg.wtype == Q8_0
     gen = torch.Generator(device="cuda")
     gen.manual_seed(seed)
@@ -72,8 +78,8 @@ def make_weights(torch, cfg: Qwen2Config, seed: int) -> dict:
     def linear(n, k):
         return quantize_q8_0(torch, torch.randn(n, k, device="cuda", generator=gen) * 0.02).contiguous()
 
-    def norm():
-        w = (1.0 + 0.1 * torch.randn(cfg.hidden, device="cuda", generator=gen)).to(torch.bfloat16)
+    def norm(n=cfg.hidden):
+        w = (1.0 + 0.1 * torch.randn(n, device="cuda", generator=gen)).to(torch.bfloat16)
         return w.view(torch.int16).contiguous()
 
     H, F = cfg.hidden, cfg.ffn
@@ -82,6 +88,8 @@ def make_weights(torch, cfg: Qwen2Config, seed: int) -> dict:
         layers.append({"wq": linear(cfg.q_dim, H), "wk": linear(cfg.kv_dim, H), "wv": linear(cfg.kv_dim, H),
                        "wo": linear(H, cfg.q_dim), "wg": linear(F, H), "wu": linear(F, H), "wd": linear(H, F),
                        "attn_norm": norm(), "ffn_norm": norm()})
+        if cfg.qk_norm:
+            layers[-1].update(q_norm=norm(cfg.head_dim), k_norm=norm(cfg.head_dim))
     return {"layers": layers, "final_norm": norm(), "table": linear(cfg.vocab, H)}
 
 
@@ -111,13 +119,46 @@ class Qwen2Decoder:
         self.act = torch.zeros(P, F, dtype=f32, device=dev)
         self.logits = torch.zeros(cfg.vocab, dtype=f32, device=dev)
         self.pick_scratch = torch.zeros(8192, dtype=torch.uint8, device=dev)  # the head's per-workgroup picks
-        self.kc = [torch.zeros(max_seq, cfg.kv_dim, dtype=f32, device=dev) for _ in range(cfg.layers)]
-        self.vc = [torch.zeros(max_seq, cfg.kv_dim, dtype=f32, device=dev) for _ in range(cfg.layers)]
+        f32_caches = 0 if cfg.kv8 else cfg.layers
+        self.kc = [torch.zeros(max_seq, cfg.kv_dim, dtype=f32, device=dev) for _ in range(f32_caches)]
+        self.vc = [torch.zeros(max_seq, cfg.kv_dim, dtype=f32, device=dev) for _ in range(f32_caches)]
         self.prompt_ids = torch.zeros(P, dtype=i32, device=dev)
         self.token = torch.zeros(1, dtype=i32, device=dev)      # the next step's input token
         self.pos = torch.zeros(1, dtype=i32, device=dev)        # the next step's position
         self.zero = torch.zeros(1, dtype=i32, device=dev)
         self.L = qlin.lib()
+        self.controls = None
+        if cfg.qk_norm or cfg.kv8:
+            qlin.set_stream(torch.cuda.current_stream())
+            self.rotation = torch.empty(max_seq, cfg.head_dim, dtype=f32, device=dev)
+            qlin.rope_table(self.rotation, cfg.theta)
+            self.how = [qlin.QkRope(W.get("q_norm"), W.get("k_norm"), 0, cfg.eps, 0, self.rotation, cfg.head_dim)
+                        for W in weights["layers"]]
+        if cfg.kv8:
+            self.kv8 = [qlin.Kv8Cache.empty(torch, 1, cfg.kv_heads, cfg.head_dim, max_seq) for _ in range(cfg.layers)]
+            need = max(qlin.attend_kv8_workspace_bytes(1, rows, cfg.n_heads, cfg.kv_heads, cfg.head_dim,
+                                                       self.kv8[0].blocks_per_seq) for rows in range(1, P + 1))
+            self.attend_ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+
+    def set_controls(self, repetition=1.0, frequency=0.0, presence=0.0, bias=None, mask=None) -> None:
+        """From the next pick on (and in every graph captured after this): penalties for the tokens of the prompt and
+        those picked since the last prefill, a bias {token: value}, and a mask (int32 words, 32 tokens each, a bit set for
+        a token that may follow; the tensor is read at every pick, so a grammar rewrites it between steps)."""
+        torch, c = self.torch, self.cfg
+        if mask is not None and (mask.dtype != torch.int32 or tuple(mask.shape) != (1, (c.vocab + 31) // 32)):
+            raise ValueError(f"mask: int32 [1, {(c.vocab + 31) // 32}]")
+        one = lambda v: torch.full((1,), float(v), dtype=torch.float32, device="cuda")
+        if self.controls is None:  # (graphs captured before keep their buffers)
+            self.history = torch.full((1, self.max_seq), -1, dtype=torch.int32, device="cuda")
+            self.history_len = torch.zeros(1, dtype=torch.int32, device="cuda")
+            self.controlled = torch.zeros(1, c.vocab, dtype=torch.float32, device="cuda")
+            self.controls_scratch = torch.empty(max(16, qlin.logits_controls_scratch_bytes(1, c.vocab)), dtype=torch.uint8,
+                                                device="cuda")
+        self.controls = dict(repetition=one(repetition), frequency=one(frequency), presence=one(presence), mask=mask)
+        if bias:
+            self.controls.update(
+                bias_ids=torch.tensor([list(bias)], dtype=torch.int32, device="cuda"),
+                bias_values=torch.tensor([list(bias.values())], dtype=torch.float32, device="cuda"))
 
     # ---- the calls -------------------------------------------------------------------------------
 
@@ -147,7 +188,15 @@ class Qwen2Decoder:
                 self._norm(h, xn, W["attn_norm"], rows)
                 for name, y, n in (("wq", q, QD), ("wk", k, KD), ("wv", v, KD)):
                     self._ok("matmul", L.qlin_launch_quant_matmul(c.wtype, t(W[name]), self.rb_h, xn, y, n, H, rows))
-            if fuse:
+            if c.kv8:
+                qlin.qk_norm_rope_store_kv8(self.how[i], self.kv8[i], q, QD, k, KD, v, KD, q, rows, c.n_heads, pos_ptr)
+                qlin.attend_kv8(self.kv8[i], q, attn, rows, c.n_heads, pos_ptr, None, c.head_dim ** -0.5, self.attend_ws)
+            elif c.qk_norm:
+                qlin.qk_norm_rope_store_kv(self.how[i], q, QD, k, KD, v, KD, q, self.kc[i], self.vc[i], rows, c.n_heads,
+                                           c.kv_heads, c.head_dim, self.max_seq, pos_ptr)
+                self._ok("attend", L.qlin_launch_attend(q, t(self.kc[i]), t(self.vc[i]), attn, rows, c.n_heads,
+                                                        c.kv_heads, c.head_dim, self.max_seq, pos_ptr))
+            elif fuse:
                 self._ok("rope_attend", L.qlin_launch_rope_attend(q, k, v, t(self.kc[i]), t(self.vc[i]), attn,
                                                                   c.n_heads, c.kv_heads, c.head_dim, self.max_seq,
                                                                   pos_ptr, c.theta))
@@ -175,6 +224,18 @@ class Qwen2Decoder:
         """Final norm of residual row `row`, the tied output head, and the greedy pick into token."""
         c, L, t = self.cfg, self.L, c_ptr
         hr = t(self.h) + 4 * row * c.hidden
+        if self.controls is not None:
+            if self.fuse and hr % 16 == 0:
+                qlin.rms_norm_quant_gemv_multi(c.wtype, [self.w["table"]], self.rb_h, hr, self.w["final_norm"], 0, c.eps, 0,
+                                               [self.logits], [c.vocab], c.hidden)
+            else:
+                self._norm(hr, t(self.xn), self.w["final_norm"], 1)
+                self._ok("lm_head", L.qlin_launch_quant_gemv(c.wtype, t(self.w["table"]), self.rb_h, t(self.xn),
+                                                             t(self.logits), c.vocab, c.hidden, 1))
+            qlin.logits_controls(self.logits.view(1, -1), self.controlled, 1, c.vocab, history=self.history,
+                                 history_lens=self.history_len, picks=self.token, scratch=self.controls_scratch,
+                                 **self.controls)
+            return
         if self.fuse and hr % 16 == 0:
             # the norm inside the head GEMV, and each of its workgroups' greedy pick in its epilogue (one
             # small launch reduces the picks): two launches instead of norm, GEMV and a scan of every logit
@@ -198,6 +259,9 @@ class Qwen2Decoder:
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.prompt_ids), t(self.h),
                                                                  t(self.w["table"]), self.rb_h, c.hidden, n))
         self._layers(n, t(self.zero))
+        if self.controls is not None:
+            self.history[0, :n].copy_(prompt)
+            self.history_len.fill_(n)
         self._head(n - 1)
         self.pos.fill_(n)
 
@@ -209,6 +273,9 @@ class Qwen2Decoder:
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.token), t(self.h),
                                                                  t(self.w["table"]), self.rb_h, c.hidden, 1))
         self._layers(1, t(self.pos))
+        if self.controls is not None:
+            self.history[0].scatter_(0, self.pos.long(), self.token)  # the step's token is history for its pick
+            self.torch.add(self.pos, 1, out=self.history_len)
         self._head(0)
         self.pos.add_(1)
 
