@@ -34,8 +34,9 @@ Kv8View kv8_view(const qlin_kv8_cache *c);
 
 namespace {
 
-constexpr int kWaves = 4, kTile = 16;
+constexpr int kTile = 16;
 constexpr int kMinItems = 8;  // blocks of a split, at least
+constexpr int kCus = 256;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -312,7 +313,7 @@ struct Sums {
     }
 };
 
-// A workgroup of 4 waves per (RT tiles of 16 query rows, sequence, key head, split of the positions); its waves take the
+// A workgroup of 4 or 8 waves per (RT tiles of 16 query rows, sequence, key head, split of the positions); its waves take the
 // split's blocks in turn, each with sums of its own, which meet in LDS.  A wave knows the pages of its next 64 blocks,
 // requests a block's keys while it weighs the values of the one before, and turns codes into operands for its RT tiles
 // in registers: there is no barrier before the end.
@@ -321,7 +322,7 @@ struct Sums {
 // then 4 fmas for 64 of its values, and half of the codes' 128.  (A workgroup that turned a block's codes once, into
 // LDS, for 64 rows took half of these, but one block after the other: the longest row's time, 86 us for 2011 rows of 28
 // heads, was all of it.)
-template <int HD, int RT>
+template <int HD, int RT, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, const float *__restrict__ q,
                                                                     float *__restrict__ out, int rows, int n_heads,
                                                                     const int *__restrict__ start_pos,
@@ -617,25 +618,94 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c
     }
 }
 
+// The same for at most kFewSplits splits, a wave per query row: a workgroup each would find little to do (8000 rows of
+// two splits 17 us, so 6; 112 rows of 8 splits with their attention 18.1, so 17.3; but of 16 splits 10.8, so 11.3).
+constexpr int kFewSplits = 8;
+template <int HD>
+__global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_rows_kernel(Kv8View c, float *__restrict__ out, int rows,
+                                                                            int n_heads, const int *__restrict__ start_pos,
+                                                                            const int *__restrict__ n_rows, int tiles,
+                                                                            int macro, int splits,
+                                                                            const float *__restrict__ part) {
+    constexpr int D4 = HD / 4, C = 64 / D4, kSlots = kFewSplits / C;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = (blockIdx.x * 4 + wave) % kTile;
+    const unsigned group_id = blockIdx.x / (kTile / 4);
+    const float *src = part + (static_cast<size_t>(group_id) * splits * kTile + row) * (HD + 4);
+    const size_t step = static_cast<size_t>(kTile) * (HD + 4);
+    const int cls = lane / D4, d4 = lane % D4;
+    // requested before it is known how many splits there are; what the others hold is not used
+    const float2 ml = lane < splits ? *reinterpret_cast<const float2 *>(src + lane * step + HD) : make_float2(-INFINITY, 0.0f);
+    f32x4 o[kSlots];
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u)
+        o[u] = cls < C && cls + u * C < splits ? *reinterpret_cast<const f32x4 *>(src + (cls + u * C) * step + 4 * d4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int id = group_id;
+    const int kh = id % c.kv;
+    id /= c.kv;
+    const int tile = id % tiles, seq = id / tiles;
+    const int group = n_heads / c.kv, p0 = tile * kTile;
+    const Kv8Rows w = kv8_rows(start_pos, n_rows, seq, rows, c.per * kKv8Block);
+    const int pr = p0 + row;
+    if (pr >= w.rows * group) return;
+    const Span sp = span_of(w, p0 / macro * macro, macro, group);
+    const int per = items_per_split(sp.items(), splits), used = (sp.items() + per - 1) / per;
+    if (used <= 1) return;  // written already
+    const float mi = lane < used ? ml.x : -INFINITY, li = lane < used ? ml.y : 0.0f;
+    const float mx = wave_max_dpp(mi);
+    const float f = mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : exp2_fast(mi - mx);
+    const float den = wave_sum(li * f);
+    f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u) {
+        const float fu = __shfl(f, cls + u * C, 64);
+        if (cls + u * C < used)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) num[r] = fmaf(o[u][r], fu, num[r]);
+    }
+#pragma unroll
+    for (int k = 1; k < C; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float v = __shfl(num[r], (lane + k * D4) & 63, 64);
+            if (cls == 0) num[r] += v;
+        }
+    if (lane < D4) {
+        const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) num[r] *= inv;
+        *reinterpret_cast<f32x4 *>(out + ((static_cast<size_t>(seq) * rows + pr / group) * n_heads + kh * group + pr % group) * HD + 4 * d4) = num;
+    }
+}
+
 struct Plan {
-    int rt;                 // tiles of a wave
-    int64_t tiles, groups;  // tiles of a (sequence, key head), of the launch (padded to whole workgroups)
-    int64_t work;           // workgroups of a split
+    int rt, waves;                     // tiles of a wave, waves of a workgroup
+    int64_t macros, tiles, groups;     // workgroups and tiles of a (sequence, key head), tiles of the launch
+    int64_t work;                      // workgroups of a split
     int splits;
+    size_t bytes;                      // of workspace
 };
 Plan plan_of(int n_seqs, int rows, int n_heads, int kv, int head_dim, int blocks) {
     Plan p;
     const int64_t pairs = static_cast<int64_t>(rows) * (n_heads / kv);
     p.rt = pairs > kTile && head_dim <= 128 ? 2 : 1;  // (at 192 two tiles' sums and queries do not fit a wave's registers)
-    const int64_t macros = (pairs + p.rt * kTile - 1) / (p.rt * kTile);
-    p.tiles = macros * p.rt;
-    p.work = macros * kv * n_seqs;
+    p.macros = (pairs + p.rt * kTile - 1) / (p.rt * kTile);
+    p.tiles = p.macros * p.rt;
+    p.work = p.macros * kv * n_seqs;
     p.groups = p.work * p.rt;
-    // two workgroups for every CU, but no split of less than kMinItems blocks of the longest sequence
-    const int64_t want = p.work > 0 ? (512 + p.work - 1) / p.work : 1;
+    // From a half (three quarters for single tiles) to one workgroup a CU: 8 waves each, and no splits.  384 rows of 14
+    // heads of 64 in 168 workgroups 9.2 us, in splits of 4 waves and their join 13.5; 250 rows behind 6000 positions, 32
+    // heads of 128, in 256 65, so 72; 64 sequences of 1 .. 8 thousand positions and 4 key heads 35, so 38.  Fewer
+    // leave CUs without work: 56 workgroups of 128 rows 10.5, so 9.5; 24 sequences of 8 key heads 31.7, so 29.
+    p.waves = 4 * p.work > (p.rt == 2 ? 2 : 3) * kCus && p.work <= kCus ? 8 : 4;
+    // Otherwise two workgroups of 4 waves for every CU, but no split of less than kMinItems blocks of the longest sequence,
+    // and none at all above one workgroup a CU: 512 rows of 28 heads of 128 in 448 workgroups 18.3 us, in halves 34; 48
+    // sequences of 8 key heads 48, so 50.
+    const int64_t want = p.work > 0 && p.work <= kCus && p.waves == 4 ? (2 * kCus + p.work - 1) / p.work : 1;
     const int64_t most = (blocks + kMinItems) / kMinItems;
     p.splits = static_cast<int>(want < most ? want : most);
     if (p.splits > kMaxSplits) p.splits = kMaxSplits;
+    p.bytes = p.splits > 1 ? static_cast<size_t>(p.groups) * p.splits * kTile * (static_cast<size_t>(head_dim) + 4) * sizeof(float) : 0;
     return p;
 }
 
@@ -652,8 +722,7 @@ size_t qlin_attend_kv8_workspace_bytes(int n_seqs, int rows, int n_heads, int kv
     if (n_seqs <= 0 || rows <= 0 || n_heads <= 0 || kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || blocks_per_seq <= 0)
         return 0;
     const qlin::Plan p = qlin::plan_of(n_seqs, rows, n_heads, kv_heads, head_dim, blocks_per_seq);
-    if (p.splits <= 1) return 0;
-    return static_cast<size_t>(p.groups) * p.splits * qlin::kTile * (static_cast<size_t>(head_dim) + 4) * sizeof(float);
+    return p.bytes;
 }
 
 int qlin_launch_attend_kv8(const qlin_kv8_cache *cache, const float *q, float *attn, int rows, int n_heads,
@@ -678,26 +747,32 @@ int qlin_launch_attend_kv8(const qlin_kv8_cache *cache, const float *q, float *a
     const float q_scale = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
     float *part = static_cast<float *>(workspace);
     const qlin::Kv8View view = qlin::kv8_view(cache);
-    auto go = [&](auto attend, auto join) {
-        hipLaunchKernelGGL(attend, dim3(static_cast<unsigned>(grid)), dim3(64 * qlin::kWaves), 0, qlin::current_stream(),
-                           view, q, attn, rows, n_heads, start_pos_dev, n_rows_dev, q_scale,
-                           static_cast<int>(p.tiles / p.rt), p.splits, part);
+    auto go = [&](auto attend, auto join, auto join_rows) {
+        hipLaunchKernelGGL(attend, dim3(static_cast<unsigned>(grid)), dim3(64 * p.waves), 0, qlin::current_stream(), view, q,
+                           attn, rows, n_heads, start_pos_dev, n_rows_dev, q_scale, static_cast<int>(p.macros),
+                           p.splits, part);
         if (hipGetLastError() != hipSuccess) return QLIN_ERR_LAUNCH;
         if (p.splits > 1) {
-            hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(p.groups * qlin::kTile)), dim3(qlin::kJoinThreads), 0,
-                               qlin::current_stream(), view, attn, rows, n_heads, start_pos_dev, n_rows_dev,
+            const bool few = p.splits <= qlin::kFewSplits;
+            hipLaunchKernelGGL(few ? join_rows : join, dim3(static_cast<unsigned>(p.groups * qlin::kTile / (few ? 4 : 1))),
+                               dim3(qlin::kJoinThreads), 0, qlin::current_stream(), view, attn, rows, n_heads, start_pos_dev, n_rows_dev,
                                static_cast<int>(p.tiles), p.rt * qlin::kTile, p.splits, part);
             if (hipGetLastError() != hipSuccess) return QLIN_ERR_LAUNCH;
         }
         return QLIN_OK;
     };
+#define QLIN_GO(HD, RT)                                                                                          \
+    return go(p.rt == 1 ? p.waves == 4 ? qlin::attend_kv8_kernel<HD, 1, 4> : qlin::attend_kv8_kernel<HD, 1, 8>   \
+              : p.waves == 4 ? qlin::attend_kv8_kernel<HD, RT, 4> : qlin::attend_kv8_kernel<HD, RT, 8>,          \
+              qlin::attend_kv8_join_kernel<HD>, qlin::attend_kv8_join_rows_kernel<HD>)
     switch (hd) {
-        case 64: return go(p.rt == 2 ? qlin::attend_kv8_kernel<64, 2> : qlin::attend_kv8_kernel<64, 1>, qlin::attend_kv8_join_kernel<64>);
-        case 96: return go(p.rt == 2 ? qlin::attend_kv8_kernel<96, 2> : qlin::attend_kv8_kernel<96, 1>, qlin::attend_kv8_join_kernel<96>);
-        case 128: return go(p.rt == 2 ? qlin::attend_kv8_kernel<128, 2> : qlin::attend_kv8_kernel<128, 1>, qlin::attend_kv8_join_kernel<128>);
-        case 192: return go(qlin::attend_kv8_kernel<192, 1>, qlin::attend_kv8_join_kernel<192>);
-        default: return go(qlin::attend_kv8_kernel<256, 1>, qlin::attend_kv8_join_kernel<256>);
+        case 64: QLIN_GO(64, 2);
+        case 96: QLIN_GO(96, 2);
+        case 128: QLIN_GO(128, 2);
+        case 192: QLIN_GO(192, 1);
+        default: QLIN_GO(256, 1);
     }
+#undef QLIN_GO
 }
 
 }  // extern "C"

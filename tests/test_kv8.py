@@ -719,6 +719,30 @@ def test_attend_in_splits(rows, heads, kv, d, length):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,rows,heads,kv,d,per", [
+    (52, 1, 8, 4, 64, 9), (51, 2, 8, 4, 192, 5), (6, 70, 8, 2, 256, 6), (20, 37, 6, 2, 64, 7), (5, 70, 12, 4, 128, 9),
+    (40, 31, 4, 4, 96, 5), (70, 1, 12, 4, 64, 30), (80, 19, 4, 4, 128, 5), (24, 1, 8, 4, 128, 40), (13, 3, 24, 4, 64, 60),
+    (12, 5, 16, 2, 96, 50), (20, 1, 4, 4, 192, 70), (9, 2, 8, 4, 256, 70), (40, 1, 7, 1, 64, 140)])
+def test_attend_many_sequences(n, rows, heads, kv, d, per):
+    """Few and many rows of few and many sequences, from one block to all of them: each number of waves, splits and the
+    joins of few and of many."""
+    torch = _gpu()
+    from gpu_util import banner
+    rng = np.random.default_rng(n * rows + d)
+    table = rng.permutation(n * per + 3)[:n * per].reshape(n, per)
+    table[rng.random(table.shape) < 0.05] = -1
+    ref = _filled(rng, n, per, kv, d, table, n * per + 3)
+    cache = _device_cache(torch, ref, paged=True)
+    starts = [int(x) for x in rng.integers(0, per * BLOCK - rows + 1, n)]
+    starts[0], starts[-1] = per * BLOCK - rows, 0
+    counts = [int(x) for x in rng.integers(0, rows + 1, n)]
+    counts[0] = rows
+    banner(f"attend n={n} rows={rows} heads={heads}/{kv} d={d} per={per}")
+    q = rng.standard_normal((n, rows, heads, d)).astype(np.float32)
+    _check_attend(torch, ref, cache, q, starts, counts, heads, d ** -0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 40, 100])
 def test_attend_odd_values(rows):
     """What a row does not see does not reach it, NaN and infinities among it; what it sees does."""
