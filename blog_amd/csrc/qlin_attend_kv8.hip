@@ -740,7 +740,7 @@ int qlin_launch_attend_kv8(const qlin_kv8_cache *cache, const float *q, float *a
     if (static_cast<int64_t>(rows) * (n_heads / kv) > 1 << 30) return QLIN_ERR_LIMIT;
     const qlin::Plan p = qlin::plan_of(cache->n_seqs, rows, n_heads, kv, hd, cache->blocks_per_seq);
     const int64_t grid = p.work * p.splits;
-    if (grid > (1 << 23) || p.groups * qlin::kTile > (1 << 23)) return QLIN_ERR_LIMIT;
+    if (grid > (1 << 23) || (p.splits > 1 && p.groups * qlin::kTile > (1 << 23))) return QLIN_ERR_LIMIT;
     const size_t need = qlin_attend_kv8_workspace_bytes(cache->n_seqs, rows, n_heads, kv, hd, cache->blocks_per_seq);
     if (need > 0 && !workspace) return QLIN_ERR_NULL;
     if (workspace_bytes < need) return QLIN_ERR_LIMIT;

@@ -127,7 +127,7 @@ class Qwen2Decoder:
         self.pos = torch.zeros(1, dtype=i32, device=dev)        # the next step's position
         self.zero = torch.zeros(1, dtype=i32, device=dev)
         self.L = qlin.lib()
-        self.controls = None
+        self.controls, self.captured = None, []
         if cfg.qk_norm or cfg.kv8:
             qlin.set_stream(torch.cuda.current_stream())
             self.rotation = torch.empty(max_seq, cfg.head_dim, dtype=f32, device=dev)
@@ -141,14 +141,18 @@ class Qwen2Decoder:
             self.attend_ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
 
     def set_controls(self, repetition=1.0, frequency=0.0, presence=0.0, bias=None, mask=None) -> None:
-        """From the next pick on (and in every graph captured after this): penalties for the tokens of the prompt and
-        those picked since the last prefill, a bias {token: value}, and a mask (int32 words, 32 tokens each, a bit set for
-        a token that may follow; the tensor is read at every pick, so a grammar rewrites it between steps)."""
+        """From the next pick on: penalties for the tokens of the prompt and those picked since (call it before the prefill;
+        tokens that came before the first call are not counted), a bias {token: value}, and a mask (int32 words, 32 tokens
+        each, a bit set for a token that may follow; the tensor is read at every pick, so a grammar rewrites it between
+        steps).  A graph keeps the controls that it was captured with."""
         torch, c = self.torch, self.cfg
-        if mask is not None and (mask.dtype != torch.int32 or tuple(mask.shape) != (1, (c.vocab + 31) // 32)):
-            raise ValueError(f"mask: int32 [1, {(c.vocab + 31) // 32}]")
+        if not repetition > 0:
+            raise ValueError(f"repetition {repetition}: must be above 0")
+        if mask is not None and (mask.dtype != torch.int32 or tuple(mask.shape) != (1, (c.vocab + 31) // 32)
+                                 or not mask.is_contiguous() or mask.device != self.token.device):
+            raise ValueError(f"mask: contiguous int32 [1, {(c.vocab + 31) // 32}] on the decoder's device")
         one = lambda v: torch.full((1,), float(v), dtype=torch.float32, device="cuda")
-        if self.controls is None:  # (graphs captured before keep their buffers)
+        if self.controls is None:
             self.history = torch.full((1, self.max_seq), -1, dtype=torch.int32, device="cuda")
             self.history_len = torch.zeros(1, dtype=torch.int32, device="cuda")
             self.controlled = torch.zeros(1, c.vocab, dtype=torch.float32, device="cuda")
@@ -225,6 +229,8 @@ class Qwen2Decoder:
         c, L, t = self.cfg, self.L, c_ptr
         hr = t(self.h) + 4 * row * c.hidden
         if self.controls is not None:
+            if self.torch.cuda.is_current_stream_capturing():
+                self.captured.append(self.controls)  # (the graph reads these tensors)
             if self.fuse and hr % 16 == 0:
                 qlin.rms_norm_quant_gemv_multi(c.wtype, [self.w["table"]], self.rb_h, hr, self.w["final_norm"], 0, c.eps, 0,
                                                [self.logits], [c.vocab], c.hidden)
@@ -274,7 +280,8 @@ class Qwen2Decoder:
                                                                  t(self.w["table"]), self.rb_h, c.hidden, 1))
         self._layers(1, t(self.pos))
         if self.controls is not None:
-            self.history[0].scatter_(0, self.pos.long(), self.token)  # the step's token is history for its pick
+            # the step's token is history for its pick (past the last position the row there is taken, as in the caches)
+            self.history[0].scatter_(0, self.pos.long().clamp_(max=self.max_seq - 1), self.token)
             self.torch.add(self.pos, 1, out=self.history_len)
         self._head(0)
         self.pos.add_(1)

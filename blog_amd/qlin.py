@@ -303,6 +303,8 @@ def kv8_record_bytes(head_dim):
 
 def rope_table(table, theta):
     """Fills table ([n_pos, rotary_dim] f32) with the cosines and sines of every position."""
+    if table.element_size() != 4 or not table.is_contiguous():
+        raise ValueError("the table is contiguous f32")
     call("qlin_launch_rope_table", table, table.shape[0], table.shape[1], theta)
 
 
@@ -311,6 +313,11 @@ class QkRope:
     rotation table [positions, rotary_dim] (None: no rotation).  Holds on to the tensors."""
 
     def __init__(self, q_norm, k_norm, norm_type, eps, one_plus, table, rotary_dim, pairing=0):
+        if table is not None and (table.element_size() != 4 or not table.is_contiguous() or table.shape[1] != rotary_dim):
+            raise ValueError(f"a table {tuple(table.shape)} of {table.dtype} for rotary_dim {rotary_dim}: contiguous f32 rows of it")
+        for w in (q_norm, k_norm):
+            if hasattr(w, "data_ptr") and (w.element_size() != 2 or not w.is_contiguous()):
+                raise ValueError("norm weights are contiguous and of 16 bits")
         self.tensors = (q_norm, k_norm, table)
         self.args = QkRopeArgs(ptr(q_norm), ptr(k_norm), norm_type, eps, int(one_plus), ptr(table),
                                table.shape[0] if table is not None else 0, rotary_dim, pairing)
@@ -326,9 +333,11 @@ class Kv8Cache:
         n_seqs, kv_heads, _, ring, head_dim = recent.shape
         if ring != KV8_RECENT or tuple(pages.shape[1:]) != (kv_heads, kv8_record_bytes(head_dim)):
             raise ValueError(f"pages {tuple(pages.shape)} and recent {tuple(recent.shape)} are not one cache's")
-        for name, t in (("pages", pages), ("recent", recent), ("block_table", block_table)):
+        for name, t, size in (("pages", pages, 1), ("recent", recent, 4), ("block_table", block_table, 4)):
             if t is not None and not t.is_contiguous():
                 raise ValueError(f"{name} is not contiguous")
+            if t is not None and t.element_size() != size:
+                raise ValueError(f"{name} has elements of {t.element_size()} bytes, not of {size}")
         if block_table is not None:
             if block_table.shape[0] != n_seqs:
                 raise ValueError(f"a block table of {block_table.shape[0]} sequences for {n_seqs}")
@@ -392,6 +401,13 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
     """Penalties, biases and a mask on logits [rows, >= vocab] into out (which may be logits), and the greedy picks.
     history [rows, max_history], bias_ids / bias_values [rows, max_bias] and mask [rows, words] (32 tokens a word) are
     2-D and contiguous; scratch: a uint8 tensor of logits_controls_scratch_bytes(...), needed with picks."""
+    if vocab > 1 and not logits.stride(1) == out.stride(1) == 1:
+        raise ValueError("a row of logits is contiguous")
+    for t in (history, bias_ids, bias_values, mask):
+        if t is not None and not t.is_contiguous():
+            raise ValueError("history, biases and mask are contiguous")
+    if bias_ids is not None and bias_values is not None and bias_ids.numel() != bias_values.numel():
+        raise ValueError("a value for each biased token")
     a = _LOGITS_CONTROLS.pack(
         _at(history) or 0, _at(history_lens) or 0, _at(repetition) or 0, _at(frequency) or 0, _at(presence) or 0,
         _at(bias_ids) or 0, _at(bias_values) or 0, _at(mask) or 0, 0 if mask is None else mask.size(1),

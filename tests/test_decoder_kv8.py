@@ -178,6 +178,59 @@ def test_captured_step_replays_as_the_eager_one(controls):
     assert got == tokens
 
 
+def test_a_graph_keeps_the_controls_it_was_captured_with():
+    """A step captured under one set of controls, replayed after others were set (and their memory used again)."""
+    torch = _env()
+    from gpu_util import banner
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    cfg = _config(qk_norm=True, kv8=True)
+    w = make_weights(torch, cfg, seed=8)
+    prompt = torch.randint(0, cfg.vocab, (20,), dtype=torch.int32, device="cuda",
+                           generator=torch.Generator(device="cuda").manual_seed(9))
+    banner("controls of a captured step")
+    words = (cfg.vocab + 31) // 32
+    odd = lambda: torch.full((1, words), 0x2AAAAAAA, dtype=torch.int32, device="cuda")  # odd tokens, but for the words' last
+    eager, dec = (Qwen2Decoder(torch, cfg, w, max_seq=64, max_prompt=32) for _ in range(2))
+    for d in (eager, dec):
+        d.set_controls(repetition=1.3, presence=0.5, bias={3: 2.0, 9: 1.0}, mask=odd())
+    tokens = eager.generate(prompt, 12)
+    assert all(t % 2 == 1 for t in tokens)
+    dec.prefill(prompt)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dec.step()
+    qlin.set_stream(torch.cuda.current_stream())
+    dec.set_controls(repetition=0.9)
+    filler = [torch.full((n,), 0x7F7F7F7F, dtype=torch.int32, device="cuda") for n in [1, 1, 1, 2, 2, words] * 8]
+    got = [int(dec.token.item())]
+    for _ in range(11):
+        g.replay()
+        torch.cuda.synchronize()
+        got.append(int(dec.token.item()))
+    assert got == tokens
+    del filler
+    for bad in (dict(repetition=0.0), dict(repetition=-1.0), dict(mask=odd().cpu()), dict(mask=odd().long()), dict(mask=odd()[:, 1:])):
+        with pytest.raises(ValueError):
+            dec.set_controls(**bad)
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_steps_past_the_last_position(kv8):
+    """As without controls: the last position is taken again."""
+    torch = _env()
+    from gpu_util import banner
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    cfg = _config(qk_norm=True, kv8=kv8)
+    w = make_weights(torch, cfg, seed=8)
+    banner(f"steps past the last position, kv8={kv8}")
+    dec = Qwen2Decoder(torch, cfg, w, max_seq=32, max_prompt=32)
+    dec.set_controls(frequency=0.2)
+    tokens = dec.generate(torch.arange(30, dtype=torch.int32, device="cuda"), 8)
+    assert all(0 <= t < cfg.vocab for t in tokens) and int(dec.pos.item()) == 37
+    assert torch.isfinite(dec.logits).all()
+
+
 def test_graphs_that_share_a_workspace():
     """Two captured attentions (one row over a long cache, many rows) and a captured pick that share one workspace, replayed in
     turns between eager calls that use it too: bit for bit the eager results, whatever the workspace held."""

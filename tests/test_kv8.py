@@ -325,6 +325,26 @@ def test_python_cache_checks_its_tensors():
         qlin.Kv8Cache(c.pages, c.recent, torch.zeros(4, 2, dtype=torch.int32).t())
 
 
+def test_python_tensors_of_other_types():
+    import torch
+    c = qlin.Kv8Cache.empty(torch, 2, 3, 64, 100, device="cpu")
+    with pytest.raises(ValueError):
+        qlin.Kv8Cache(c.pages, c.recent, torch.zeros(2, 4, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        qlin.Kv8Cache(c.pages.to(torch.int16), c.recent, None, 4)
+    with pytest.raises(ValueError):
+        qlin.Kv8Cache(c.pages, c.recent.half(), None, 4)
+    table, w = torch.zeros(100, 64), torch.ones(64, dtype=torch.bfloat16)
+    assert qlin.QkRope(w, w, 0, 1e-6, 0, table, 64).args.table_len == 100
+    for bad in (dict(table=table.half()), dict(table=torch.zeros(100, 32)), dict(table=torch.zeros(64, 100).t()),
+                dict(q_norm=w.float()), dict(k_norm=torch.ones(128, dtype=torch.float16)[::2])):
+        a = {**dict(q_norm=w, k_norm=w, norm_type=0, eps=1e-6, one_plus=0, table=table, rotary_dim=64), **bad}
+        with pytest.raises(ValueError):
+            qlin.QkRope(**a)
+    with pytest.raises(ValueError):
+        qlin.rope_table(torch.zeros(64, 100).t(), 1e4)
+
+
 # ---- GPU ---------------------------------------------------------------------------------------
 
 def _gpu():
@@ -526,6 +546,21 @@ def test_store_token_by_token_gives_the_prompts_bytes():
     for other in got[1:]:
         for a, b in zip(got[0], other):
             assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_store_of_another_sequence_over_a_longer_one():
+    """From position 0, and from a block's first position, after more positions were stored."""
+    torch = _gpu()
+    rng = np.random.default_rng(77)
+    ref, heads = Cache(2, 7, 2, 64), 4
+    cache = _device_cache(torch, ref, paged=False)
+    how = _norm_args(rng, 64, 64, 7 * BLOCK)
+    for starts, rows in (([0, 0], 203), ([0, 32], 7), ([7, 39], 1), ([8, 40], 90), ([0, 96], 64), ([64, 160], 5)):
+        _store(torch, ref, cache, rng, starts, rows, None, heads, how)
+        _check_cache(ref, cache)
+        q = rng.standard_normal((2, rows, heads, 64)).astype(np.float32)
+        _check_attend(torch, ref, cache, q, starts, None, heads, 0.125)
 
 
 @pytest.mark.gpu

@@ -78,6 +78,17 @@ def test_validation():
     assert qlin.logits_controls_scratch_bytes(0, 5) == 0 and qlin.logits_controls_scratch_bytes(5, -1) == 0
 
 
+def test_python_layouts():
+    import torch
+    x, wide = torch.zeros(2, 64), torch.zeros(2, 128)
+    ids = torch.zeros(2, 8, dtype=torch.int32)
+    for kw in (dict(logits=wide[:, ::2]), dict(out=wide[:, ::2]), dict(history=ids[:, ::2]), dict(mask=ids[:, :2]),
+               dict(bias_ids=ids[:, :4], bias_values=x[:, :4].contiguous()),
+               dict(bias_ids=ids, bias_values=x[:, :8]), dict(bias_ids=ids, bias_values=x)):
+        with pytest.raises(ValueError):
+            qlin.logits_controls(**{**dict(logits=x, out=x, rows=2, vocab=64), **kw})
+
+
 # ---- GPU ---------------------------------------------------------------------------------------
 
 def _gpu():
