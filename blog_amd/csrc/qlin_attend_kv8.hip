@@ -321,7 +321,9 @@ struct Sums {
 // VALU; of a tile's 32 x 16 scores, 8 a lane, each costs an fma, an exp, a sum and 2 instructions for its operands,
 // then 4 fmas for 64 of its values, and half of the codes' 128.  (A workgroup that turned a block's codes once, into
 // LDS, for 64 rows took half of these, but one block after the other: the longest row's time, 86 us for 2011 rows of 28
-// heads, was all of it.)
+// heads, was all of it.  Codes turned once for all, by a launch before: 92 us, and 2.5 to 5 more for fewer rows.)
+// Heads of 128, 28 over 4: one row over 32002 positions 11.4 us, 2.9 TB/s; 24 rows over up to 8000 27.4, 4.1 TB/s; 2011
+// rows 87.5, 331 TFLOP/s (of one product each; two are made).  32 over 8: 250 rows behind 6000 64.7, 388 TFLOP/s.
 template <int HD, int RT, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, const float *__restrict__ q,
                                                                     float *__restrict__ out, int rows, int n_heads,
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
     }
 }
 
-// A workgroup per query row: the splits' sums joined.  Each wave finds the splits' weights (a split a lane), and each
+// A workgroup per query row: the splits' sums joined (28 rows of 126 splits 4.6 us: the launch and three dependent loads).  Each wave finds the splits' weights (a split a lane), and each
 // thread adds four dims of every C-th split, eight in flight.
 constexpr int kJoinThreads = 256;
 constexpr int kMaxSplits = 128;

@@ -155,7 +155,8 @@ __device__ __forceinline__ void norm_and_turn(f32x4v &va, f32x4v &vb, const Runs
 constexpr int kThreads = 256;
 constexpr f32x4v kZero4 = {0.0f, 0.0f, 0.0f, 0.0f};
 
-// A group of lanes for each query, key and value head of each row.
+// A group of lanes for each query, key and value head of each row.  Bound by bytes: 1877 rows of 28 + 4 + 4 heads of 128
+// 15.1 us, 4.6 TB/s; one row 2.4 us, the launch.
 template <int T>
 __global__ __launch_bounds__(kThreads) void norm_rope_store_kernel(qlin_qk_rope how, const float *q, size_t q_stride,
                                                                    const float *__restrict__ k, size_t k_stride,
@@ -223,6 +224,9 @@ __device__ __forceinline__ int code_of(float x, float scale) {
 // heads.  A block's workgroup holds its 32 rows of keys and values in registers, takes the rows that came earlier from
 // the ring, writes the new rows of the last two blocks there, and, if the block is complete, its codes (through LDS,
 // in the record's order) and scales.
+//
+// Bound by the queries' bytes (2011 rows of 28 + 4 + 4 heads of 128 15.0 us, 4.5 TB/s), for few rows by a block's chain: table
+// row and norm, largest value, codes through LDS (24 sequences of one row 6.0 us).
 //
 // The first block's workgroup reads ring rows; the block two (or 2i) further that would overwrite them is its second
 // job, after that read, so that no other workgroup writes what it reads.
@@ -363,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
 }
 
 // A workgroup per (sequence, key head, 32 rows): a thread per 4 dims of a row.  Its rows lie in two blocks at most, whose
-// pages are requested first.
+// pages are requested first.  Bound by the chain page, code, store: 2011 rows of 4 heads of 128 5.3 us, 24 blocks 3.8.
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(Kv8View c, int hd, const int *__restrict__ first,
                                                             const int *__restrict__ lens, int count, int parts,
                                                             float *__restrict__ k_out, float *__restrict__ v_out) {
