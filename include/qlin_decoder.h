@@ -85,8 +85,8 @@ extern "C" {
  *   - recent holds the last positions in f32: [seq][key head][keys, values][64][head_dim], position p in row p % 64.
  *     The open block (the positions after the last complete block) is read from there.
  * So what a position's code is does not depend on whether its block came as a prompt or token by token, and
- * positions may be taken back: a store may start where the last one ended, up to 32 positions before the furthest end
- * of an earlier one (drafted tokens that were rejected), or at a block's first position (0: another sequence).
+ * positions may be taken back: a store may start at a block's first position (0: another sequence), and from then on up
+ * to 32 positions before the furthest end since (drafted tokens that were rejected), but not before that start.
  * A page number that is negative or >= n_pages, or a position outside [0, capacity), is not stored, and is not
  * seen by attention (a page taken out of the table is out of every score).  Sequences may share pages that none
  * of them is storing to.
