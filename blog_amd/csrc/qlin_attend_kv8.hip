@@ -695,15 +695,21 @@ Plan plan_of(int n_seqs, int rows, int n_heads, int kv, int head_dim, int blocks
     p.tiles = p.macros * p.rt;
     p.work = p.macros * kv * n_seqs;
     p.groups = p.work * p.rt;
-    // From a half (three quarters for single tiles) to one workgroup a CU: 8 waves each, and no splits.  384 rows of 14
-    // heads of 64 in 168 workgroups 9.2 us, in splits of 4 waves and their join 13.5; 250 rows behind 6000 positions, 32
-    // heads of 128, in 256 65, so 72; 64 sequences of 1 .. 8 thousand positions and 4 key heads 35, so 38.  Fewer
-    // leave CUs without work: 56 workgroups of 128 rows 10.5, so 9.5; 24 sequences of 8 key heads 31.7, so 29.
-    p.waves = 4 * p.work > (p.rt == 2 ? 2 : 3) * kCus && p.work <= kCus ? 8 : 4;
-    // Otherwise two workgroups of 4 waves for every CU, but no split of less than kMinItems blocks of the longest sequence,
-    // and none at all above one workgroup a CU: 512 rows of 28 heads of 128 in 448 workgroups 18.3 us, in halves 34; 48
-    // sequences of 8 key heads 48, so 50.
-    const int64_t want = p.work > 0 && p.work <= kCus && p.waves == 4 ? (2 * kCus + p.work - 1) / p.work : 1;
+    // Splits fill CUs that are idle, or that a longer sequence's workgroup keeps waiting for, and cost a join.  They pay where
+    // that waiting is long, in caches of more than 64 blocks, unless a single sequence's workgroups, all alike, fill 7/8 of
+    // the chip by themselves.  (Where they do not pay: 512 rows of 28 heads of 128 in 448 workgroups behind 2500 positions 62 us,
+    // in halves 75; 48 sequences of up to 1000 positions and 8 key heads 20, so 29.  Where they do: these sequences of up to
+    // 12000 129, so 157; 320 rows in 280 behind 8000 125, so 145.)
+    const bool few = blocks <= 64;
+    auto fill = [&](int64_t slots) { return n_seqs == 1 && 8 * p.work >= 7 * slots; };
+    // Not split: 8 waves, a workgroup a CU, from a half (three quarters for single tiles) to one workgroup a CU.  384 rows of
+    // 14 heads of 64 in 168 workgroups 9.2 us, in splits of 4 waves 13.5; 250 rows behind 6000 positions, 32 heads of 128, in
+    // 256 65, so 72; 60 sequences of up to 1000 and 4 key heads 17, so 24.  With fewer workgroups CUs have no work: 56 of 128 rows
+    // 10.5, so 9.5; in longer caches 24 sequences of 5 rows and up to 8000 84, so 60.
+    p.waves = 4 * p.work > (p.rt == 2 ? 2 : 3) * kCus && p.work <= kCus && (few || fill(kCus)) ? 8 : 4;
+    const bool one = p.waves == 8 || p.work > 2 * kCus || (p.work > kCus && (few || fill(2 * kCus)));
+    // Otherwise two workgroups for every CU, but no split of less than kMinItems blocks of the longest sequence.
+    const int64_t want = p.work > 0 && !one ? (2 * kCus + p.work - 1) / p.work : 1;
     const int64_t most = (blocks + kMinItems) / kMinItems;
     p.splits = static_cast<int>(want < most ? want : most);
     if (p.splits > kMaxSplits) p.splits = kMaxSplits;

@@ -778,6 +778,23 @@ def test_attend_many_sequences(n, rows, heads, kv, d, per):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,rows,heads,kv,d", [(1, 250, 32, 8, 64), (1, 420, 28, 4, 64), (1, 500, 32, 8, 64), (70, 1, 12, 4, 64),
+                                               (66, 1, 4, 4, 192), (48, 6, 12, 4, 128), (1, 110, 8, 2, 256), (80, 7, 12, 4, 96)])
+def test_attend_long_caches(n, rows, heads, kv, d):
+    """More than 64 blocks, with as many workgroups as CUs, more and fewer: split and not."""
+    torch = _gpu()
+    from gpu_util import banner
+    rng = np.random.default_rng(n * rows + d)
+    per = 72
+    ref = _filled(rng, n, per, kv, d, rng.permutation(n * per).reshape(n, per), n * per)
+    cache = _device_cache(torch, ref, paged=True)
+    starts = [per * BLOCK - rows - 5] + [int(x) for x in rng.integers(0, per * BLOCK - rows, n - 1)]
+    banner(f"attend n={n} rows={rows} heads={heads}/{kv} d={d} start={starts[0]}")
+    q = rng.standard_normal((n, rows, heads, d)).astype(np.float32)
+    _check_attend(torch, ref, cache, q, starts, None, heads, d ** -0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 40, 100])
 def test_attend_odd_values(rows):
     """What a row does not see does not reach it, NaN and infinities among it; what it sees does."""
