@@ -401,17 +401,28 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
     """Penalties, biases and a mask on logits [rows, >= vocab] into out (which may be logits), and the greedy picks.
     history [rows, max_history], bias_ids / bias_values [rows, max_bias] and mask [rows, words] (32 tokens a word) are
     2-D and contiguous; scratch: a uint8 tensor of logits_controls_scratch_bytes(...), needed with picks."""
-    if vocab > 1 and not logits.stride(1) == out.stride(1) == 1:
+    # (strides and sizes as whole tuples: stride(0) or size(1) take 0.15 us longer each)
+    row, one = logits.stride()
+    out_row, out_one = out.stride()
+    if not one == out_one == 1 and vocab > 1:
         raise ValueError("a row of logits is contiguous")
-    for t in (history, bias_ids, bias_values, mask):
-        if t is not None and not t.is_contiguous():
-            raise ValueError("history, biases and mask are contiguous")
-    if bias_ids is not None and bias_values is not None and bias_ids.numel() != bias_values.numel():
-        raise ValueError("a value for each biased token")
+    words = max_history = max_bias = 0
+    if mask is not None:
+        words = mask.shape[1]
+        if not mask.is_contiguous():
+            raise ValueError("the mask is not contiguous")
+    if history is not None:
+        max_history = history.shape[1]
+        if not history.is_contiguous():
+            raise ValueError("the history is not contiguous")
+    if bias_ids is not None:
+        max_bias = bias_ids.shape[1]
+        if not bias_ids.is_contiguous() or bias_values is not None and (
+                not bias_values.is_contiguous() or bias_values.shape != bias_ids.shape):
+            raise ValueError("biases: tokens and values of one shape, contiguous")
     a = _LOGITS_CONTROLS.pack(
         _at(history) or 0, _at(history_lens) or 0, _at(repetition) or 0, _at(frequency) or 0, _at(presence) or 0,
-        _at(bias_ids) or 0, _at(bias_values) or 0, _at(mask) or 0, 0 if mask is None else mask.size(1),
-        0 if history is None else history.size(1), 0 if bias_ids is None else bias_ids.size(1))
+        _at(bias_ids) or 0, _at(bias_values) or 0, _at(mask) or 0, words, max_history, max_bias)
     _done("qlin_launch_logits_controls", _lib_of().qlin_launch_logits_controls(
-        a, logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, _at(picks),
-        _at(scratch), 0 if scratch is None else scratch.numel()))
+        a, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, _at(picks), _at(scratch),
+        0 if scratch is None else scratch.numel()))
