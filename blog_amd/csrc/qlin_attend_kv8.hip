@@ -44,8 +44,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ f32x4 mfma16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// No instructions in inline assembly here: the compiler does not see what it does to registers that an MFMA is still writing (byte-select
-// conversions, 1 instruction a code, wrote such a register before its MFMA's unused lanes did).
+// No instructions in inline assembly here: the compiler does not see what they do to registers that an MFMA is still
+// writing (byte-select conversions, 1 instruction a code, wrote such a register before its MFMA's unused lanes did).
 // 1024 + 128 + code, in fp16, less 1152
 __device__ __forceinline__ uint32_t less_1152(uint32_t biased) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, biased) + f16x2{-1152.0f16, -1152.0f16});
@@ -525,8 +525,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
     }
 }
 
-// A workgroup per query row: the splits' sums joined (28 rows of 126 splits 4.6 us: the launch and three dependent loads).  Each wave finds the splits' weights (a split a lane), and each
-// thread adds four dims of every C-th split, eight in flight.
+// A workgroup per query row: the splits' sums joined (28 rows of 126 splits 4.6 us: the launch and three dependent
+// loads).  Each wave finds the splits' weights (a split a lane), and each thread adds four dims of every C-th split, four
+// in flight.
 constexpr int kJoinThreads = 256;
 constexpr int kMaxSplits = 128;
 template <int HD>
