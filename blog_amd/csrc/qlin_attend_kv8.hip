@@ -171,8 +171,23 @@ constexpr float kUp = 11.0f, kSlack = 4.0f;  // (2^15 at most, in fp16)
 template <int HD>
 struct Sums {
     static constexpr int NT = (HD + 63) / 64;
-    f32x4 o[NT][4];    // of query row n: [i][j][r] is dim 64 i + 16 g + 4 r + j (past HD: zeros)
+    // Of query row n: [i][j][r] is dim 64 i + 16 g + 4 r + j, from the values' dims 64 i + 4n + j in lane n.  Of a head of 96
+    // the last 32 are [i][j < 2][r], 64 i + 16 (g % 2) + 4 r + 2 (g / 2) + j, from 64 i + 4 (n % 8) + 2 (n / 8) + j: half the
+    // products (as 64 dims, 32 of them zeros, 1000 rows of 28 heads behind 500 positions took 55 us, so 44.5).
+    f32x4 o[NT][4];
     float m, l;
+    static constexpr bool half(int i) { return 64 * (i + 1) > HD; }
+    static constexpr int js(int i) { return half(i) ? 2 : 4; }
+    static __device__ __forceinline__ int dim_of(int i, int g, int r) {
+        return half(i) ? 64 * i + 16 * (g & 1) + 4 * r + 2 * (g >> 1) : 64 * i + 16 * g + 4 * r;
+    }
+    static __device__ __forceinline__ int value_dim(int i, int n) { return half(i) ? 64 * i + 4 * (n & 7) + 2 * (n >> 3) : 64 * i + 4 * n; }
+    // 4 dims there, of the last 32 of 96 two
+    static __device__ __forceinline__ f32x4 dims_at(int i, const float *p) {
+        if (!half(i)) return *reinterpret_cast<const f32x4 *>(p);
+        const f32x2 x = *reinterpret_cast<const f32x2 *>(p);
+        return f32x4{x[0], x[1], 0.0f, 0.0f};
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -191,7 +206,7 @@ struct Sums {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < js(i); ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[i][j][r] *= al;
             m = mx;
@@ -269,16 +284,17 @@ struct Sums {
         }
         l += groups_sum((s[0] + s[1]) + (s[2] + s[3]));
         bool odd = false;  // a value that is not finite
-        f32x4 v[4][NT];    // dims 64 i + 4n .. + 3 of position 4g + r
+        f32x4 v[4][NT];    // dims value_dim .. of position 4g + r
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int pos = base + 4 * g + r;
-            const float *vrow = vr + static_cast<size_t>(pos % kKv8Recent) * HD + 4 * n;
+            const float *vrow = vr + static_cast<size_t>(pos % kKv8Recent) * HD;
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                v[r][i] = pos < len && 64 * i + 4 * n < HD ? *reinterpret_cast<const f32x4 *>(vrow + 64 * i) : zero;
+                v[r][i] = zero;
+                if (pos < len) v[r][i] = dims_at(i, vrow + value_dim(i, n));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) odd |= !isfinite(v[r][i][j]);
+                for (int j = 0; j < js(i); ++j) odd |= !isfinite(v[r][i][j]);
             }
         }
         if (base + 15 > first && __any(odd)) {  // uniform: 0 times that value, for a row that does not see it, would be NaN
@@ -291,10 +307,9 @@ struct Sums {
                     for (int i = 0; i < NT; ++i)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const int d = 64 * i + 16 * g + 4 * r;
-                            const f32x4 y = d < HD ? *reinterpret_cast<const f32x4 *>(vrow + d) : zero;
+                            const f32x4 y = dims_at(i, vrow + dim_of(i, g, r));
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) o[i][j][r] = fmaf(p, y[j], o[i][j][r]);
+                            for (int j = 0; j < js(i); ++j) o[i][j][r] = fmaf(p, y[j], o[i][j][r]);
                         }
                 }
             }
@@ -302,7 +317,7 @@ struct Sums {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < js(i); ++j) {
                     f32x4 x = zero;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) x = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i][j], s[r], x, 0, 0, 0);
@@ -379,9 +394,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd)  // dims 64 i + 4n .. + 3 of positions 4g + odd, + 2, 16 + 4g + odd, + 2
-                vc[i][odd] = 64 * (i + 1) <= HD || 64 * i + 4 * n < HD
-                                 ? *reinterpret_cast<const u32x4 *>(rec + kv8_value_byte(4 * g + odd, 64 * i + 4 * n, HD))
-                                 : u32x4{0u, 0u, 0u, 0u};
+                vc[i][odd] = *reinterpret_cast<const u32x4 *>(rec + kv8_value_byte(4 * g + odd, 64 * i + 4 * (Sums<HD>::half(i) ? n & 7 : n), HD));
     };
     int page = __builtin_amdgcn_readlane(pages, 0);
     load_k(page);
@@ -457,8 +470,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
             };
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
+                if (Sums<HD>::half(i))
+#pragma unroll
+                    for (int odd = 0; odd < 2; ++odd) vc[i][odd] >>= 2 * (n & 8);
                 values(i, std::integral_constant<int, 0>());
-                values(i, std::integral_constant<int, 2>());
+                if (!Sums<HD>::half(i)) values(i, std::integral_constant<int, 2>());
             }
             load_v(next);
         } else {
@@ -485,8 +501,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int d = 64 * i + 16 * g + 4 * r;
-                if (d < HD) *reinterpret_cast<f32x4 *>(&s_o[wave][n][d]) = f32x4{t[k].o[i][0][r], t[k].o[i][1][r], t[k].o[i][2][r], t[k].o[i][3][r]};
+                float *dst = &s_o[wave][n][Sums<HD>::dim_of(i, g, r)];
+                if (Sums<HD>::half(i)) *reinterpret_cast<f32x2 *>(dst) = f32x2{t[k].o[i][0][r], t[k].o[i][1][r]};
+                else *reinterpret_cast<f32x4 *>(dst) = f32x4{t[k].o[i][0][r], t[k].o[i][1][r], t[k].o[i][2][r], t[k].o[i][3][r]};
             }
         __syncthreads();
         for (int e = threadIdx.x; e < kTile * (HD / 4); e += 64 * kWaves) {
