@@ -16,6 +16,7 @@
 // position of less weight than that adds nothing.  (Three bf16 parts, which lose nothing, took 3 products instead of 2.)
 // A block's own sum joins the output by one fma with the block's scale: a chain of blocks through the MFMA's C would be
 // cut off downwards each time.
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -165,9 +166,12 @@ struct Queries {
 };
 
 // One wave's running sums of a tile.
-// Probabilities are 2^(s - m + kUp), and m is left as it is until a score is kSlack above it: after the first few blocks
-// it rarely changes, where the exact maximum of one row in 16 changes in most of a prompt's blocks (47 instructions).
+// Probabilities are 2^(s + a) with a = kUp - m, and a is left as it is until a score would give more than 2^(kUp + kSlack):
+// after the first few blocks it rarely changes, where the exact maximum of one row in 16 changes in most of a prompt's blocks
+// (47 instructions).  From maxima of 2^20 on (kFar), kUp - m and the unrounded s would be off from each other by more than a
+// sixteenth, from 2^24 on by more than fp16 has room for: there s is rounded first and a is -m, so that s + a is exact.
 constexpr float kUp = 11.0f, kSlack = 4.0f;  // (2^15 at most, in fp16)
+constexpr float kFar = 1048576.0f;
 template <int HD>
 struct Sums {
     static constexpr int NT = (HD + 63) / 64;
@@ -175,7 +179,8 @@ struct Sums {
     // the last 32 are [i][j < 2][r], 64 i + 16 (g % 2) + 4 r + 2 (g / 2) + j, from 64 i + 4 (n % 8) + 2 (n / 8) + j: half the
     // products (as 64 dims, 32 of them zeros, 1000 rows of 28 heads behind 500 positions took 55 us, so 44.5).
     f32x4 o[NT][4];
-    float m, l;
+    float a, l;  // (a: FLT_MAX without a score, whose sum with -inf is -inf)
+    bool far;    // uniform: a maximum has been kFar or beyond
     static constexpr bool half(int i) { return 64 * (i + 1) > HD; }
     static constexpr int js(int i) { return half(i) ? 2 : 4; }
     static __device__ __forceinline__ int dim_of(int i, int g, int r) {
@@ -193,15 +198,18 @@ struct Sums {
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m = -INFINITY;
+        a = FLT_MAX;
         l = 0.0f;
+        far = false;
     }
-    // the maximum becomes the tile's where one is kSlack above it; mx: of this lane's scores.  Returns what is added to
-    // the scores.
-    __device__ __forceinline__ float raise(float mx) {
-        if (__any(mx > m + kSlack)) {  // uniform
-            mx = fmaxf(m, groups_max(mx));
-            const float al = m == -INFINITY ? 0.0f : exp2_fast(m - mx);
+    // a for scores s f, of which mx is this lane's largest; far ones are rounded (and f is 1 then)
+    template <int U>
+    __device__ __forceinline__ void raise(float mx, f32x4 (&s)[U], float &f) {
+        if (__any(mx + a > kUp + kSlack) || far) {  // uniform
+            const float top = groups_max(mx);
+            far |= __any(fabsf(top) >= kFar && top != -INFINITY);
+            const float to = fminf(a, top == -INFINITY ? FLT_MAX : fabsf(top) >= kFar ? -top : kUp - top);
+            const float al = exp2_fast(to - a);
             l *= al;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
@@ -209,9 +217,15 @@ struct Sums {
                 for (int j = 0; j < js(i); ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[i][j][r] *= al;
-            m = mx;
+            a = to;
+            if (far) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[u][r] *= f;
+                f = 1.0f;
+            }
         }
-        return m == -INFINITY ? 0.0f : kUp - m;
     }
     // a block's sums S (positions block * 32 + 16 u + 4 g + r) to probabilities, as operands
     __device__ __forceinline__ void weigh(f32x4 (&s)[2], float f, bool edge, int block, int g, int seen, u32x4 &hi, u32x4 &lo) {
@@ -234,12 +248,12 @@ struct Sums {
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][r]);
             mx *= f;  // (f > 0, 0 with sums of 0, or NaN)
         }
-        const float add = raise(mx);
+        raise(mx, s, f);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[u][r] = exp2_fast(fmaf(s[u][r], f, add));
+                s[u][r] = exp2_fast(fmaf(s[u][r], f, a));
             }
         split2(s[0], s[1], hi, lo);
         // the sum of the operands that the values meet, by products with ones (8 additions took as long as 5 MFMAs)
@@ -269,20 +283,19 @@ struct Sums {
             for (int e = 0; e < 8; ++e)
                 acc[e % 4] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e / 4][e % 4], f16_at(q.hi[i], e) + f16_at(q.lo[i], e), acc[e % 4], 0, 0, 0);
         }
-        f32x4 s;
-        float mx = -INFINITY;
+        f32x4 s[1];
+        float mx = -INFINITY, f = 1.0f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float v = ((acc[0][r] + acc[1][r]) + (acc[2][r] + acc[3][r])) * q.inv;
-            s[r] = base + 4 * g + r > q.seen ? -INFINITY : v;
-            mx = fmaxf(mx, s[r]);
+            s[0][r] = base + 4 * g + r > q.seen ? -INFINITY : v;
+            mx = fmaxf(mx, s[0][r]);
         }
-        const float add = raise(mx);
+        raise(mx, s, f);
+        f32x4 p;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            s[r] = exp2_fast(s[r] + add);
-        }
-        l += groups_sum((s[0] + s[1]) + (s[2] + s[3]));
+        for (int r = 0; r < 4; ++r) p[r] = exp2_fast(s[0][r] + a);
+        l += groups_sum((p[0] + p[1]) + (p[2] + p[3]));
         bool odd = false;  // a value that is not finite
         f32x4 v[4][NT];    // dims value_dim .. of position 4g + r
 #pragma unroll
@@ -299,8 +312,8 @@ struct Sums {
         }
         if (base + 15 > first && __any(odd)) {  // uniform: 0 times that value, for a row that does not see it, would be NaN
             for (int e = 0; e < 16 && base + e < len; ++e) {
-                float p = e % 4 == 0 ? s[0] : e % 4 == 1 ? s[1] : e % 4 == 2 ? s[2] : s[3];
-                p = __shfl(p, 16 * (e / 4) + n, 64);
+                float pe = e % 4 == 0 ? p[0] : e % 4 == 1 ? p[1] : e % 4 == 2 ? p[2] : p[3];
+                pe = __shfl(pe, 16 * (e / 4) + n, 64);
                 if (base + e <= q.seen) {
                     const float *vrow = vr + static_cast<size_t>((base + e) % kKv8Recent) * HD;
 #pragma unroll
@@ -309,7 +322,7 @@ struct Sums {
                         for (int r = 0; r < 4; ++r) {
                             const f32x4 y = dims_at(i, vrow + dim_of(i, g, r));
 #pragma unroll
-                            for (int j = 0; j < js(i); ++j) o[i][j][r] = fmaf(p, y[j], o[i][j][r]);
+                            for (int j = 0; j < js(i); ++j) o[i][j][r] = fmaf(pe, y[j], o[i][j][r]);
                         }
                 }
             }
@@ -320,7 +333,7 @@ struct Sums {
                 for (int j = 0; j < js(i); ++j) {
                     f32x4 x = zero;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i][j], s[r], x, 0, 0, 0);
+                    for (int r = 0; r < 4; ++r) x = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i][j], p[r], x, 0, 0, 0);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[i][j][r] += x[r];
                 }
@@ -494,7 +507,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
         const int pk = p0 + k * kTile;
         if (k > 0) __syncthreads();  // (the tile before is read)
         if (g == 0) {
-            s_m[wave][n] = t[k].m;
+            s_m[wave][n] = -t[k].a;
             s_l[wave][n] = t[k].l;
         }
 #pragma unroll
@@ -517,8 +530,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, c
 #pragma unroll
             for (int i = 0; i < kWaves; ++i) {
                 const float mi = s_m[i][row], li = s_l[i][row];
-                if (mi == -INFINITY && li == 0.0f) continue;                    // no position of this row
-                const float f = mi == -INFINITY ? 1.0f : exp2_fast(mi - mx);  // (-inf: then li is NaN)
+                const float f = exp2_fast(mi - mx);  // (no position of this row: -FLT_MAX, and sums of 0)
                 const f32x4 o = *reinterpret_cast<const f32x4 *>(&s_o[i][row][d]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) num[r] = fmaf(o[r], f, num[r]);
@@ -593,8 +605,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_kernel(Kv8View c
     float den = 0.0f;
 #pragma unroll
     for (int k = 0; k < kSlots; ++k) {
-        // no position of this row: nothing; a maximum of -inf otherwise: li is NaN
-        const float f = mi[k] == -INFINITY ? (li[k] == 0.0f ? 0.0f : 1.0f) : exp2_fast(mi[k] - mx);
+        const float f = exp2_fast(mi[k] - mx);
         s_f[wave][lane + 64 * k] = f;
         den = fmaf(li[k], f, den);
     }
@@ -673,7 +684,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_kv8_join_rows_kernel(Kv8V
     if (used <= 1) return;  // written already
     const float mi = lane < used ? ml.x : -INFINITY, li = lane < used ? ml.y : 0.0f;
     const float mx = wave_max_dpp(mi);
-    const float f = mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : exp2_fast(mi - mx);
+    const float f = exp2_fast(mi - mx);
     const float den = wave_sum(li * f);
     f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
