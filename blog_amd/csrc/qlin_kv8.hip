@@ -82,11 +82,11 @@ __device__ __forceinline__ double weight_of(uint2 w, int e, int type, int one_pl
     return one_plus ? static_cast<double>(v) + 1.0 : static_cast<double>(v);
 }
 
-// One head's norm (w NULL: none) and turn by the table's row of pos, in place; every lane of the group calls it,
-// those past the head's end (live false) with zeros.
+// One head's norm (w NULL: none) and turn by the table's row of pos (clamped to 0 .. cap - 1), in place; every lane of the
+// group calls it, those past the head's end (live false) with zeros.
 template <int T>
 __device__ __forceinline__ void norm_and_turn(f32x4v &va, f32x4v &vb, const Runs &r, bool live, int hd, const uint16_t *w,
-                                              const qlin_qk_rope &how, int pos) {
+                                              const qlin_qk_rope &how, int pos, int cap) {
     double a[4], b[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -100,10 +100,10 @@ __device__ __forceinline__ void norm_and_turn(f32x4v &va, f32x4v &vb, const Runs
         wa = weights_at(w, r.a);
         wb = weights_at(w, r.b);
     }
-    const int half = how.rotary_dim / 2;
+    const int half = how.rotary_dim / 2, at = min(max(pos, 0), cap - 1);
     f32x4v c0, s0;  // halves: the pairs' cosines and sines; neighbours: (cos, cos, sin, sin) of run a's and b's pairs
     if (r.turned) {
-        const float *row = how.table + static_cast<size_t>(min(max(pos, 0), how.table_len - 1)) * how.rotary_dim;
+        const float *row = how.table + static_cast<size_t>(min(at, how.table_len - 1)) * how.rotary_dim;
         if (how.pairing == 0) {
             c0 = ld4(row + r.a);
             s0 = ld4(row + half + r.a);
@@ -126,6 +126,7 @@ __device__ __forceinline__ void norm_and_turn(f32x4v &va, f32x4v &vb, const Runs
         }
     }
     if (r.turned) {
+        if (at >= how.table_len) c0 = f32x4v{NAN, NAN, NAN, NAN};  // (another position's angles would go unseen)
         if (how.pairing == 0) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kernel(qlin_qk_rope 
     f32x4v x = a, y = b;
     Runs rr = r;
     rr.turned = rr.turned && live && (is_q || is_k);
-    norm_and_turn<T>(x, y, rr, live, hd, is_q ? how.q_norm : how.k_norm, how, pos);
+    norm_and_turn<T>(x, y, rr, live, hd, is_q ? how.q_norm : how.k_norm, how, pos, max_seq);
     if (live) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // (by value: a choice between vectors goes through memory)
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
         f32x4v a = live ? ld4(src + r.a) : kZero4, b = live ? ld4(src + r.b) : kZero4;
         Runs rr = r;
         rr.turned = rr.turned && live;
-        norm_and_turn<T>(a, b, rr, live, HD, how.q_norm, how, w.start + row);
+        norm_and_turn<T>(a, b, rr, live, HD, how.q_norm, how, w.start + row, cap);
         if (live) {
             float *dst = q_out + (static_cast<size_t>(line) * n_heads + head) * HD;
             st4(dst + r.a, a);
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
             f32x4v a = ka[p], bb = kb[p];
             Runs rr = r;
             rr.turned = rr.turned && fresh;
-            norm_and_turn<T>(a, bb, rr, fresh, HD, how.k_norm, how, pos);
+            norm_and_turn<T>(a, bb, rr, fresh, HD, how.k_norm, how, pos, cap);
             if (fresh) {
                 ka[p] = a;
                 kb[p] = bb;

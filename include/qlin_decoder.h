@@ -69,7 +69,9 @@ extern "C" {
  *           and then sines: pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with pairing 1, become
  *           (a cos_i - b sin_i, b cos_i + a sin_i); the rest stays.  rotary_dim 0: no rotation (table unused).
  * Both are computed in 64 bits and rounded once.  The table (qlin_launch_rope_table, or a caller's own with
- * other frequencies) keeps far positions' angles exact, which powf and cosf of one f32 product do not.
+ * other frequencies) keeps far positions' angles exact, which powf and cosf of one f32 product do not.  Heads at a
+ * position of the cache that the table does not have become NaN where they are turned (a position outside the cache is
+ * taken as the nearest one in it).
  *
  * qlin_kv8_cache is one layer's cache of n_seqs sequences, up to blocks_per_seq blocks of QLIN_KV8_BLOCK
  * positions each (its capacity):
@@ -124,7 +126,7 @@ typedef struct qlin_qk_rope {
     float eps;
     int one_plus;
     const float *table;              /* [table_len, rotary_dim] */
-    int table_len;                   /* >= the cache's capacity */
+    int table_len;                   /* positions 0 .. table_len - 1 */
     int rotary_dim;                  /* a multiple of 8, <= head_dim */
     int pairing;                     /* 0: (i, i + rotary_dim / 2), 1: (2i, 2i + 1) */
 } qlin_qk_rope;
