@@ -132,8 +132,8 @@ class Qwen2Decoder:
             qlin.set_stream(torch.cuda.current_stream())
             self.rotation = torch.empty(max_seq, cfg.head_dim, dtype=f32, device=dev)
             qlin.rope_table(self.rotation, cfg.theta)
-            self.how = [qlin.QkRope(W.get("q_norm"), W.get("k_norm"), 0, cfg.eps, 0, self.rotation, cfg.head_dim)
-                        for W in weights["layers"]]
+            norms = [(W["q_norm"], W["k_norm"]) if cfg.qk_norm else (None, None) for W in weights["layers"]]
+            self.how = [qlin.QkRope(q, k, 0, cfg.eps, 0, self.rotation, cfg.head_dim) for q, k in norms]
         if cfg.kv8:
             self.kv8 = [qlin.Kv8Cache.empty(torch, 1, cfg.kv_heads, cfg.head_dim, max_seq) for _ in range(cfg.layers)]
             need = max(qlin.attend_kv8_workspace_bytes(1, rows, cfg.n_heads, cfg.kv_heads, cfg.head_dim,
