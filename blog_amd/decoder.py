@@ -125,12 +125,14 @@ class Qwen2Decoder:
         self.prompt_ids = torch.zeros(P, dtype=i32, device=dev)
         self.token = torch.zeros(1, dtype=i32, device=dev)      # the next step's input token
         self.pos = torch.zeros(1, dtype=i32, device=dev)        # the next step's position
+        self.at = torch.zeros(1, dtype=i32, device=dev)         # where a step is taken: past the last position, there
         self.zero = torch.zeros(1, dtype=i32, device=dev)
         self.L = qlin.lib()
         self.controls, self.captured = None, []
         if cfg.qk_norm or cfg.kv8:
             qlin.set_stream(torch.cuda.current_stream())
-            self.rotation = torch.empty(max_seq, cfg.head_dim, dtype=f32, device=dev)
+            rows = -(-max_seq // qlin.KV8_BLOCK) * qlin.KV8_BLOCK if cfg.kv8 else max_seq  # (the cache's whole blocks)
+            self.rotation = torch.empty(rows, cfg.head_dim, dtype=f32, device=dev)
             qlin.rope_table(self.rotation, cfg.theta)
             norms = [(W["q_norm"], W["k_norm"]) if cfg.qk_norm else (None, None) for W in weights["layers"]]
             self.how = [qlin.QkRope(q, k, 0, cfg.eps, 0, self.rotation, cfg.head_dim) for q, k in norms]
@@ -278,10 +280,13 @@ class Qwen2Decoder:
         qlin.set_stream(self.torch.cuda.current_stream())
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.token), t(self.h),
                                                                  t(self.w["table"]), self.rb_h, c.hidden, 1))
-        self._layers(1, t(self.pos))
+        if c.kv8 or self.controls is not None:
+            # past the last position that one is taken again, as the f32 caches' launches do by themselves
+            self.torch.clamp(self.pos, max=self.max_seq - 1, out=self.at)
+        self._layers(1, t(self.at if c.kv8 else self.pos))
         if self.controls is not None:
-            # the step's token is history for its pick (past the last position the row there is taken, as in the caches)
-            self.history[0].scatter_(0, self.pos.long().clamp_(max=self.max_seq - 1), self.token)
+            # the step's token is history for its pick
+            self.history[0].scatter_(0, self.at.long(), self.token)
             self.torch.add(self.pos, 1, out=self.history_len)
         self._head(0)
         self.pos.add_(1)

@@ -31,3 +31,61 @@ def test_head_norms_are_the_configurations():
     for kv8 in (False, True):
         with pytest.raises(KeyError):
             Qwen2Decoder(torch, _config(qk_norm=True, kv8=kv8), without, max_seq=64, max_prompt=32)
+
+
+@pytest.mark.parametrize("qk_norm,kv8", [(True, True), (False, True), (True, False)])
+@pytest.mark.parametrize("max_seq", [100, 96, 33])
+def test_steps_across_the_last_position(qk_norm, kv8, max_seq):
+    """Past the last position a step takes it again, with the token's key and value in place of the former ones, in either
+    cache, also where max_seq is not a whole number of the 8-bit cache's blocks; captured and replayed alike."""
+    torch = _env()
+    from gpu_util import banner, host
+    from blog_amd import qlin
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    from test_decoder_kv8 import Twin, _close
+    cfg = _config(qk_norm=qk_norm, kv8=kv8)
+    w = make_weights(torch, cfg, seed=7)
+    prompt = _prompt(torch, cfg, max_seq - 4 if max_seq < 64 else 64)
+    eager, dec = (Qwen2Decoder(torch, cfg, w, max_seq=max_seq, max_prompt=64) for _ in range(2))
+    twin = Twin(cfg, w, max_seq)
+    n = max_seq + 40 - len(prompt)
+    banner(f"across the last position, max_seq={max_seq} qk_norm={qk_norm} kv8={kv8}")
+    tokens = _prompt(torch, cfg, n, seed=2)  # (given: picks of their own soon repeat one token there)
+    eager.prefill(prompt)
+    ref, ids, at = [], host(prompt), 0
+    for i in range(n):
+        got, want = host(eager.logits), twin.run(ids, at)
+        assert _close(got, want), (i, np.linalg.norm(got - want) / np.linalg.norm(want))
+        ref.append(eager.logits.clone())
+        ids, at = host(tokens[i:i + 1]), min(len(prompt) + i, max_seq - 1)
+        for k, v in twin.exact:  # (the position that is taken again)
+            del k[at:], v[at:]
+        eager.token.copy_(tokens[i:i + 1])
+        eager.step()
+    dec.prefill(prompt)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dec.step()
+    qlin.set_stream(torch.cuda.current_stream())
+    for i in range(1, n):
+        dec.token.copy_(tokens[i - 1:i])
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dec.logits, ref[i]), i
+    assert int(dec.pos.item()) == len(prompt) + n - 1
+
+
+def test_history_past_the_last_position():
+    """The last row of the history is taken again too."""
+    torch = _env()
+    from gpu_util import banner, host
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    cfg = _config(qk_norm=True, kv8=True)
+    dec = Qwen2Decoder(torch, cfg, make_weights(torch, cfg, seed=8), max_seq=40, max_prompt=32)
+    dec.set_controls(presence=1.0, frequency=0.3)
+    prompt = _prompt(torch, cfg, 30)
+    banner("history past the last position")
+    tokens = dec.generate(prompt, 20)
+    seen = host(prompt).tolist() + tokens[:-1]
+    assert host(dec.history)[0].tolist() == seen[:39] + seen[-1:]
