@@ -159,18 +159,20 @@ class QlinError(RuntimeError):
 
 
 _lib = None
+_F32 = _I32 = None  # torch's types
 
 
 def lib() -> C.CDLL:
     """Loads the HIP library; raises if it has not been built (no fallback path exists)."""
-    global _lib
+    global _lib, _F32, _I32
     if _lib is None:
         # torch ships its own HIP runtime (torch/lib/libamdhip64.so, soname libamdhip64.so.7).  Loaded
         # first, it satisfies this library's libamdhip64.so.7 dependency, so the process has one HIP
         # runtime; loaded after, it would bring a second one next to /opt/rocm's, and device memory of
         # one is unusable from the other.
         try:
-            import torch  # noqa: F401
+            import torch
+            _F32, _I32 = torch.float32, torch.int32
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -387,6 +389,10 @@ def attend_kv8(cache, q, attn, rows, n_heads, start_pos, n_rows, softmax_scale, 
         0 if workspace is None else workspace.numel()))
 
 
+def _wrong(name, t, dtype, rows):
+    return ValueError(f"{name}: {tuple(t.shape)} of {t.dtype}, not {rows} contiguous values of {dtype}")
+
+
 # struct qlin_logits_controls, packed (filling a ctypes structure takes 0.4 us longer)
 _LOGITS_CONTROLS = struct.Struct("@8PNii")
 assert _LOGITS_CONTROLS.size == C.sizeof(LogitsControlsArgs)
@@ -400,29 +406,78 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
                     presence=None, bias_ids=None, bias_values=None, mask=None, picks=None, scratch=None):
     """Penalties, biases and a mask on logits [rows, >= vocab] into out (which may be logits), and the greedy picks.
     history [rows, max_history], bias_ids / bias_values [rows, max_bias] and mask [rows, words] (32 tokens a word) are
-    2-D and contiguous; scratch: a uint8 tensor of logits_controls_scratch_bytes(...), needed with picks."""
+    2-D and contiguous, with at least `rows` rows; history_lens, repetition, frequency, presence and picks hold a value for
+    each row.  Token ids, lengths, picks and the mask are int32, the rest float32.  scratch: a uint8 tensor of
+    logits_controls_scratch_bytes(...), needed with picks."""
+    library = _lib or lib()
+    f32, i32 = _F32, _I32
     # (strides and sizes as whole tuples: stride(0) or size(1) take 0.15 us longer each)
-    row, one = logits.stride()
-    out_row, out_one = out.stride()
-    if not one == out_one == 1 and vocab > 1:
-        raise ValueError("a row of logits is contiguous")
-    words = max_history = max_bias = 0
+    n, width = logits.shape
+    out_n, out_width = out.shape
+    row, out_row = width, out_width
+    if not (logits.is_contiguous() and out.is_contiguous()):
+        row, one = logits.stride()
+        out_row, out_one = out.stride()
+        if not one == out_one == 1 and vocab > 1:
+            raise ValueError("a row of logits is contiguous")
+    if n < rows or width < vocab or out_n < rows or out_width < vocab or logits.dtype is not f32 or out.dtype is not f32:
+        raise ValueError(f"{tuple(logits.shape)} logits of {logits.dtype} into {tuple(out.shape)} of {out.dtype}: "
+                         f"float32 [>= {rows}, >= {vocab}] both")
+    words = max_history = max_bias = p_mask = p_history = p_ids = p_values = 0
     if mask is not None:
-        words = mask.shape[1]
-        if not mask.is_contiguous():
-            raise ValueError("the mask is not contiguous")
+        n, words = mask.shape
+        if n < rows or mask.dtype is not i32 or not mask.is_contiguous():
+            raise ValueError(f"the mask: {tuple(mask.shape)} of {mask.dtype}, not contiguous int32 [{rows}, words]")
+        p_mask = mask.data_ptr()
     if history is not None:
-        max_history = history.shape[1]
-        if not history.is_contiguous():
-            raise ValueError("the history is not contiguous")
+        n, max_history = history.shape
+        if n < rows or history.dtype is not i32 or not history.is_contiguous():
+            raise ValueError(f"the history: {tuple(history.shape)} of {history.dtype}, not contiguous int32 [{rows}, tokens]")
+        p_history = history.data_ptr()
     if bias_ids is not None:
-        max_bias = bias_ids.shape[1]
-        if not bias_ids.is_contiguous() or bias_values is not None and (
-                not bias_values.is_contiguous() or bias_values.shape != bias_ids.shape):
-            raise ValueError("biases: tokens and values of one shape, contiguous")
-    a = _LOGITS_CONTROLS.pack(
-        _at(history) or 0, _at(history_lens) or 0, _at(repetition) or 0, _at(frequency) or 0, _at(presence) or 0,
-        _at(bias_ids) or 0, _at(bias_values) or 0, _at(mask) or 0, words, max_history, max_bias)
-    _done("qlin_launch_logits_controls", _lib_of().qlin_launch_logits_controls(
-        a, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, _at(picks), _at(scratch),
-        0 if scratch is None else scratch.numel()))
+        shape = bias_ids.shape
+        n, max_bias = shape
+        if n < rows or bias_ids.dtype is not i32 or not bias_ids.is_contiguous() or bias_values is not None and (
+                bias_values.dtype is not f32 or not bias_values.is_contiguous() or bias_values.shape != shape):
+            raise ValueError(f"biases: int32 tokens and float32 values of one shape [{rows}, entries], contiguous")
+        p_ids = bias_ids.data_ptr()
+        p_values = 0 if bias_values is None else bias_values.data_ptr()
+    # (what has a value for each row, written out: a function's call for each takes 0.3 us more.  An address stands for
+    # itself; a tensor without values has none)
+    p_lens = p_repetition = p_frequency = p_presence = p_picks = 0
+    if history_lens is not None:
+        if history_lens.__class__ is int:
+            p_lens = history_lens
+        elif history_lens.dtype is not i32 or not (p_lens := history_lens.data_ptr()) and rows or rows > 1 and (
+                history_lens.numel() < rows or not history_lens.is_contiguous()):
+            raise _wrong("history_lens", history_lens, i32, rows)
+    if repetition is not None:
+        if repetition.__class__ is int:
+            p_repetition = repetition
+        elif repetition.dtype is not f32 or not (p_repetition := repetition.data_ptr()) and rows or rows > 1 and (
+                repetition.numel() < rows or not repetition.is_contiguous()):
+            raise _wrong("repetition", repetition, f32, rows)
+    if frequency is not None:
+        if frequency.__class__ is int:
+            p_frequency = frequency
+        elif frequency.dtype is not f32 or not (p_frequency := frequency.data_ptr()) and rows or rows > 1 and (
+                frequency.numel() < rows or not frequency.is_contiguous()):
+            raise _wrong("frequency", frequency, f32, rows)
+    if presence is not None:
+        if presence.__class__ is int:
+            p_presence = presence
+        elif presence.dtype is not f32 or not (p_presence := presence.data_ptr()) and rows or rows > 1 and (
+                presence.numel() < rows or not presence.is_contiguous()):
+            raise _wrong("presence", presence, f32, rows)
+    if picks is not None:
+        if picks.__class__ is int:
+            p_picks = picks
+        elif picks.dtype is not i32 or not (p_picks := picks.data_ptr()) and rows or rows > 1 and (
+                picks.numel() < rows or not picks.is_contiguous()):
+            raise _wrong("picks", picks, i32, rows)
+    a = _LOGITS_CONTROLS.pack(p_history, p_lens, p_repetition, p_frequency, p_presence, p_ids, p_values, p_mask, words,
+                              max_history, max_bias)
+    rc = library.qlin_launch_logits_controls(a, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, p_picks,
+                                             *((None, 0) if scratch is None else (_at(scratch), scratch.numel())))
+    if rc != 0:
+        raise QlinError("qlin_launch_logits_controls", rc)
