@@ -317,13 +317,20 @@ class QkRope:
     def __init__(self, q_norm, k_norm, norm_type, eps, one_plus, table, rotary_dim, pairing=0):
         if table is not None and (table.element_size() != 4 or not table.is_contiguous() or table.shape[1] != rotary_dim):
             raise ValueError(f"a table {tuple(table.shape)} of {table.dtype} for rotary_dim {rotary_dim}: contiguous f32 rows of it")
+        self.norm_dims = 1 << 30  # of the shorter weights, as far as they are known
         for w in (q_norm, k_norm):
-            if hasattr(w, "data_ptr") and (w.element_size() != 2 or not w.is_contiguous()):
-                raise ValueError("norm weights are contiguous and of 16 bits")
+            if hasattr(w, "data_ptr"):
+                if w.element_size() != 2 or not w.is_contiguous():
+                    raise ValueError("norm weights are contiguous and of 16 bits")
+                self.norm_dims = min(self.norm_dims, w.numel())
         self.tensors = (q_norm, k_norm, table)
         self.args = QkRopeArgs(ptr(q_norm), ptr(k_norm), norm_type, eps, int(one_plus), ptr(table),
                                table.shape[0] if table is not None else 0, rotary_dim, pairing)
         self.address = C.addressof(self.args)
+
+
+def _short_norms(how, head_dim):
+    return ValueError(f"norm weights of {how.norm_dims} values for heads of {head_dim}")
 
 
 class Kv8Cache:
@@ -361,6 +368,8 @@ class Kv8Cache:
 
 def qk_norm_rope_store_kv(how, q, q_stride, k, k_stride, v, v_stride, q_out, kc, vc, rows, n_heads, kv_heads, head_dim,
                           max_seq, start_pos):
+    if how.norm_dims < head_dim:
+        raise _short_norms(how, head_dim)
     _done("qlin_launch_qk_norm_rope_store_kv", _lib_of().qlin_launch_qk_norm_rope_store_kv(
         how.address, _at(q), q_stride, _at(k), k_stride, _at(v), v_stride, _at(q_out), _at(kc), _at(vc), rows, n_heads,
         kv_heads, head_dim, max_seq, _at(start_pos)))
@@ -368,6 +377,8 @@ def qk_norm_rope_store_kv(how, q, q_stride, k, k_stride, v, v_stride, q_out, kc,
 
 def qk_norm_rope_store_kv8(how, cache, q, q_stride, k, k_stride, v, v_stride, q_out, rows, n_heads, start_pos,
                            n_rows=None):
+    if how.norm_dims < cache.head_dim:
+        raise _short_norms(how, cache.head_dim)
     _done("qlin_launch_qk_norm_rope_store_kv8", _lib_of().qlin_launch_qk_norm_rope_store_kv8(
         how.address, cache.address, _at(q), q_stride, _at(k), k_stride, _at(v), v_stride, _at(q_out), rows, n_heads,
         _at(start_pos), _at(n_rows)))
