@@ -289,10 +289,6 @@ def _at(t):
     return t if t is None or t.__class__ is int else t.data_ptr()
 
 
-def _lib_of():
-    return _lib or lib()
-
-
 def _done(name, rc):
     if rc != 0:
         raise QlinError(name, rc)
@@ -327,6 +323,15 @@ class QkRope:
         self.args = QkRopeArgs(ptr(q_norm), ptr(k_norm), norm_type, eps, int(one_plus), ptr(table),
                                table.shape[0] if table is not None else 0, rotary_dim, pairing)
         self.address = C.addressof(self.args)
+
+
+def _of_sequences(t, n, name):
+    """The address of positions or counts, int32, one for each of n sequences (or an address, or None, as it is)."""
+    if t is None or t.__class__ is int:
+        return t
+    if t.dtype is not _I32 or n > 1 and (t.numel() < n or not t.is_contiguous()) or not (at := t.data_ptr()) and n:
+        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype}, not {n} contiguous values of int32")
+    return at
 
 
 def _short_norms(how, head_dim):
@@ -370,23 +375,26 @@ def qk_norm_rope_store_kv(how, q, q_stride, k, k_stride, v, v_stride, q_out, kc,
                           max_seq, start_pos):
     if how.norm_dims < head_dim:
         raise _short_norms(how, head_dim)
-    _done("qlin_launch_qk_norm_rope_store_kv", _lib_of().qlin_launch_qk_norm_rope_store_kv(
+    library = _lib or lib()
+    _done("qlin_launch_qk_norm_rope_store_kv", library.qlin_launch_qk_norm_rope_store_kv(
         how.address, _at(q), q_stride, _at(k), k_stride, _at(v), v_stride, _at(q_out), _at(kc), _at(vc), rows, n_heads,
-        kv_heads, head_dim, max_seq, _at(start_pos)))
+        kv_heads, head_dim, max_seq, _of_sequences(start_pos, 1, "start_pos")))
 
 
 def qk_norm_rope_store_kv8(how, cache, q, q_stride, k, k_stride, v, v_stride, q_out, rows, n_heads, start_pos,
                            n_rows=None):
     if how.norm_dims < cache.head_dim:
         raise _short_norms(how, cache.head_dim)
-    _done("qlin_launch_qk_norm_rope_store_kv8", _lib_of().qlin_launch_qk_norm_rope_store_kv8(
+    library, n = _lib or lib(), cache.n_seqs
+    _done("qlin_launch_qk_norm_rope_store_kv8", library.qlin_launch_qk_norm_rope_store_kv8(
         how.address, cache.address, _at(q), q_stride, _at(k), k_stride, _at(v), v_stride, _at(q_out), rows, n_heads,
-        _at(start_pos), _at(n_rows)))
+        _of_sequences(start_pos, n, "start_pos"), _of_sequences(n_rows, n, "n_rows")))
 
 
 def kv8_read(cache, first, lens, count, k_out, v_out):
-    _done("qlin_launch_kv8_read", _lib_of().qlin_launch_kv8_read(cache.address, _at(first), _at(lens), count, _at(k_out),
-                                                                 _at(v_out)))
+    library, n = _lib or lib(), cache.n_seqs
+    _done("qlin_launch_kv8_read", library.qlin_launch_kv8_read(
+        cache.address, _of_sequences(first, n, "first"), _of_sequences(lens, n, "lens"), count, _at(k_out), _at(v_out)))
 
 
 def attend_kv8_workspace_bytes(n_seqs, rows, n_heads, kv_heads, head_dim, blocks_per_seq):
@@ -395,9 +403,10 @@ def attend_kv8_workspace_bytes(n_seqs, rows, n_heads, kv_heads, head_dim, blocks
 
 def attend_kv8(cache, q, attn, rows, n_heads, start_pos, n_rows, softmax_scale, workspace):
     """workspace: a uint8 tensor of at least attend_kv8_workspace_bytes(...) (None where that is 0)."""
-    _done("qlin_launch_attend_kv8", _lib_of().qlin_launch_attend_kv8(
-        cache.address, _at(q), _at(attn), rows, n_heads, _at(start_pos), _at(n_rows), softmax_scale, _at(workspace),
-        0 if workspace is None else workspace.numel()))
+    library, n = _lib or lib(), cache.n_seqs
+    _done("qlin_launch_attend_kv8", library.qlin_launch_attend_kv8(
+        cache.address, _at(q), _at(attn), rows, n_heads, _of_sequences(start_pos, n, "start_pos"),
+        _of_sequences(n_rows, n, "n_rows"), softmax_scale, _at(workspace), 0 if workspace is None else workspace.numel()))
 
 
 def _wrong(name, t, dtype, rows):
