@@ -48,12 +48,11 @@ __device__ __forceinline__ void split3(const f32x4 &a, const f32x4 &b, u32x4 &hi
     }
 }
 
-// max(|a|, |b|, c) in one instruction
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, |%1|, |%2|, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
+// No instructions in inline assembly in what follows: it stands next to MFMAs, and the compiler does not see what assembly
+// does to registers that an MFMA in flight still reads or writes.
+
+// max(|a|, |b|, c): one v_max3_f32
+__device__ __forceinline__ float max3_abs(float a, float b, float c) { return fmaxf(fmaxf(fabsf(a), fabsf(b)), c); }
 // whether values of largest magnitude am (NaNs aside, which the parts carry) go as f32
 __device__ __forceinline__ bool out_of_range(float am) { return !(am < 0x1p100f) || (am < 0x1p-100f && am > 0.0f); }
 
@@ -69,17 +68,16 @@ __device__ __forceinline__ u32x4 bf16_of_i8(uint32_t a, uint32_t b) {
     }
     return r;
 }
-// byte I of v as a float in one instruction (a compiler's choice is a shift, a mask and a conversion)
+// byte I of v as a float: one v_cvt_f32_ubyte, if v's known bits and the float's uses are hidden (else shifts, masks and
+// subtractions of integers come before the conversion)
 template <int I>
 __device__ __forceinline__ float f32_of_byte(uint32_t v) {
-    float f;
-    if constexpr (I == 0) asm("v_cvt_f32_ubyte0 %0, %1" : "=v"(f) : "v"(v));
-    else if constexpr (I == 1) asm("v_cvt_f32_ubyte1 %0, %1" : "=v"(f) : "v"(v));
-    else if constexpr (I == 2) asm("v_cvt_f32_ubyte2 %0, %1" : "=v"(f) : "v"(v));
-    else asm("v_cvt_f32_ubyte3 %0, %1" : "=v"(f) : "v"(v));
+    float f = static_cast<float>(v >> (8 * I) & 0xffu);
+    asm("" : "+v"(f));
     return f;
 }
 __device__ __forceinline__ u32x4 bf16_of_u8(uint32_t a, uint32_t b, float off) {
+    asm("" : "+v"(a), "+v"(b));
     return u32x4{bf16_tops(f32_of_byte<0>(a) - off, f32_of_byte<1>(a) - off),
                  bf16_tops(f32_of_byte<2>(a) - off, f32_of_byte<3>(a) - off),
                  bf16_tops(f32_of_byte<0>(b) - off, f32_of_byte<1>(b) - off),
