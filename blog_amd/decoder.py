@@ -129,6 +129,7 @@ class Qwen2Decoder:
         self.zero = torch.zeros(1, dtype=i32, device=dev)
         self.L = qlin.lib()
         self.controls, self.captured = None, []
+        self.stream, self.controlled_on = None, set()  # the calls' stream, and those whose picks read the controls
         if cfg.qk_norm or cfg.kv8:
             qlin.set_stream(torch.cuda.current_stream())
             rows = -(-max_seq // qlin.KV8_BLOCK) * qlin.KV8_BLOCK if cfg.kv8 else max_seq  # (the cache's whole blocks)
@@ -160,6 +161,12 @@ class Qwen2Decoder:
             self.controlled = torch.zeros(1, c.vocab, dtype=torch.float32, device="cuda")
             self.controls_scratch = torch.empty(max(16, qlin.logits_controls_scratch_bytes(1, c.vocab)), dtype=torch.uint8,
                                                 device="cuda")
+        if self.controls is not None:
+            # picks on other streams than the tensors' own may still have to read them
+            for t in self.controls.values():
+                for stream in self.controlled_on if t is not None else ():
+                    t.record_stream(stream)
+            self.controlled_on.clear()
         self.controls = dict(repetition=one(repetition), frequency=one(frequency), presence=one(presence), mask=mask)
         if bias:
             self.controls.update(
@@ -233,6 +240,8 @@ class Qwen2Decoder:
         if self.controls is not None:
             if self.torch.cuda.is_current_stream_capturing():
                 self.captured.append(self.controls)  # (the graph reads these tensors)
+            else:
+                self.controlled_on.add(self.stream)
             if self.fuse and hr % 16 == 0:
                 qlin.rms_norm_quant_gemv_multi(c.wtype, [self.w["table"]], self.rb_h, hr, self.w["final_norm"], 0, c.eps, 0,
                                                [self.logits], [c.vocab], c.hidden)
@@ -262,7 +271,8 @@ class Qwen2Decoder:
         c, t = self.cfg, c_ptr
         n = int(prompt.numel())
         assert 0 < n <= self.max_prompt and n <= self.max_seq
-        qlin.set_stream(self.torch.cuda.current_stream())
+        self.stream = self.torch.cuda.current_stream()
+        qlin.set_stream(self.stream)
         self.prompt_ids[:n].copy_(prompt)
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.prompt_ids), t(self.h),
                                                                  t(self.w["table"]), self.rb_h, c.hidden, n))
@@ -277,7 +287,8 @@ class Qwen2Decoder:
         """One decode token: the token id and position held on the device; leaves the logits, the next
         greedy token and pos + 1 (no host synchronisation, so a HIP graph can hold it)."""
         c, t = self.cfg, c_ptr
-        qlin.set_stream(self.torch.cuda.current_stream())
+        self.stream = self.torch.cuda.current_stream()
+        qlin.set_stream(self.stream)
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.token), t(self.h),
                                                                  t(self.w["table"]), self.rb_h, c.hidden, 1))
         if c.kv8 or self.controls is not None:

@@ -89,3 +89,37 @@ def test_history_past_the_last_position():
     tokens = dec.generate(prompt, 20)
     seen = host(prompt).tolist() + tokens[:-1]
     assert host(dec.history)[0].tolist() == seen[:39] + seen[-1:]
+
+
+def test_controls_that_are_replaced_while_a_step_waits():
+    """A step on another stream than the controls' own reads those it was launched with, also where they are replaced, and
+    their memory asked for again, before it runs."""
+    torch = _env()
+    from gpu_util import banner
+    from blog_amd import qlin
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    cfg = _config(qk_norm=True, kv8=True)
+    w = make_weights(torch, cfg, seed=8)
+    prompt = _prompt(torch, cfg, 20)
+    words = (cfg.vocab + 31) // 32
+    controls = lambda: dict(repetition=1.3, frequency=0.1, presence=0.5, bias={3: 2.0, 9: 1.0},
+                            mask=torch.full((1, words), 0x2AAAAAAA, dtype=torch.int32, device="cuda"))
+    banner("controls replaced while a step waits")
+    side = torch.cuda.Stream()
+    results = []
+    for replaced in (False, True):
+        dec = Qwen2Decoder(torch, cfg, w, max_seq=64, max_prompt=32)
+        dec.set_controls(**controls())
+        dec.prefill(prompt)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)  # (about 10 ms)
+            dec.step()
+        if replaced:
+            dec.set_controls(repetition=0.9)
+            filler = [torch.full((n,), 0x7F7F7F7F, dtype=torch.int32, device="cuda") for n in [1, 1, 1, 2, 2, words] * 8]
+        torch.cuda.synchronize()
+        results.append((dec.controlled.clone(), dec.token.clone()))
+        qlin.set_stream(torch.cuda.current_stream())
+    del filler
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
