@@ -145,7 +145,7 @@ class Qwen2Decoder:
 
     def set_controls(self, repetition=1.0, frequency=0.0, presence=0.0, bias=None, mask=None) -> None:
         """From the next pick on: penalties for the tokens of the prompt and those picked since (call it before the prefill;
-        tokens that came before the first call are not counted), a bias {token: value}, and a mask (int32 words, 32 tokens
+        tokens that came before the first call are not counted), a bias {token: value} of up to 4096 tokens, and a mask (int32 words, 32 tokens
         each, a bit set for a token that may follow; the tensor is read at every pick, so a grammar rewrites it between
         steps).  A graph keeps the controls that it was captured with."""
         torch, c = self.torch, self.cfg
@@ -154,6 +154,8 @@ class Qwen2Decoder:
         if mask is not None and (mask.dtype != torch.int32 or tuple(mask.shape) != (1, (c.vocab + 31) // 32)
                                  or not mask.is_contiguous() or mask.device != self.token.device):
             raise ValueError(f"mask: contiguous int32 [1, {(c.vocab + 31) // 32}] on the decoder's device")
+        if bias and len(bias) > qlin.MAX_BIAS:
+            raise ValueError(f"{len(bias)} biases: at most {qlin.MAX_BIAS}")
         one = lambda v: torch.full((1,), float(v), dtype=torch.float32, device="cuda")
         if self.controls is None:
             self.history = torch.full((1, self.max_seq), -1, dtype=torch.int32, device="cuda")

@@ -282,6 +282,7 @@ def dequantize(qtype, src, out, n, f16=True):
 # ---- head norms with the rotation, the 8-bit attention cache, controls on logits (qlin_decoder.h) ---
 
 KV8_BLOCK, KV8_RECENT = 32, 64
+MAX_BIAS = 4096  # biases of a row of logits
 
 
 # (call() looks at every argument twice: 2 to 4 us of a launch of 5)

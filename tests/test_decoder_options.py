@@ -123,3 +123,20 @@ def test_controls_that_are_replaced_while_a_step_waits():
         qlin.set_stream(torch.cuda.current_stream())
     del filler
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
+def test_more_biases_than_a_pick_takes():
+    """Refused by set_controls, which then leaves what was set as it was, and not by the step after it."""
+    torch = _env()
+    from gpu_util import banner
+    from blog_amd import qlin
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    cfg = _config(vocab=5000)
+    dec = Qwen2Decoder(torch, cfg, make_weights(torch, cfg, seed=8), max_seq=64, max_prompt=32)
+    dec.set_controls(repetition=1.3)
+    banner("as many biases as a pick takes")
+    with pytest.raises(ValueError):
+        dec.set_controls(bias={t: 1.0 for t in range(qlin.MAX_BIAS + 1)})
+    assert dec.controls["repetition"].item() == np.float32(1.3)
+    dec.set_controls(bias={t: -100.0 for t in range(qlin.MAX_BIAS)})
+    assert all(t >= qlin.MAX_BIAS for t in dec.generate(_prompt(torch, cfg, 5), 4))
