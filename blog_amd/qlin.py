@@ -498,7 +498,10 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
             raise _wrong("picks", picks, i32, rows)
     a = _LOGITS_CONTROLS.pack(p_history, p_lens, p_repetition, p_frequency, p_presence, p_ids, p_values, p_mask, words,
                               max_history, max_bias)
-    rc = library.qlin_launch_logits_controls(a, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, p_picks,
-                                             *((None, 0) if scratch is None else (_at(scratch), scratch.numel())))
+    p_scratch = scratch_bytes = 0
+    if scratch is not None:
+        p_scratch, scratch_bytes = scratch.data_ptr(), scratch.numel()
+    rc = library.qlin_launch_logits_controls(a, logits.data_ptr(), row, out.data_ptr(), out_row, rows, vocab, p_picks, p_scratch,
+                                             scratch_bytes)
     if rc != 0:
         raise QlinError("qlin_launch_logits_controls", rc)
