@@ -145,9 +145,10 @@ class Qwen2Decoder:
 
     def set_controls(self, repetition=1.0, frequency=0.0, presence=0.0, bias=None, mask=None) -> None:
         """From the next pick on: penalties for the tokens of the prompt and those picked since (call it before the prefill;
-        tokens that came before the first call are not counted), a bias {token: value} of up to 4096 tokens, and a mask (int32 words, 32 tokens
-        each, a bit set for a token that may follow; the tensor is read at every pick, so a grammar rewrites it between
-        steps).  A graph keeps the controls that it was captured with."""
+        tokens that came before the first call are not counted), a bias {token: value} of up to 4096 tokens, and a mask
+        (int32 words, 32 tokens each, a bit set for a token that may follow; the tensor is read at every pick, so a grammar
+        rewrites it between steps).  A graph keeps the controls that it was captured with; what one without controls picks is
+        not counted."""
         torch, c = self.torch, self.cfg
         if not repetition > 0:
             raise ValueError(f"repetition {repetition}: must be above 0")
@@ -280,6 +281,7 @@ class Qwen2Decoder:
                                                                  t(self.w["table"]), self.rb_h, c.hidden, n))
         self._layers(n, t(self.zero))
         if self.controls is not None:
+            self.history.fill_(-1)  # (steps of a graph without controls leave rows between: no tokens of another text)
             self.history[0, :n].copy_(prompt)
             self.history_len.fill_(n)
         self._head(n - 1)

@@ -140,3 +140,32 @@ def test_more_biases_than_a_pick_takes():
     assert dec.controls["repetition"].item() == np.float32(1.3)
     dec.set_controls(bias={t: -100.0 for t in range(qlin.MAX_BIAS)})
     assert all(t >= qlin.MAX_BIAS for t in dec.generate(_prompt(torch, cfg, 5), 4))
+
+
+def test_steps_without_controls_between():
+    """A step captured before there were controls does not count its token; no token of the text before is counted for it."""
+    torch = _env()
+    from gpu_util import banner, host
+    from blog_amd import qlin
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    cfg = _config(qk_norm=True, kv8=True)
+    dec = Qwen2Decoder(torch, cfg, make_weights(torch, cfg, seed=8), max_seq=64, max_prompt=32)
+    dec.prefill(_prompt(torch, cfg, 4))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dec.step()
+    qlin.set_stream(torch.cuda.current_stream())
+    banner("steps without controls between")
+    dec.set_controls(frequency=1.0)
+    dec.generate(_prompt(torch, cfg, 20, seed=3), 20)
+    prompt = _prompt(torch, cfg, 10, seed=4)
+    dec.prefill(prompt)
+    for _ in range(5):
+        g.replay()
+    token = dec.token.clone()
+    dec.step()
+    torch.cuda.synchronize()
+    assert host(dec.history)[0, :16].tolist() == host(prompt).tolist() + 5 * [-1] + host(token).tolist()
+    counts = np.bincount(np.append(host(prompt), host(token)), minlength=cfg.vocab).astype(np.float32)
+    assert np.array_equal(host(dec.controlled)[0], host(dec.logits) - counts)
