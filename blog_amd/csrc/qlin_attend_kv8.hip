@@ -345,13 +345,16 @@ struct Sums {
 // split's blocks in turn, each with sums of its own, which meet in LDS.  A wave knows the pages of its next 64 blocks,
 // requests a block's keys while it weighs the values of the one before, and turns codes into operands for its RT tiles
 // in registers: there is no barrier before the end.
-// Few rows (RT = 1): bound by the latency of a wave's few blocks, and by the codes' bytes.  Many (RT = 2): bound by the
-// VALU; of a tile's 32 x 16 scores, 8 a lane, each costs an fma, an exp, a sum and 2 instructions for its operands,
-// then 4 fmas for 64 of its values, and half of the codes' 128.  (A workgroup that turned a block's codes once, into
+// Few rows (RT = 1): bound by the latency of a wave's few blocks, and by the codes' bytes.  Many (RT = 2): bound by each
+// wave's chain of scores, maximum, exponentials, pairs and values, which its registers let only one other wave of the SIMD
+// hide: the vector unit issues in 2/3 of the busy cycles, the matrix unit works in 1/3 (2011 rows of 28 heads 68% and 31%,
+// 250 behind 6000 of 32 66% and 37%).  Of a tile's 32 x 16 scores, 8 a lane, each costs an fma, an exp, a sum and 2
+// instructions for its operands, then 4 fmas for 64 of its values, and half of the codes' 128.  (A workgroup that turned a block's codes once, into
 // LDS, for 64 rows took half of these, but one block after the other: the longest row's time, 86 us for 2011 rows of 28
 // heads, was all of it.  Codes turned once for all, by a launch before: 92 us, and 2.5 to 5 more for fewer rows.)
-// Heads of 128, 28 over 4: one row over 32002 positions 11.4 us, 2.9 TB/s; 24 rows over up to 8000 27.4, 4.1 TB/s; 2011
-// rows 87.5, 331 TFLOP/s (of one product each; two are made).  32 over 8: 250 rows behind 6000 64.7, 388 TFLOP/s.
+// Heads of 128, 28 over 4: one row over 32002 positions 11.2 us, 2.9 TB/s; 24 rows over up to 8000 27.0, 4.2 TB/s (the
+// shortest of 20 in a kernel trace); 2011 rows 85.8, 338 TFLOP/s (of one product each; two are made).  32 over 8: 250 rows
+// behind 6000 63.8, 394 TFLOP/s (in a run of passes; in the trace, with clocks and caches colder, 99.9 and 74.6).
 template <int HD, int RT, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_kv8_kernel(Kv8View c, const float *__restrict__ q,
                                                                     float *__restrict__ out, int rows, int n_heads,

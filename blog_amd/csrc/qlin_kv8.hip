@@ -28,7 +28,7 @@ __device__ __forceinline__ f32x4v ld4(const float *p) {
     return v;
 }
 // Streaming stores: what lies dirty in the L2s at the kernel's end is written back then (a 2011-row prompt's store and
-// read back 26.0 us, so 22.2; 1877 rows into the f32 cache 18.3 and 16.5).
+// read back 26.0 us, so 22.2; 1877 rows into the f32 cache 18.3 and 16.5, in graphs).
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ void st4(float *p, const f32x4v &v) { __builtin_nontemporal_store(v, reinterpret_cast<f32x4u *>(p)); }
 
@@ -157,7 +157,7 @@ constexpr int kThreads = 256;
 constexpr f32x4v kZero4 = {0.0f, 0.0f, 0.0f, 0.0f};
 
 // A group of lanes for each query, key and value head of each row.  Bound by bytes: 1877 rows of 28 + 4 + 4 heads of 128
-// 15.1 us, 4.6 TB/s; one row 2.4 us, the launch.
+// 14.1 to 15.8 us in a kernel trace, 4.4 to 5.0 TB/s; one row 2.6 us, the launch.
 template <int T>
 __global__ __launch_bounds__(kThreads) void norm_rope_store_kernel(qlin_qk_rope how, const float *q, size_t q_stride,
                                                                    const float *__restrict__ k, size_t k_stride,
@@ -226,7 +226,7 @@ __device__ __forceinline__ int code_of(float x, float scale) {
 // the ring, writes the new rows of the last two blocks there, and, if the block is complete, its codes (through LDS,
 // in the record's order) and scales.
 //
-// Bound by the queries' bytes (2011 rows of 28 + 4 + 4 heads of 128 15.0 us, 4.5 TB/s), for few rows by a block's chain: table
+// Bound by the queries' bytes (2011 rows of 28 + 4 + 4 heads of 128 14.3 us in a kernel trace, 4.7 TB/s), for few rows by a block's chain: table
 // row and norm, largest value, codes through LDS (24 sequences of one row 6.0 us).
 //
 // The first block's workgroup reads ring rows; the block two (or 2i) further that would overwrite them is its second
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kv8_kernel(qlin_qk_r
 }
 
 // A workgroup per (sequence, key head, 32 rows): a thread per 4 dims of a row.  Its rows lie in two blocks at most, whose
-// pages are requested first.  Bound by the chain page, code, store: 2011 rows of 4 heads of 128 5.3 us, 24 blocks 3.8.
+// pages are requested first.  Bound by the chain page, code, store: 2011 rows of 4 heads of 128 5.6 us, 24 blocks 3.9.
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(Kv8View c, int hd, const int *__restrict__ first,
                                                             const int *__restrict__ lens, int count, int parts,
                                                             float *__restrict__ k_out, float *__restrict__ v_out) {

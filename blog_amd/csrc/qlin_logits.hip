@@ -6,7 +6,8 @@
 // mask, and leaves its best (value, token) for a second small launch.  Biased tokens are few: a bit each in LDS takes
 // them out of the pass, and the thread that holds a token's first list entry computes that token alone, the sum of its
 // entries in list order.  Bound by bytes: each workgroup reads the history again (from L2).  48 rows of 151936 with
-// histories of 4000, biases and masks 16.9 us, 3.6 TB/s; one row 4.4; the second launch 2.1.
+// histories of 4000, biases and masks 16.2 to 20.5 us in a kernel trace, 2.9 to 3.7 TB/s; one row 4.5; the second launch
+// 1.9 to 4.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

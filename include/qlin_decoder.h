@@ -103,7 +103,7 @@ extern "C" {
  *                               64 bits; n_pos rows.
  *   qlin_launch_qk_norm_rope_store_kv   q_out = the queries, and keys and values into the f32 caches of
  *                               qlin_launch_rope_store_kv, whose counterpart with norms it is (one sequence, positions
- *                               clamped as there, so that it is followed by qlin_launch_attend).  head_dim and
+ *                               clamped as there, so that it is followed by qlin_launch_attend).  head_dim a
  *                               multiple of 8, <= 256.  q_out may be q (q_stride = n_heads * head_dim).
  *   qlin_launch_qk_norm_rope_store_kv8  the same into the 8-bit cache.
  *   qlin_launch_kv8_read        k_out, v_out [n_seqs, count, kv_heads, head_dim]: row r the values that position
@@ -112,8 +112,11 @@ extern "C" {
  *   qlin_launch_attend_kv8      attn[s, r, h] = sum_j p_j v_j, p = softmax_j(softmax_scale * q . k_j) over the positions
  *                               j <= the row's that the cache holds, which ends at start_pos_dev[s] + the sequence's rows
  *                               (their keys and values are stored first); heads and key heads as in qlin_launch_attend.
- *                               A row that sees no position gives 0.  f32 accuracy: products of q and p with the codes
- *                               are exact.  workspace: qlin_attend_kv8_workspace_bytes(...) bytes, 16-byte aligned, used
+ *                               A row that sees no position gives 0.  f32 accuracy: q softmax_scale log2(e) and p are
+ *                               rounded to pairs of fp16 values, 22 bits and a sign each (what is below 2^-39 of a row's
+ *                               largest q, or 2^-36 of its largest p, is lost), and their products with the codes are
+ *                               exact; scores may be as large as f32 holds.  A row whose q softmax_scale log2(e) is beyond
+ *                               f32 is NaN, and values are below 2^90 in magnitude.  workspace: qlin_attend_kv8_workspace_bytes(...) bytes, 16-byte aligned, used
  *                               by nothing else while the launches run (calls on one stream, or graphs that are not
  *                               replayed at the same time, may share it); its contents do not matter before or after.
  */
