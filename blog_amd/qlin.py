@@ -159,12 +159,12 @@ class QlinError(RuntimeError):
 
 
 _lib = None
-_F32 = _I32 = None  # torch's types
+_F32 = _I32 = _U32 = None  # torch's types
 
 
 def lib() -> C.CDLL:
     """Loads the HIP library; raises if it has not been built (no fallback path exists)."""
-    global _lib, _F32, _I32
+    global _lib, _F32, _I32, _U32
     if _lib is None:
         # torch ships its own HIP runtime (torch/lib/libamdhip64.so, soname libamdhip64.so.7).  Loaded
         # first, it satisfies this library's libamdhip64.so.7 dependency, so the process has one HIP
@@ -172,7 +172,7 @@ def lib() -> C.CDLL:
         # one is unusable from the other.
         try:
             import torch
-            _F32, _I32 = torch.float32, torch.int32
+            _F32, _I32, _U32 = torch.float32, torch.int32, torch.uint32
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -428,7 +428,7 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
     """Penalties, biases and a mask on logits [rows, >= vocab] into out (which may be logits), and the greedy picks.
     history [rows, max_history], bias_ids / bias_values [rows, max_bias] and mask [rows, words] (32 tokens a word) are
     2-D and contiguous, with at least `rows` rows; history_lens, repetition, frequency, presence and picks hold a value for
-    each row.  Token ids, lengths, picks and the mask are int32, the rest float32.  scratch: a uint8 tensor of
+    each row.  Token ids, lengths and picks are int32, the mask int32 or uint32, the rest float32.  scratch: a uint8 tensor of
     logits_controls_scratch_bytes(...), needed with picks."""
     library = _lib or lib()
     f32, i32 = _F32, _I32
@@ -447,8 +447,8 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
     words = max_history = max_bias = p_mask = p_history = p_ids = p_values = 0
     if mask is not None:
         n, words = mask.shape
-        if n < rows or mask.dtype is not i32 or not mask.is_contiguous():
-            raise ValueError(f"the mask: {tuple(mask.shape)} of {mask.dtype}, not contiguous int32 [{rows}, words]")
+        if n < rows or mask.dtype is not i32 and mask.dtype is not _U32 or not mask.is_contiguous():
+            raise ValueError(f"the mask: {tuple(mask.shape)} of {mask.dtype}, not contiguous int32 or uint32 [{rows}, words]")
         p_mask = mask.data_ptr()
     if history is not None:
         n, max_history = history.shape

@@ -86,3 +86,7 @@ def test_what_is_taken():
     qlin.logits_controls(**{**one, "logits": wide[:, 3:VOCAB + 3]}, rows=1, vocab=VOCAB, scratch=scratch)
     torch.cuda.synchronize()
     assert torch.equal(t["out"][1], out[1]) and int(t["picks"][1]) == int(picks[1])
+    t["out"].zero_()
+    qlin.logits_controls(**{**t, "mask": t["mask"].view(torch.uint32)}, rows=5, vocab=VOCAB, scratch=scratch)
+    torch.cuda.synchronize()
+    assert torch.equal(t["out"], out)
