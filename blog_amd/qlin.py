@@ -49,6 +49,17 @@ class LogitsControlsArgs(C.Structure):
                 ("max_bias", I)]
 
 
+class MoeRoutingArgs(C.Structure):
+    """struct qlin_moe_routing (include/qlin.h)."""
+    _fields_ = [("bias", P), ("sigmoid", I), ("n_groups", I), ("top_groups", I), ("group_pairs", I), ("renormalise", I),
+                ("scaling", F)]
+
+
+class LoraArgs(C.Structure):
+    """struct qlin_lora (include/qlin_decoder.h)."""
+    _fields_ = [("a", P), ("b", P), ("base", P), ("y", P), ("base_stride", SZ), ("y_stride", SZ), ("out_dim", I)]
+
+
 # name -> (restype, argtypes); every symbol of include/qlin.h
 SIGNATURES = {
     "qlin_status_string": (C.c_char_p, [I]),
@@ -82,6 +93,8 @@ SIGNATURES = {
     "qlin_launch_quant_swiglu_indexed": (I, [I, P, P, SZ, SZ, SZ, SZ, P, P, P, I, I, I]),
     "qlin_launch_quant_down_f32_indexed_accum_ordered": (I, [I, P, SZ, SZ, P, P, P, P, I, I, I]),
     "qlin_launch_moe_router_topk": (I, [P, P, P, I, I, I, F]),
+    "qlin_launch_moe_route": (I, [P, P, SZ, P, P, I, I, I]),
+    "qlin_launch_dequantize_q8_1": (I, [P, P, I, I, I]),
     "qlin_launch_dequantize_to_f16": (I, [I, P, P, I64]),
     "qlin_launch_dequantize_q4k_to_f16": (I, [P, P, I64]),
     "qlin_launch_dequantize_q80_to_f16": (I, [P, P, I64]),
@@ -116,6 +129,11 @@ SIGNATURES = {
     "qlin_launch_attend_kv8": (I, [P, P, P, I, I, P, P, F, P, SZ]),
     "qlin_logits_controls_scratch_bytes": (SZ, [I, I]),
     "qlin_launch_logits_controls": (I, [P, P, SZ, P, SZ, I, I, P, P, SZ]),
+    "qlin_launch_add_rms_norm": (I, [P, SZ, P, SZ, P, SZ, P, I, F, I, P, SZ, P, I, I, I, I]),
+    "qlin_lora_workspace_bytes": (SZ, [I, I, I, I, I]),
+    "qlin_launch_lora_add": (I, [P, I, I, I, I, I, P, P, P, SZ, P, I, P, SZ]),
+    "qlin_verify_drafts_workspace_bytes": (SZ, [I, I, I]),
+    "qlin_launch_verify_drafts": (I, [P, SZ, P, SZ, P, P, P, P, P, P, P, P, I, I, I, P, SZ]),
     "qlin_launch_quant_embedding": (I, [I, P, P, P, SZ, I, I]),
     "qlin_launch_mla_absorb_q_nope": (I, [I, P, P, SZ, P, I, I, I, I, I]),
     "qlin_launch_mla_absorb_q4_xsum_delta": (I, [P, P, SZ, P, I, I, I, I, I]),
@@ -159,12 +177,13 @@ class QlinError(RuntimeError):
 
 
 _lib = None
-_F32 = _I32 = _U32 = None  # torch's types
+_F32 = _I32 = _U32 = _U8 = None  # torch's types
+_LORA_TYPES = {}
 
 
 def lib() -> C.CDLL:
     """Loads the HIP library; raises if it has not been built (no fallback path exists)."""
-    global _lib, _F32, _I32, _U32
+    global _lib, _F32, _I32, _U32, _U8, _LORA_TYPES
     if _lib is None:
         # torch ships its own HIP runtime (torch/lib/libamdhip64.so, soname libamdhip64.so.7).  Loaded
         # first, it satisfies this library's libamdhip64.so.7 dependency, so the process has one HIP
@@ -172,7 +191,8 @@ def lib() -> C.CDLL:
         # one is unusable from the other.
         try:
             import torch
-            _F32, _I32, _U32 = torch.float32, torch.int32, torch.uint32
+            _F32, _I32, _U32, _U8 = torch.float32, torch.int32, torch.uint32, torch.uint8
+            _LORA_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -505,3 +525,190 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
                                              scratch_bytes)
     if rc != 0:
         raise QlinError("qlin_launch_logits_controls", rc)
+
+
+# ---- a server's step around the linears: norms with the residual's addition, adapters, routing, drafts -------
+#
+# These take tensors of one GPU (the current device's, whose stream set_stream was given) and refuse others, and types,
+# shapes and layouts that would be read as something else.
+
+def _rows_of(t, rows, width, name, device):
+    """The address and the row stride of t: f32 [>= rows, >= width] whose rows are contiguous."""
+    n, have = t.shape
+    row, one = t.stride()
+    if t.dtype is not _F32 or n < rows or have < width or one != 1 and width > 1 or t.get_device() != device:
+        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device}, not float32 [{rows}, {width}] with contiguous rows "
+                         f"on device {device}")
+    return t.data_ptr(), row if n > 1 else max(row, width)
+
+
+def _values_of(t, n, dtype, name, device):
+    """The address of at least n contiguous values of dtype (None: none)."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device}, not {n} contiguous values of {dtype} on device {device}")
+    return t.data_ptr()
+
+
+def _device_of(t, name):
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{name} is on {t.device}, not on a GPU")
+    return device
+
+
+def q8_1_bytes(in_dim, rows, mmq=False):
+    """Bytes of rows rows of in_dim values in Q8_1 blocks."""
+    return (in_dim + 127) // 128 * rows * 144 if mmq else rows * ((in_dim + 31) // 32) * 36
+
+
+def add_rms_norm(x, delta, sum, weight, norm_type, eps, one_plus, *, normed=None, q8_1=None, mmq=False, raw_sum=False):
+    """sum = x + delta, and its RMSNorm into normed [rows, hidden], into Q8_1 blocks (uint8), or both.  x, delta, sum and normed
+    are float32 [rows, hidden] with contiguous rows; delta and sum may be None, sum may be x or delta."""
+    library, device = _lib or lib(), _device_of(x, "x")
+    rows, hidden = x.shape
+    p_x, n_x = _rows_of(x, rows, hidden, "x", device)
+    p_delta, n_delta = (0, 0) if delta is None else _rows_of(delta, rows, hidden, "delta", device)
+    p_sum, n_sum = (0, 0) if sum is None else _rows_of(sum, rows, hidden, "sum", device)
+    p_normed, n_normed = (0, 0) if normed is None else _rows_of(normed, rows, hidden, "normed", device)
+    if weight.element_size() != 2 or weight.numel() < hidden or not weight.is_contiguous() or weight.get_device() != device:
+        raise ValueError(f"weight: {tuple(weight.shape)} of {weight.dtype} on {weight.device}, not {hidden} contiguous values of 16 bits")
+    p_q8 = _values_of(q8_1, q8_1_bytes(hidden, rows, mmq), _U8, "q8_1", device)
+    rc = library.qlin_launch_add_rms_norm(p_x, n_x, p_delta, n_delta, p_sum, n_sum, weight.data_ptr(), norm_type, eps, int(one_plus),
+                                          p_normed, n_normed, p_q8, int(mmq), int(raw_sum), rows, hidden)
+    if rc != 0:
+        raise QlinError("qlin_launch_add_rms_norm", rc)
+
+
+def dequantize_q8_1(x_q8_1, x, in_dim, m, mmq=False):
+    """The values that m rows of Q8_1 blocks (uint8) stand for, into x (float32, contiguous)."""
+    library, device = _lib or lib(), _device_of(x, "x")
+    rc = library.qlin_launch_dequantize_q8_1(_values_of(x_q8_1, q8_1_bytes(in_dim, m, mmq), _U8, "x_q8_1", device),
+                                             _values_of(x, in_dim * m, _F32, "x", device), in_dim, m, int(mmq))
+    if rc != 0:
+        raise QlinError("qlin_launch_dequantize_q8_1", rc)
+
+
+class Lora:
+    """Adapters of one projection in slots: a [n_adapters, max_rank, in_dim] and b [n_adapters, out_dim, max_rank], both
+    bfloat16, float16 or float32.  Holds on to the tensors."""
+
+    def __init__(self, a, b):
+        lib()
+        (n, rank, n_in), (n_b, out, rank_b) = a.shape, b.shape
+        if a.dtype is not b.dtype or a.dtype not in _LORA_TYPES or n_b != n or rank_b != rank or a.device != b.device:
+            raise ValueError(f"a {tuple(a.shape)} of {a.dtype} and b {tuple(b.shape)} of {b.dtype} are not one projection's adapters")
+        if not a.is_contiguous() or not b.is_contiguous():
+            raise ValueError("a and b are contiguous")
+        self.a, self.b, self.type = a, b, _LORA_TYPES[a.dtype]
+        self.n_adapters, self.max_rank, self.in_dim, self.out_dim = n, rank, n_in, out
+
+
+def lora_workspace_bytes(rows, n_mats, n_adapters, max_rank, in_dim):
+    return int(lib().qlin_lora_workspace_bytes(rows, n_mats, n_adapters, max_rank, in_dim))
+
+
+# struct qlin_lora, packed (filling ctypes structures takes several times as long)
+_LORA = struct.Struct("@4PNNi4x")
+assert _LORA.size == C.sizeof(LoraArgs)
+
+
+def lora_add(x, adapter_ids, mats, *, ranks=None, scales=None, workspace=None):
+    """mats: up to 4 (Lora, base, y) whose adapters read the same x: y = base + scale B (A x) of each row's adapter, y = base in
+    rows without one (id < 0, or no slot's).  x [rows, in_dim], base and y [rows, out_dim] are float32 with contiguous rows, y may
+    be base; adapter_ids [rows] and ranks [n_adapters] int32, scales [n_adapters] float32.  workspace: a uint8 tensor of
+    lora_workspace_bytes(...)."""
+    library, device = _lib or lib(), _device_of(x, "x")
+    if not 1 <= len(mats) <= 4:
+        raise ValueError(f"{len(mats)} projections: 1 to 4")
+    first, rows = mats[0][0], x.shape[0]
+    p_x, n_x = _rows_of(x, rows, first.in_dim, "x", device)
+    packed = b""
+    for w, base, y in mats:
+        if w.type != first.type or w.n_adapters != first.n_adapters or w.max_rank != first.max_rank or w.in_dim != first.in_dim:
+            raise ValueError("the projections' adapters have one type, number of slots, rank and input")
+        if w.a.get_device() != device:
+            raise ValueError(f"adapters on {w.a.device}, x on device {device}")
+        p_base, n_base = _rows_of(base, rows, w.out_dim, "base", device)
+        p_y, n_y = (p_base, n_base) if y is base else _rows_of(y, rows, w.out_dim, "y", device)
+        packed += _LORA.pack(w.a.data_ptr(), w.b.data_ptr(), p_base, p_y, n_base, n_y, w.out_dim)
+    p_ws = _values_of(workspace, 0, _U8, "workspace", device)
+    rc = library.qlin_launch_lora_add(packed, len(mats), first.type, first.n_adapters, first.max_rank, first.in_dim,
+                                      _values_of(ranks, first.n_adapters, _I32, "ranks", device),
+                                      _values_of(scales, first.n_adapters, _F32, "scales", device), p_x, n_x,
+                                      _values_of(adapter_ids, rows, _I32, "adapter_ids", device), rows, p_ws,
+                                      0 if workspace is None else workspace.numel())
+    if rc != 0:
+        raise QlinError("qlin_launch_lora_add", rc)
+
+
+class MoeRouting:
+    """How experts are chosen (struct qlin_moe_routing).  bias: float32 [n_experts] or None.  Holds on to the tensor."""
+
+    def __init__(self, *, sigmoid=False, bias=None, n_groups=1, top_groups=1, group_pairs=False, renormalise=False, scaling=1.0):
+        lib()
+        if bias is not None and (bias.dtype is not _F32 or not bias.is_contiguous()):
+            raise ValueError(f"a bias of {bias.dtype}: contiguous float32")
+        self.bias = bias
+        self.args = MoeRoutingArgs(ptr(bias), int(sigmoid), n_groups, top_groups, int(group_pairs), int(renormalise), scaling)
+        self.address = C.addressof(self.args)
+
+
+def moe_route(how, logits, ids, weights):
+    """The k experts of each token and their weights: logits float32 [tokens, n_experts] with contiguous rows into ids int32 and
+    weights float32, both [tokens, k] and contiguous."""
+    library, device = _lib or lib(), _device_of(logits, "logits")
+    tokens, n_experts = logits.shape
+    p_logits, stride = _rows_of(logits, tokens, n_experts, "logits", device)
+    k = ids.shape[1]
+    if how.bias is not None and (how.bias.numel() < n_experts or how.bias.get_device() != device):
+        raise ValueError(f"a bias of {how.bias.numel()} values on {how.bias.device} for {n_experts} experts on device {device}")
+    if ids.shape[0] < tokens or tuple(weights.shape) != tuple(ids.shape):
+        raise ValueError(f"ids {tuple(ids.shape)} and weights {tuple(weights.shape)} for {tokens} tokens")
+    rc = library.qlin_launch_moe_route(how.address, p_logits, stride, _values_of(ids, 0, _I32, "ids", device),
+                                       _values_of(weights, 0, _F32, "weights", device), tokens, n_experts, k)
+    if rc != 0:
+        raise QlinError("qlin_launch_moe_route", rc)
+
+
+def verify_drafts_workspace_bytes(n_seqs, max_drafts, vocab):
+    return int(lib().qlin_verify_drafts_workspace_bytes(n_seqs, max_drafts, vocab))
+
+
+def _logits_of(t, n, rows, name, device):
+    """The address, the row stride and the vocabulary of [n, rows, vocab] logits that lie row after row."""
+    a, b, vocab = t.shape
+    seq, row, one = t.stride()
+    if t.dtype is not _F32 or a != n or b != rows or t.get_device() != device or one != 1 and vocab > 1 or a > 1 and b > 0 and seq != b * row:
+        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype}, strides {t.stride()}, on {t.device}, not float32 [{n}, {rows}, vocab] "
+                         f"row after row on device {device}")
+    return t.data_ptr(), row if b > 1 else seq if a > 1 else max(row, vocab), vocab
+
+
+def verify_drafts(target, drafts, uniform, tokens, accepted, *, draft_logits=None, n_drafts=None, temperature=None, logprobs=None,
+                  rates=None, workspace=None):
+    """Drafted tokens checked against the target's probabilities, and the next token of each sequence.  target float32
+    [n_seqs, max_drafts + 1, vocab] and draft_logits [n_seqs, max_drafts, vocab] (None: drafted by lookup) row after row; drafts
+    int32 [n_seqs, max_drafts] (None with max_drafts 0), uniform float32 [n_seqs, max_drafts + 1]; n_drafts int32 and
+    temperature float32 [n_seqs] or None.  Into tokens int32 [n_seqs, max_drafts + 1], accepted int32 [n_seqs], and, where given,
+    logprobs float32 [n_seqs, max_drafts + 1] and rates float32 [n_seqs, max_drafts].  workspace: a uint8 tensor of
+    verify_drafts_workspace_bytes(...)."""
+    library, device = _lib or lib(), _device_of(target, "target")
+    n, rows, vocab = target.shape
+    d = rows - 1
+    p_target, target_stride, _ = _logits_of(target, n, rows, "target", device)
+    p_draft = draft_stride = 0
+    if draft_logits is not None:
+        p_draft, draft_stride, width = _logits_of(draft_logits, n, d, "draft_logits", device)
+        if width != vocab:
+            raise ValueError(f"draft logits of {width} tokens, the target's of {vocab}")
+    rc = library.qlin_launch_verify_drafts(
+        p_target, target_stride, p_draft if d else 0, draft_stride, _values_of(drafts, n * d, _I32, "drafts", device),
+        _values_of(n_drafts, n, _I32, "n_drafts", device), _values_of(temperature, n, _F32, "temperature", device),
+        _values_of(uniform, n * rows, _F32, "uniform", device), _values_of(tokens, n * rows, _I32, "tokens", device),
+        _values_of(accepted, n, _I32, "accepted", device), _values_of(logprobs, n * rows, _F32, "logprobs", device),
+        _values_of(rates, n * d, _F32, "rates", device), n, d, vocab, _values_of(workspace, 0, _U8, "workspace", device),
+        0 if workspace is None else workspace.numel())
+    if rc != 0:
+        raise QlinError("qlin_launch_verify_drafts", rc)

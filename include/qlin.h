@@ -108,6 +108,11 @@ size_t qlin_q8_1_row_bytes(int in_dim);
  * or the raw f32 sum when store_raw_sum != 0.  Replaces launch_quantize_q8_1 (launch.cu:201-207). */
 int qlin_launch_quantize_q8_1(const float *x, uint8_t *x_q8_1, int in_dim, int m, int store_raw_sum);
 
+/* x[r, i] = d * q of the Q8_1 blocks that qlin_launch_quantize_q8_1 writes (mmq 0) or qlin_launch_quantize_q8_1_mmq
+ * (mmq not 0) for m rows of in_dim values: what they stand for, d as the f16 it is stored as.  No reference
+ * counterpart. */
+int qlin_launch_dequantize_q8_1(const uint8_t *x_q8_1, float *x, int in_dim, int m, int mmq);
+
 /* y[r, o] = W[o] . x_q8_1[r] with block-dot semantics (kernel.cu:2305-2402).
  * Replaces launch_quant_matmul_q8_1 (launch.cu:500-531). */
 int qlin_launch_quant_matmul_q8_1(int type, const uint8_t *weight, size_t row_bytes, const uint8_t *x_q8_1,
@@ -198,6 +203,31 @@ int qlin_launch_quant_down_f32_indexed_accum_ordered(int type, const uint8_t *do
  * Replaces launch_moe_router_topk (kernel.cu:3463-3511). */
 int qlin_launch_moe_router_topk(const float *router_logits, int *top_idx, float *top_w, int tokens,
                                 int n_experts, int k, float routed_scaling);
+
+/* Routing by scores (no reference counterpart; qlin_launch_moe_router_topk is the reference's softmax alone).  For a
+ * token's logits l over n_experts experts:
+ *   s[e] = softmax(l)[e], or 1 / (1 + exp(-l[e])) where sigmoid is not 0, computed in 64 bits and rounded to f32;
+ *   c[e] = s[e] + bias[e] (f32), or s[e] without a bias: what the choice goes by;
+ *   with n_groups > 1 the experts stand in n_groups groups of n_experts / n_groups one after the other, and only those of
+ *     the top_groups best ones are left: by a group's largest c, or by the f32 sum of its two largest where group_pairs is
+ *     not 0 (a group with one expert that is left: by that one);
+ *   expert_ids[t, 0 .. k) = the experts of the k largest c that are left, the largest first;
+ *   weights[t, r] = s of that expert (not c), divided by the sum of the k picks' s plus 1e-20 where renormalise is not 0,
+ *     times scaling, in 64 bits and rounded once.
+ * Among equals the lowest index goes first, for experts and for groups.  An expert whose logit is not finite has score 0,
+ * and one with such a logit or with a c that is -inf or NaN (a bias of -inf switches an expert off) is not picked: where
+ * none is left the picks are -1 with weight 0, which the routed products skip.  So the picks go straight into
+ * qlin_moe_routed_decode_indexed and qlin_moe_routed_decode_grouped.
+ * logits_stride: floats from a token's logits to the next one's, >= n_experts.  n_experts <= 1024, n_groups <= 64 and
+ * k <= 64 (else QLIN_ERR_LIMIT); n_groups divides n_experts, 1 <= top_groups <= n_groups, and k is at most the number of
+ * experts in top_groups groups (else QLIN_ERR_SHAPE). */
+typedef struct qlin_moe_routing {
+    const float *bias; /* [n_experts], or NULL */
+    int sigmoid, n_groups, top_groups, group_pairs, renormalise;
+    float scaling;
+} qlin_moe_routing;
+int qlin_launch_moe_route(const qlin_moe_routing *how, const float *router_logits, size_t logits_stride, int *expert_ids,
+                          float *weights, int tokens, int n_experts, int k);
 
 /* out[i] += weight * expert_out[i] (one expert's output into the MoE sum).
  * Replaces launch_moe_accumulate (kernel.cuh:339, kernel.cu:3514-3518). */

@@ -169,8 +169,82 @@ typedef struct qlin_logits_controls {
     int max_history, max_bias;
 } qlin_logits_controls;
 
+/* ---- the residual's addition with the norm, into f32 or Q8_1 blocks ------------------------------
+ *
+ * qlin_launch_add_rms_norm, for each of rows rows of hidden values:
+ *   s = x + delta (f32; delta NULL: s = x);   sum = s (sum NULL: not stored);
+ *   y[j] = s[j] * (mean_j s^2 + eps)^(-1/2) * w[j], in 64 bits and rounded once, w of norm_type 0 (bf16) or 1 (f16), plus
+ *   one if one_plus;   normed = y (NULL: not stored);
+ *   q8_1 = the Q8_1 blocks of y, byte for byte those of qlin_launch_quantize_q8_1 (mmq 0) or
+ *   qlin_launch_quantize_q8_1_mmq (mmq not 0) with raw_sum (NULL: not stored).
+ * normed or q8_1 or both.  *_stride: floats from a row to the next one, >= hidden.  sum may be x or delta (same pointer and
+ * stride: the residual stream in place), and normed may be x or delta where sum is not; else outputs overlap nothing.
+ * Norm weights 2-byte aligned, q8_1 and the rest 4-byte (else QLIN_ERR_ALIGN).
+ */
+
+/* ---- low-rank adapters of many requests beside a shared projection -------------------------------
+ *
+ * qlin_launch_lora_add: for each row r with the adapter a = adapter_ids[r] and n_mats (1 .. 4) projections that read the same x,
+ *   y[r, o] = base[r, o] + scales[a] * sum_{k < ranks[a]} B[a, o, k] * (sum_i A[a, k, i] x[r, i]).
+ * A row whose id is negative or >= n_adapters has no adapter: y[r] = base[r].  y may be base (same pointer and stride: rows
+ * without an adapter are then not touched), else it overlaps nothing.  Requests with adapters of their own stand in one
+ * batch in any order, each adapter's weights are read for all the rows that have it.
+ * The adapters stand in slots of max_rank: a [n_adapters, max_rank, in_dim] and b [n_adapters, out_dim, max_rank] of
+ * weight_type 0 (bf16), 1 (f16) or 2 (f32).  ranks [n_adapters] (NULL: max_rank each; clamped to 0 .. max_rank) says how
+ * much of a slot counts: the rest is not used, whatever it holds.  scales [n_adapters] or NULL (1).
+ * Accuracy: products of exact operands, sums in f32; A x is held in f32, then multiplied by the scale.
+ * in_dim and max_rank are multiples of 8 (else QLIN_ERR_SHAPE), max_rank <= 256, n_adapters <= 1024 and rows <= 65536 (else
+ * QLIN_ERR_LIMIT); a and b 16-byte aligned, the rest 4-byte (else QLIN_ERR_ALIGN).  Strides in floats, >= the row.
+ * workspace: qlin_lora_workspace_bytes(...) bytes, 16-byte aligned, used by nothing else while the launches run (calls
+ * on one stream, or graphs that are not replayed at the same time, may share it); its contents do not matter before or after.
+ */
+typedef struct qlin_lora {
+    const void *a, *b;
+    const float *base;
+    float *y;
+    size_t base_stride, y_stride;
+    int out_dim;
+} qlin_lora;
+
+/* ---- drafted tokens against the target's probabilities -------------------------------------------
+ *
+ * qlin_launch_verify_drafts, for each of n_seqs sequences with n = n_drafts[s] drafted tokens x_0 .. x_{n-1} (n_drafts NULL:
+ * max_drafts; clamped to 0 .. max_drafts):
+ *   p_i = softmax(target row i / T), i <= n, and q_i = softmax(draft row i / T), i < n, T = temperature[s] (NULL: 1); without
+ *     draft logits q_i is 1 at x_i (a draft by lookup).  T = 0 (or below, or NaN): all of it at the largest logit, the
+ *     lowest index among equals;
+ *   rates[s, i] = min(1, p_i(x_i) / q_i(x_i)) for i < n (where q_i(x_i) is 0: 1 if p_i(x_i) > 0, else 0), 0 after that;
+ *   x_i is accepted if those before it were and uniform[s, i] * q_i(x_i) < p_i(x_i);
+ *   accepted[s] = m, the number of accepted ones.  The next token y comes from max(p_m - q_m, 0) where x_m was rejected, and
+ *     from p_n where all were accepted (from p_m, too, where the former is 0 everywhere): the first v at which the sum of
+ *     the weights up to v is above uniform[s, max_drafts] times their sum over all v;
+ *   tokens[s] = x_0 .. x_{m-1}, y, and -1 after that;  logprobs[s, i] = log p_i(tokens[s, i]) for i <= m, 0 after that.
+ * So what comes out is distributed as the target alone would have it, and with max_drafts 0 the call is the draw of one
+ * token for each sequence.  rates and logprobs may be NULL.
+ * Everything is computed in 64 bits: a random number falls to one side of a border whatever the order of the sums is.
+ * target [n_seqs, max_drafts + 1] rows and draft [n_seqs, max_drafts] rows of vocab logits, target_stride and draft_stride
+ * floats from a row to the next (>= vocab); uniform [n_seqs, max_drafts + 1] in [0, 1) (below: 0; above: the largest f32
+ * below 1; NaN: 0).  A logit that is NaN counts as -inf; tokens at +inf share a row's probability.  A row without any
+ * logit above -inf accepts nothing; where y would come from it, y is 0 with logprob -inf.  A drafted token outside
+ * [0, vocab) is not accepted (and by lookup takes nothing from p).
+ * vocab <= 1 << 28 and max_drafts <= 63 (else QLIN_ERR_LIMIT).  Pointers 4-byte aligned, the workspace 16-byte
+ * (qlin_verify_drafts_workspace_bytes(...) bytes; rules as qlin_launch_lora_add's).
+ */
+
 int qlin_launch_rms_norm(const float *input, float *output, const uint16_t *weight, int weight_type, int rows,
                          int hidden_size, float eps, int one_plus);
+int qlin_launch_add_rms_norm(const float *x, size_t x_stride, const float *delta, size_t delta_stride, float *sum,
+                             size_t sum_stride, const uint16_t *weight, int norm_type, float eps, int one_plus,
+                             float *normed, size_t normed_stride, uint8_t *q8_1, int mmq, int raw_sum, int rows, int hidden);
+size_t qlin_lora_workspace_bytes(int rows, int n_mats, int n_adapters, int max_rank, int in_dim);
+int qlin_launch_lora_add(const qlin_lora *mats, int n_mats, int weight_type, int n_adapters, int max_rank, int in_dim,
+                         const int *ranks, const float *scales, const float *x, size_t x_stride, const int *adapter_ids,
+                         int rows, void *workspace, size_t workspace_bytes);
+size_t qlin_verify_drafts_workspace_bytes(int n_seqs, int max_drafts, int vocab);
+int qlin_launch_verify_drafts(const float *target, size_t target_stride, const float *draft, size_t draft_stride,
+                              const int *drafts, const int *n_drafts, const float *temperature, const float *uniform,
+                              int *tokens, int *accepted, float *logprobs, float *rates, int n_seqs, int max_drafts,
+                              int vocab, void *workspace, size_t workspace_bytes);
 int qlin_launch_rope_store_kv(float *q, const float *k, const float *v, float *key_cache, float *value_cache, int rows,
                               int n_heads, int kv_heads, int head_dim, int max_seq_len, const int *start_pos_dev,
                               float rope_theta);
