@@ -1,8 +1,8 @@
 // qlin_norm.hip -- the residual's addition, the RMSNorm and its result in f32 and in Q8_1 blocks in one pass, and Q8_1
 // blocks read back as the values they stand for (qlin_launch_add_rms_norm, qlin_launch_dequantize_q8_1), gfx950.
 //
-// Mathematics (qlin_decoder.h): s = x + delta, y = s (mean s^2 + eps)^(-1/2) w, blocks of 32 values as codes rint(y 127 /
-// amax).  The sum of squares, the root and the product are in f64: y then is the same f32 value whatever the order of
+// Mathematics (qlin_decoder.h): s = x + delta, y = s (mean s^2 + eps)^(-1/2) w, blocks of 32 values as codes rint(y / d),
+// d = amax / 127.  The sum of squares, the root and the product are in f64: y then is the same f32 value whatever the order of
 // the sum, and so are the codes (an f64 operation takes an f32 one's time here).
 //
 // A row is taken by W waves, 4 consecutive values a lane and U such runs in registers, so that x is read once; 8 lanes hold
@@ -127,11 +127,11 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(Norm
             const int b = i / 32, j = t & 7;
             if (a.mmq) {
                 uint8_t *at = a.q8 + (static_cast<size_t>(b >> 2) * a.rows + row) * 144;
-                quantize_values_q8_1_lanes(y, j, reinterpret_cast<uint32_t *>(at) + (b & 3),
+                quantize_normed_lanes(y, j, reinterpret_cast<uint32_t *>(at) + (b & 3),
                                            reinterpret_cast<uint32_t *>(at + 16 + 32 * (b & 3)), a.raw != 0);
             } else {
                 uint32_t *at = reinterpret_cast<uint32_t *>(a.q8 + (static_cast<size_t>(row) * (a.padded / 32) + b) * 36);
-                quantize_values_q8_1_lanes(y, j, at, at + 1, a.raw != 0);
+                quantize_normed_lanes(y, j, at, at + 1, a.raw != 0);
             }
         }
     };

@@ -61,10 +61,19 @@ __device__ __forceinline__ void quantize_block_q8_1(const float *src, int valid,
     quantize_block_q8_1(src, valid, out, out + 1, raw);
 }
 
-// One Q8_1 block by 8 consecutive lanes (all active) from their values, 4 each in order (0 past the row's end): lane j = 0..7
-// writes its q into dword j at q8, lane 0 (d, s) at ds.  The same bytes as quantize_block_q8_1: the maximum and the integer
-// sum have no order, and the raw sum's adds pair the same values (lanes 4, 2 and 1 apart, then within the lane).
-__device__ __forceinline__ void quantize_values_q8_1_lanes(float (&v)[4], int j, uint32_t *ds, uint32_t *q8, bool raw) {
+// One Q8_1 block by 8 consecutive lanes (all active): lane j = 0..7 takes the 4 values at index k0 of the
+// row src (those at in_dim or past it are 0) and writes their q; lane 0 writes (d, s).  The same bytes as
+// quantize_block_q8_1: the maximum and the integer sum have no order, and the raw sum's adds pair the
+// same values (lanes 4, 2 and 1 apart, then within the lane).
+__device__ __forceinline__ void quantize_block_q8_1_lanes(const float *src, int k0, int in_dim, int j, uint32_t *out,
+                                                          bool raw) {
+    float v[4];
+    if (k0 + 4 <= in_dim) {
+        __builtin_memcpy(v, src + k0, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = k0 + e < in_dim ? src[k0 + e] : 0.0f;
+    }
     float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
     amax = fmaxf(amax, dpp_move<0xb1>(amax));
     amax = fmaxf(amax, dpp_move<0x4e>(amax));
@@ -76,6 +85,46 @@ __device__ __forceinline__ void quantize_values_q8_1_lanes(float (&v)[4], int j,
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         int q = static_cast<int>(rintf(__fmul_rn(v[e], id)));
+        q = q < -127 ? -127 : (q > 127 ? 127 : q);
+        qsum += q;
+        word |= (static_cast<uint32_t>(q) & 0xffu) << (8 * e);
+    }
+    out[1 + j] = word;
+    float sum;
+    if (raw) {  // uniform
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], off, 64);
+        sum = (v[0] + v[2]) + (v[1] + v[3]);
+    } else {
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) qsum += __shfl_xor(qsum, off, 64);
+        sum = __fmul_rn(d, static_cast<float>(qsum));
+    }
+    if (j == 0) *out = f32_to_f16_bits(d) | (f32_to_f16_bits(sum) << 16);
+}
+
+// One block of a norm's output by 8 consecutive lanes (all active) from their values, 4 each in order (0 past the row's end):
+// lane j = 0..7 writes its q into dword j at q8, lane 0 (d, s) at ds.  As quantize_block_q8_1_lanes but for the scale, which
+// is the 8-bit cache's, amax * (1.0f / 127.0f) (a division by 127 is off from it by at most a step of f32), and for a block
+// with a value that is not finite: scale NaN, q 0.
+__device__ __forceinline__ void quantize_normed_lanes(float (&v)[4], int j, uint32_t *ds, uint32_t *q8, bool raw) {
+    // (magnitudes as whole numbers: infinities are above all finite ones, NaN above these)
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+    top = max(top, __builtin_bit_cast(uint32_t, dpp_move<0xb1>(__builtin_bit_cast(float, top))));
+    top = max(top, __builtin_bit_cast(uint32_t, dpp_move<0x4e>(__builtin_bit_cast(float, top))));
+    top = max(top, __builtin_bit_cast(uint32_t, dpp_move<0x141>(__builtin_bit_cast(float, top))));
+    const bool finite = top < 0x7f800000u;
+    const float d = finite ? __fmul_rn(__builtin_bit_cast(float, top), 1.0f / 127.0f) : __builtin_nanf("");
+    const float id = d >= 0x1p-126f ? 1.0f / d : 0.0f;  // (below, d as f16 is 0 as well; 0 for NaN)
+    uint32_t word = 0;
+    int qsum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        int q = finite ? static_cast<int>(rintf(__fmul_rn(v[e], id))) : 0;
         q = q < -127 ? -127 : (q > 127 ? 127 : q);
         qsum += q;
         word |= (static_cast<uint32_t>(q) & 0xffu) << (8 * e);
@@ -94,19 +143,6 @@ __device__ __forceinline__ void quantize_values_q8_1_lanes(float (&v)[4], int j,
         sum = __fmul_rn(d, static_cast<float>(qsum));
     }
     if (j == 0) *ds = f32_to_f16_bits(d) | (f32_to_f16_bits(sum) << 16);
-}
-
-// ... of the 4 values at index k0 of the row src (those at in_dim or past it are 0), into the contiguous block at out.
-__device__ __forceinline__ void quantize_block_q8_1_lanes(const float *src, int k0, int in_dim, int j, uint32_t *out,
-                                                          bool raw) {
-    float v[4];
-    if (k0 + 4 <= in_dim) {
-        __builtin_memcpy(v, src + k0, sizeof(v));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k0 + e < in_dim ? src[k0 + e] : 0.0f;
-    }
-    quantize_values_q8_1_lanes(v, j, out, out + 1, raw);
 }
 
 // Block qb of a weight row against activation block (dx, sx, qx[32]).

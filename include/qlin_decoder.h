@@ -175,8 +175,10 @@ typedef struct qlin_logits_controls {
  *   s = x + delta (f32; delta NULL: s = x);   sum = s (sum NULL: not stored);
  *   y[j] = s[j] * (mean_j s^2 + eps)^(-1/2) * w[j], in 64 bits and rounded once, w of norm_type 0 (bf16) or 1 (f16), plus
  *   one if one_plus;   normed = y (NULL: not stored);
- *   q8_1 = the Q8_1 blocks of y, byte for byte those of qlin_launch_quantize_q8_1 (mmq 0) or
- *   qlin_launch_quantize_q8_1_mmq (mmq not 0) with raw_sum (NULL: not stored).
+ *   q8_1 = the Q8_1 blocks of y (NULL: not stored), where qlin_launch_quantize_q8_1 (mmq 0) or qlin_launch_quantize_q8_1_mmq
+ *   (mmq not 0) put theirs, with raw_sum as there.  The scale is the 8-bit cache's, d = amax * (1.0f / 127.0f), which is at
+ *   most an f32 step from theirs; code = clamp(round-to-even(y * (1 / d)), -127, 127), 0 where d is below 2^-126; a block
+ *   with a value that is not finite has scale NaN and codes 0.
  * normed or q8_1 or both.  *_stride: floats from a row to the next one, >= hidden.  sum may be x or delta (same pointer and
  * stride: the residual stream in place), and normed may be x or delta where sum is not; else outputs overlap nothing.
  * Norm weights 2-byte aligned, q8_1 and the rest 4-byte (else QLIN_ERR_ALIGN).
@@ -193,7 +195,7 @@ typedef struct qlin_logits_controls {
  * weight_type 0 (bf16), 1 (f16) or 2 (f32).  ranks [n_adapters] (NULL: max_rank each; clamped to 0 .. max_rank) says how
  * much of a slot counts: the rest is not used, whatever it holds.  scales [n_adapters] or NULL (1).
  * Accuracy: products of exact operands, sums in f32; A x is held in f32, then multiplied by the scale.
- * in_dim and max_rank are multiples of 8 (else QLIN_ERR_SHAPE), max_rank <= 256, n_adapters <= 1024 and rows <= 65536 (else
+ * n_adapters >= 1, in_dim and max_rank are multiples of 8, from 8 on (else QLIN_ERR_SHAPE), max_rank <= 256, n_adapters <= 1024 and rows <= 65536 (else
  * QLIN_ERR_LIMIT); a and b 16-byte aligned, the rest 4-byte (else QLIN_ERR_ALIGN).  Strides in floats, >= the row.
  * workspace: qlin_lora_workspace_bytes(...) bytes, 16-byte aligned, used by nothing else while the launches run (calls
  * on one stream, or graphs that are not replayed at the same time, may share it); its contents do not matter before or after.

@@ -2,8 +2,9 @@
 (qlin_launch_dequantize_q8_1).
 
 The sum is one f32 addition and has to be equal; y is computed in 64 bits and rounded once, so it is off by at most half a step
-of f32 (2^-24 of the value; 2^-50 more for the 64-bit arithmetic); the blocks are, byte for byte, those that the quantizers give
-for the y that the same call returns."""
+of f32 (2^-24 of the value; 2^-50 more for the 64-bit arithmetic); the blocks are, byte for byte, those of the documented steps
+for the y that the same call returns.  Sums of the values themselves (raw_sum) are f32 sums of 32 terms (a tree of depth 5: 5
+half steps of f32 of the sum of magnitudes) rounded to f16 once (half a step, 2^-11, or half of its smallest, 2^-25)."""
 import numpy as np
 import pytest
 
@@ -84,20 +85,33 @@ def _run(torch, rng, rows, hidden, *, delta=True, kind=0, one_plus=0, mmq=False,
     assert (got[rows:] == 7.0).all() and (got[:, hidden:] == 7.0).all()
     got = got[:rows, :hidden]
     if blocks:
-        ref = torch.full((size + 64,), 0x55, dtype=torch.uint8, device="cuda")
-        flat = dev(got)
-        qlin.call("qlin_launch_quantize_q8_1_mmq" if mmq else "qlin_launch_quantize_q8_1", flat, ref, hidden, rows, int(raw))
-        assert torch.equal(q, ref)
+        unit = 128 if mmq else 32
+        v = np.zeros((rows, -(-hidden // unit) * unit), np.float32)
+        v[:, :hidden] = got
+        v = v.reshape(rows, -1, 32)
+        scale = np.abs(v).max(2) * (np.float32(1) / np.float32(127))
+        inverse = np.where(scale >= 2.0 ** -126, np.float32(1) / np.maximum(scale, np.float32(2.0 ** -126)), np.float32(0))
+        q_want = np.clip(np.rint(v * inverse[:, :, None]), -127, 127).astype(np.int8)
+        b = host(q)
+        assert (b[size:] == 0x55).all()
+        if mmq:
+            b = b[:size].reshape(-1, rows, 144).transpose(1, 0, 2)
+            heads, codes = b[:, :, :16].copy().view(np.float16).reshape(rows, -1, 2), b[:, :, 16:].copy().view(np.int8)
+        else:
+            b = b[:size].reshape(rows, -1, 36)
+            heads, codes = b[:, :, :4].copy().view(np.float16).reshape(rows, -1, 2), b[:, :, 4:].copy().view(np.int8)
+        assert np.array_equal(codes.reshape(q_want.shape), q_want)
+        assert np.array_equal(heads[:, :, 0], scale.astype(np.float16))
+        if raw:
+            v64 = v.astype(np.float64)
+            sums = v64.sum(2)
+            assert (np.abs(heads[:, :, 1] - sums) <= 2.0 ** -11 * np.abs(sums) + 2.0 ** -25 + 6 * 2.0 ** -24 * np.abs(v64).sum(2)).all()
+        else:
+            assert np.array_equal(heads[:, :, 1], (scale * q_want.sum(2, dtype=np.int32).astype(np.float32)).astype(np.float16))
+        d, codes = heads[:, :, 0], codes.reshape(rows, -1)
         back = torch.full((rows * hidden + 5,), 7.0, device="cuda")
         qlin.dequantize_q8_1(q, back, hidden, rows, mmq=mmq)
-        b = host(q)[:size]
-        if mmq:
-            b = b.reshape(-1, rows, 144).transpose(1, 0, 2)
-            d, codes = b[:, :, :16].copy().view(np.float16)[:, :, ::2].reshape(rows, -1), b[:, :, 16:].reshape(rows, -1)
-        else:
-            b = b.reshape(rows, -1, 36)
-            d, codes = b[:, :, :2].copy().view(np.float16)[:, :, 0], b[:, :, 4:].reshape(rows, -1)
-        values = d.astype(np.float32).repeat(32, 1) * codes.copy().view(np.int8).astype(np.float32)
+        values = d.astype(np.float32).repeat(32, 1) * codes.astype(np.float32)
         back = host(back)
         assert np.array_equal(back[:rows * hidden].reshape(rows, hidden), values[:, :hidden], equal_nan=True) and (back[rows * hidden:] == 7.0).all()
     return got, want
@@ -184,3 +198,41 @@ def test_many_rows():
         banner(f"add_rms_norm rows={rows} hidden={hidden}")
         got, want = _run(torch, np.random.default_rng(rows), rows, hidden, mmq=True)
         assert (np.abs(got - want) <= HALF_STEP * np.abs(want) + 2.0 ** -149).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mmq", [False, True])
+def test_blocks_as_the_quantizers(mmq):
+    """qlin_launch_quantize_q8_1's blocks of the same y: scales a step of f16 apart at most (2^-10 of 127 steps) and codes one,
+    which few are."""
+    torch = _gpu()
+    from gpu_util import banner, host
+    banner(f"add_rms_norm and quantize_q8_1 mmq={mmq}")
+    rows, hidden = 50, 4096
+    x = torch.randn(rows, hidden, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    y, size = torch.empty_like(x), qlin.q8_1_bytes(hidden, rows, mmq)
+    q, ref = (torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(2))
+    qlin.add_rms_norm(x, None, None, torch.ones(hidden, dtype=torch.bfloat16, device="cuda"), 0, 1e-6, 0, normed=y, q8_1=q, mmq=mmq)
+    qlin.call("qlin_launch_quantize_q8_1_mmq" if mmq else "qlin_launch_quantize_q8_1", y, ref, hidden, rows, 0)
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    qlin.dequantize_q8_1(q, a, hidden, rows, mmq=mmq)
+    qlin.dequantize_q8_1(ref, b, hidden, rows, mmq=mmq)
+    step = np.abs(host(y)).reshape(rows, -1, 32).max(2).repeat(32, 1) / 127
+    assert (np.abs(host(a) - host(b)) <= 1.13 * step).all() and (host(a) != host(b)).mean() <= 1e-2
+
+
+@pytest.mark.gpu
+def test_blocks_that_are_not_finite():
+    torch = _gpu()
+    from gpu_util import banner, host
+    banner("add_rms_norm blocks that are not finite")
+    x = torch.ones(3, 96, device="cuda")
+    x[1, 40] = float("nan")
+    x[2, 40] = float("inf")
+    q = torch.zeros(qlin.q8_1_bytes(96, 3), dtype=torch.uint8, device="cuda")
+    y = torch.zeros(3, 96, device="cuda")
+    qlin.add_rms_norm(x, None, None, torch.ones(96, dtype=torch.bfloat16, device="cuda"), 0, 1e-6, 0, q8_1=q)
+    qlin.dequantize_q8_1(q, y, 96, 3)
+    got = host(y)
+    assert np.isfinite(got[0]).all() and np.isnan(got[1]).all()
+    assert (got[2, :32] == 0).all() and np.isnan(got[2, 32:64]).all() and (got[2, 64:] == 0).all()  # 1 / inf, inf / inf
