@@ -26,6 +26,9 @@ namespace qlin {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kDecideThreads = 1024;  // a wave a row of a sequence's
+constexpr int kDrawThreads = 512;
+constexpr int kMostVocab = 1 << 21;    // a slice a thread of the draws
 constexpr int kMostDrafts = 63;
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
@@ -34,12 +37,12 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 struct Stat {
     double sum;  // of exp((l - top) / T)
     float top;
-    int at;      // of top, the first one
+    int at;      // of top, the first one; only at T = 0
 };
 // What is left to do for a sequence after verify_decide_kernel.
 struct Rest {
     double inv_p, inv_q;  // one over the sums
-    double heat;          // 1 / T
+    double heat;          // 32 / (T ln 2)
     float top_p, top_q;
     int row;              // -1: nothing is left
 };
@@ -60,22 +63,42 @@ struct VerifyArgs {
 __device__ __forceinline__ int drafts_of(const VerifyArgs &a, int seq) {
     return a.n_drafts ? min(max(a.n_drafts[seq], 0), a.max_drafts) : a.max_drafts;
 }
-__device__ __forceinline__ double heat_of(const VerifyArgs &a, int seq) {
-    const float t = a.temperature ? a.temperature[seq] : 1.0f;
-    return t > 0.0f ? 1.0 / static_cast<double>(t) : 0.0;  // 0: the largest takes all
-}
-__device__ __forceinline__ bool greedy_of(const VerifyArgs &a, int seq) { return a.temperature && !(a.temperature[seq] > 0.0f); }
+constexpr double kSteps = 0x1.71547652b82fep+5;  // 32 / ln 2
+__device__ __forceinline__ double heat_of(float t) { return t > 0.0f ? kSteps / static_cast<double>(t) : 0.0; }
+__device__ __forceinline__ float temperature_of(const VerifyArgs &a, int seq) { return a.temperature ? a.temperature[seq] : 1.0f; }
 __device__ __forceinline__ const float *target_row(const VerifyArgs &a, int seq, int i) {
     return a.target + (static_cast<size_t>(seq) * (a.max_drafts + 1) + i) * a.target_stride;
 }
 __device__ __forceinline__ const float *draft_row(const VerifyArgs &a, int seq, int i) {
     return a.draft + (static_cast<size_t>(seq) * a.max_drafts + i) * a.draft_stride;
 }
-// exp((l - top) / T) of a logit l of a row whose largest is top; 0 for what is not above -inf (NaN among it), 1 at top
-__device__ __forceinline__ double weight(float l, float top, double heat) {
-    return l == top && l > -INFINITY ? 1.0 : l > -INFINITY ? exp_f64((static_cast<double>(l) - static_cast<double>(top)) * heat) : 0.0;
+__device__ __forceinline__ float uniform_at(float u) { return fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f); }
+__device__ __forceinline__ float number(float l) { return fmaxf(l, -INFINITY); }  // -inf for NaN
+
+// exp((l - top) / T), heat = 32 / (T ln 2): 2^(n / 32) from a table of 32 values in LDS, 2^(r / 32) for the rest |r| <= 1/2 by
+// its Taylor polynomial of degree 5 (the first term left out is below 2e-15 of it).  16 operations; the polynomial of degree
+// 13 alone (exp_f64) took 28 with what is around it, and the pass over 216 rows of 151936 took 44.7 us, so 29.1 (4.5 TB/s).
+// l is not NaN.  0 for l = -inf, 1 at top, also where both are infinite; a row whose top is -inf is not asked.
+__device__ __forceinline__ double step_of(int j) { return exp_f64(j * 0x1.62e42fefa39efp-6); }  // 2^(j / 32)
+__device__ __forceinline__ double weight(float l, double top, double heat, const double *steps) {
+    const double d = fmin(static_cast<double>(l) - top, 0.0);    // (0 for inf - inf)
+    const double t = fmax(d * heat, -35200.0);                   // (and this for -inf * 0)
+    const double m = t + 0x1.8p52;
+    const int n = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, m)));
+    const double r = t - (m - 0x1.8p52);
+    constexpr double c = 0x1.62e42fefa39efp-6;  // ln 2 / 32
+    double p = __builtin_fma(c * c * c * c * c / 120.0, r, c * c * c * c / 24.0);
+    p = __builtin_fma(p, r, c * c * c / 6.0);
+    p = __builtin_fma(p, r, c * c / 2.0);
+    p = __builtin_fma(p, r, c);
+    const double s = steps[n & 31];
+    return __builtin_ldexp(__builtin_fma(s * r, p, s), n >> 5);
 }
-__device__ __forceinline__ float uniform_at(const float *p) { return fminf(fmaxf(*p, 0.0f), 0x1.fffffep-1f); }
+
+// log exp((l - top) / T)
+__device__ __forceinline__ double log_of(float l, float top, float t) {
+    return l == top ? 0.0 : (static_cast<double>(l) - static_cast<double>(top)) / static_cast<double>(t);
+}
 
 // the larger of two (value, index) pairs, the lower index among equals; NaN never
 __device__ __forceinline__ void better(float &v, int &i, float w, int j) {
@@ -88,12 +111,25 @@ __device__ __forceinline__ void wave_best(float &v, int &i) {
     for (int o = 32; o > 0; o >>= 1) better(v, i, __shfl_xor(v, o, 64), __shfl_xor(i, o, 64));
 }
 
+// logits i .. i + 3 of the n at p, NaN and what is past them as -inf
+__device__ __forceinline__ f32x4v logits_at(const float *p, int i, int n) {
+    f32x4v v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (i + 4 <= n) {
+        __builtin_memcpy(&v, __builtin_assume_aligned(p + i, 4), 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) v[e] = p[i + e];
+    }
+    return v;
+}
+
 // U runs of 4 tokens a thread.
 template <int U>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
     __shared__ float s_v[kWaves];
     __shared__ int s_i[kWaves];
-    __shared__ double s_sum[kWaves];
+    __shared__ double s_sum[kWaves], s_steps[32];
     const int rows = a.max_drafts + 1 + (a.draft ? a.max_drafts : 0);
     const int slice = blockIdx.x % a.slices, r = blockIdx.x / a.slices % rows, seq = blockIdx.x / a.slices / rows;
     const int n_drafts = drafts_of(a, seq);
@@ -102,25 +138,27 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
     const float *src = (r <= a.max_drafts ? target_row(a, seq, r) : draft_row(a, seq, r - a.max_drafts - 1)) + v0;
     f32x4v x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int i = 4 * (u * kThreads + tid);
-        x[u] = f32x4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i + 4 <= n) {
-            __builtin_memcpy(&x[u], __builtin_assume_aligned(src + i, 4), 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i + e < n) x[u][e] = src[i + e];
-        }
-    }
-    const double heat = heat_of(a, seq);
+    for (int u = 0; u < U; ++u) x[u] = logits_at(src, 4 * (u * kThreads + tid), n);
+    const float t = temperature_of(a, seq);
+    if (tid < 32) s_steps[tid] = step_of(tid);
     float top = -INFINITY;
     int at = 0;
+    if (t > 0.0f) {  // uniform
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) better(top, at, x[u][e], v0 + 4 * (u * kThreads + tid) + e);
-    wave_best(top, at);
+            for (int e = 0; e < 4; ++e) {
+                x[u][e] = number(x[u][e]);
+                top = fmaxf(top, x[u][e]);
+            }
+        top = wave_max_dpp(top);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) better(top, at, x[u][e], v0 + 4 * (u * kThreads + tid) + e);
+        wave_best(top, at);
+    }
     if ((tid & 63) == 0) {
         s_v[tid >> 6] = top;
         s_i[tid >> 6] = at;
@@ -131,143 +169,198 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) better(top, at, s_v[w], s_i[w]);
     double sum = 0.0;
-    if (!greedy_of(a, seq)) {
+    if (t > 0.0f) {
+        const double heat = heat_of(t), top64 = top;
+        double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += weight(x[u][e], top, heat);
-        sum = wave_sum_f64(sum);
+            for (int e = 0; e < 4; ++e) part[e] += weight(x[u][e], top64, heat, s_steps);
+        sum = wave_sum_f64((part[0] + part[1]) + (part[2] + part[3]));
+        if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
+        __syncthreads();
+        sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
     }
-    if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        sum = 0.0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
-        a.stats[(static_cast<size_t>(seq) * (2 * a.max_drafts + 1) + r) * a.slices + slice] = Stat{sum, top, at};
-    }
+    if (tid == 0) a.stats[(static_cast<size_t>(seq) * (2 * a.max_drafts + 1) + r) * a.slices + slice] = Stat{sum, top, at};
 }
 
-// The running sum of one value a thread over the workgroup, in thread order: what stands before this thread's, and the total.
-__device__ __forceinline__ double before(double v, double &total, double *s_part) {
-    double run = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(run, o, 64);
-        if ((threadIdx.x & 63) >= static_cast<unsigned>(o)) run += up;
-    }
-    __syncthreads();  // (s_part's readers of before are done)
-    if ((threadIdx.x & 63) == 63) s_part[threadIdx.x >> 6] = run;
-    __syncthreads();
-    double base = 0.0;
-    total = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < static_cast<int>(threadIdx.x >> 6)) base += s_part[w];
-        total += s_part[w];
-    }
-    return base + (run - v);
-}
-
-// The workgroup's draw: the first index i of 0 .. n - 1 at which the running sum of weight(i) (>= 0) is above goal(total); where
-// rounding leaves none, the last one with a weight; -1 where there is no weight at all.  base: the running sum before i.
-// Each thread takes consecutive indices.  A thread's sum and its walk add the same numbers from another start, so a goal
-// can lie beyond the walk's end by a rounding: then its last index with a weight.
-struct Pick {
-    int at;
-    double base;
-};
-template <class Weight, class Goal>
-__device__ __forceinline__ Pick draw(int n, Weight weight_of, Goal goal_of, double *s_part, int *s_found, double *s_base) {
-    const int each = (n + kThreads - 1) / kThreads, from = min(n, static_cast<int>(threadIdx.x) * each), to = min(n, from + each);
-    double mine = 0.0;
-    for (int i = from; i < to; ++i) mine += weight_of(i);
-    double total;
-    const double start = before(mine, total, s_part), goal = goal_of(total);
-    if (threadIdx.x == 0) {
-        s_found[0] = 0x7fffffff;  // the first thread whose range passes the goal
-        s_found[1] = -1;          // the last thread with a weight
-        s_found[2] = -1;
-    }
-    __syncthreads();
-    if (mine > 0.0) {
-        if (start + mine > goal) atomicMin(&s_found[0], static_cast<int>(threadIdx.x));
-        atomicMax(&s_found[1], static_cast<int>(threadIdx.x));
-    }
-    __syncthreads();
-    const int who = s_found[0] != 0x7fffffff ? s_found[0] : s_found[1];
-    if (who == static_cast<int>(threadIdx.x)) {
-        double run = start;
-        for (int i = from; i < to; ++i) {
-            const double w = weight_of(i);
-            if (w > 0.0) {
-                s_found[2] = i;
-                *s_base = run;
-                if (run + w > goal) break;
-            }
-            run += w;
-        }
-    }
-    __syncthreads();
-    return Pick{s_found[2], *s_base};
-}
-
+template <int N>
 struct Shared {
-    double part[kWaves], base;
+    double steps[32], part[N / 64], base;
     int found[3];
 };
 
-// A workgroup a sequence.
-__global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
+// A draw by N threads: from the slices of a row, then from the tokens of a slice.  Thread t has the weights w (>= 0) of the
+// items t U .. t U + U - 1 (of a slice each one item, in w[0]).  The first item at which the running sum is above goal(total); where
+// rounding leaves none, the last one with a weight; -1 where there is no weight at all.  base: the running sum before it.
+// (A thread's sum and its walk add the same numbers from another start, so a goal can lie beyond the walk's end by a
+// rounding: then the last item with a weight.)
+struct Pick {
+    int at;
+    double base, total;
+};
+template <int N, int U, class Goal>
+__device__ __forceinline__ Pick draw(const double (&w)[U], int each, Goal goal_of, Shared<N> &sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    double mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < U; ++e) mine += w[e];
+    double run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(run, o, 64);
+        if (lane >= o) run += up;
+    }
+    __syncthreads();  // (sh's readers of before are done)
+    if (lane == 63) sh.part[wave] = run;
+    if (tid == 0) {
+        sh.found[0] = 0x7fffffff;  // the first thread whose items pass the goal
+        sh.found[1] = -1;          // the last thread with a weight
+        sh.found[2] = -1;
+    }
+    __syncthreads();
+    double start = 0.0, total = 0.0;
+#pragma unroll
+    for (int v = 0; v < N / 64; ++v) {
+        if (v < wave) start += sh.part[v];
+        total += sh.part[v];
+    }
+    start += run - mine;
+    const double goal = goal_of(total);
+    const uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && start + mine > goal);
+    if (past && lane == static_cast<int>(__ffsll(static_cast<long long>(past))) - 1) atomicMin(&sh.found[0], tid);
+    if (some && lane == 63 - static_cast<int>(__clzll(static_cast<long long>(some)))) atomicMax(&sh.found[1], tid);
+    __syncthreads();
+    const int who = sh.found[0] != 0x7fffffff ? sh.found[0] : sh.found[1];
+    if (who == tid) {
+        run = start;
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+            if (w[e] > 0.0 && !done) {
+                sh.found[2] = tid * each + e;
+                sh.base = run;
+                done = run + w[e] > goal;
+            }
+            run += w[e];
+        }
+    }
+    __syncthreads();
+    return Pick{sh.found[2], sh.base, total};
+}
+
+// The whole draw of a row from given sums of its slices: slice_weight(k, all) and token_weights(first, i, n, all, w).  all: not
+// without what is taken out, where nothing else has a weight.
+template <int N, int U, class Slice, class Tokens>
+__device__ __forceinline__ int draw_row(const VerifyArgs &a, double u, Slice slice_weight, Tokens token_weights, Shared<N> &sh) {
+    int slice = -1;
+    double goal = 0.0;
+    bool all = false;
+#pragma unroll 1
+    for (;;) {  // (in one piece of code: instructions that are met once cost more time than the arithmetic)
+        double w[U];
+        if (slice < 0) {
+#pragma unroll
+            for (int e = 0; e < U; ++e) w[e] = 0.0;
+            if (static_cast<int>(threadIdx.x) < a.slices) w[0] = slice_weight(threadIdx.x, all);
+        } else {
+            token_weights(slice * a.slice, static_cast<int>(threadIdx.x) * U, min(a.slice, a.vocab - slice * a.slice), all, w);
+        }
+        const Pick k = draw<N, U>(w, slice < 0 ? 1 : U, [&](double total) { return slice < 0 ? u * total : goal; }, sh);
+        if (slice >= 0) return slice * a.slice + max(k.at, 0);
+        if (k.at < 0) {  // uniform
+            if (all) return 0;
+            all = true;
+            continue;
+        }
+        slice = k.at;
+        goal = u * k.total - k.base;
+    }
+}
+template <int U>
+__device__ __forceinline__ void logits_of(const float *p, int i, int n, float (&v)[U]) {
+#pragma unroll
+    for (int e = 0; e < U; ++e) v[e] = i + e < n ? p[i + e] : -INFINITY;
+#pragma unroll
+    for (int e = 0; e < U; ++e) v[e] = number(v[e]);
+}
+
+// A workgroup a sequence.  What does not wait for the statistics is requested first.
+template <int U, bool DRAFT>
+__global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArgs a) {
     __shared__ Stat s_row[2 * kMostDrafts + 1];
-    __shared__ Shared sh;
-    __shared__ int s_accepted;
+    __shared__ Shared<kDecideThreads> sh;
+    __shared__ int s_accepted, s_rejected;
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = drafts_of(a, seq), D = a.max_drafts;
-    const double heat = heat_of(a, seq);
-    const bool greedy = greedy_of(a, seq);
+    const float t = temperature_of(a, seq);
+    const bool greedy = !(t > 0.0f);
+    const double heat = heat_of(t);
+    int x = -1;
+    float u_x = 0.0f, l_p = -INFINITY, l_q = -INFINITY;
+    if (wave == 0 && lane < n) {  // a draft a lane
+        x = a.drafts[static_cast<size_t>(seq) * D + lane];
+        u_x = uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + lane]);
+        if (x >= 0 && x < a.vocab) {
+            l_p = number(target_row(a, seq, lane)[x]);
+            if (DRAFT) l_q = number(draft_row(a, seq, lane)[x]);
+        }
+    }
+    const double u = static_cast<double>(uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + D]));
+    if (tid < 32) sh.steps[tid] = step_of(tid);
+    __syncthreads();
     const Stat *stats = a.stats + static_cast<size_t>(seq) * (2 * D + 1) * a.slices;
-    const int rows = 2 * n + 1;  // the target's n + 1, then the drafts'
-    for (int r = wave; r < (a.draft ? rows : n + 1); r += kWaves) {
+    const int rows = DRAFT ? 2 * n + 1 : n + 1;  // the target's n + 1, then the drafts'
+#pragma unroll 1
+    for (int r = wave; r < rows; r += kDecideThreads / 64) {
         const Stat *of = stats + static_cast<size_t>(r <= n ? r : D + r - n) * a.slices;
         float top = -INFINITY;
         int at = 0;
-        for (int k = lane; k < a.slices; k += 64) better(top, at, of[k].top, of[k].at);
-        wave_best(top, at);
         double sum = 0.0;
-        if (!greedy) {
-            for (int k = lane; k < a.slices; k += 64) sum += of[k].sum * weight(of[k].top, top, heat);
+        if (greedy) {
+#pragma unroll 1
+            for (int k = lane; k < a.slices; k += 64) better(top, at, of[k].top, of[k].at);
+            wave_best(top, at);
+        } else {
+            const Stat mine = lane < a.slices ? of[lane] : Stat{0.0, -INFINITY, 0};  // (read once)
+            top = mine.top;
+#pragma unroll 1
+            for (int k = lane + 64; k < a.slices; k += 64) top = fmaxf(top, of[k].top);
+            top = wave_max_dpp(top);
+            Stat s = mine;
+#pragma unroll 1
+            for (int k = lane;;) {
+                sum += s.sum * weight(s.top, top, heat, sh.steps);
+                k += 64;
+                if (k >= a.slices) break;
+                s = of[k];
+            }
             sum = wave_sum_f64(sum);
         }
         if (lane == 0) s_row[r] = Stat{sum, top, at};
     }
     __syncthreads();
-    if (wave == 0) {  // a draft a lane
+    if (wave == 0) {
         const float inf = INFINITY;
         bool ok = false;
         double px = 0.0, log_px = 0.0;
-        int x = 0;
         if (lane < n) {
-            x = a.drafts[static_cast<size_t>(seq) * D + lane];
             const bool token = x >= 0 && x < a.vocab;
             const Stat p = s_row[lane];
             double qx = token ? 1.0 : 0.0;
             if (token && p.top > -inf) {
-                const float l = target_row(a, seq, lane)[x];
                 if (greedy) {
                     px = x == p.at ? 1.0 : 0.0;
                 } else {
-                    px = weight(l, p.top, heat) / p.sum;
-                    log_px = (l == p.top ? 0.0 : (static_cast<double>(l) - static_cast<double>(p.top)) * heat) - log(p.sum);
+                    px = weight(l_p, p.top, heat, sh.steps) / p.sum;
+                    if (a.logprobs) log_px = log_of(l_p, p.top, t) - log(p.sum);
                 }
             }
-            if (token && a.draft) {
+            if (DRAFT && token) {
                 const Stat q = s_row[n + 1 + lane];
-                qx = !(q.top > -inf) ? 0.0
-                     : greedy        ? (x == q.at ? 1.0 : 0.0)
-                                     : weight(draft_row(a, seq, lane)[x], q.top, heat) / q.sum;
+                qx = !(q.top > -inf) ? 0.0 : greedy ? (x == q.at ? 1.0 : 0.0) : weight(l_q, q.top, heat, sh.steps) / q.sum;
             }
-            ok = static_cast<double>(uniform_at(a.uniform + static_cast<size_t>(seq) * (D + 1) + lane)) * qx < px;
+            ok = static_cast<double>(u_x) * qx < px;
             if (a.rates) a.rates[static_cast<size_t>(seq) * D + lane] = static_cast<float>(qx > px ? px / qx : px > 0.0 ? 1.0 : 0.0);
         } else if (lane < D && a.rates) {
             a.rates[static_cast<size_t>(seq) * D + lane] = 0.0f;
@@ -277,66 +370,58 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
             a.tokens[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? x : -1;
             if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? static_cast<float>(log_px) : 0.0f;
         }
+        const int rejected = __shfl(x, m, 64);  // (-1 where all were accepted)
         if (lane == 0) {
             a.accepted[seq] = m;
             s_accepted = m;
+            s_rejected = rejected;
         }
     }
     __syncthreads();
     const int m = s_accepted;
     const Stat p = s_row[m];
-    const float *row = target_row(a, seq, m);
-    const int x = m < n ? a.drafts[static_cast<size_t>(seq) * D + m] : -1;  // rejected
-    const double u = static_cast<double>(uniform_at(a.uniform + static_cast<size_t>(seq) * (D + 1) + D));
-    Rest rest = {0.0, 0.0, heat, p.top, 0.0f, -1};
-    int token = p.at;  // (0 where the row has nothing)
     const bool some = p.top > -INFINITY;
-    if (some && !greedy) {
-        if (a.draft && m < n && s_row[n + 1 + m].top > -INFINITY) {
-            const Stat q = s_row[n + 1 + m];
-            rest = Rest{1.0 / p.sum, 1.0 / q.sum, heat, p.top, q.top, m};
-        } else {
-            // the target's own weights, without the rejected token of a draft by lookup
-            const Stat *of = stats + static_cast<size_t>(m) * a.slices;
-            const int out = a.draft ? -1 : x;
-            auto slice_sum = [&](int k) {
-                double w = of[k].sum * weight(of[k].top, p.top, heat);
-                if (out >= 0 && out < a.vocab && out / a.slice == k) w = fmax(w - weight(row[out], p.top, heat), 0.0);
-                return w;
-            };
-            double goal = 0.0;
-            Pick k = draw(a.slices, slice_sum, [&](double total) { return goal = u * total; }, sh.part, sh.found, &sh.base);
-            bool all = out < 0;
-            if (k.at < 0) {  // uniform: nothing but the rejected token has a weight
-                all = true;
-                k = draw(a.slices, [&](int i) { return of[i].sum * weight(of[i].top, p.top, heat); },
-                         [&](double total) { return goal = u * total; }, sh.part, sh.found, &sh.base);
-            }
-            const int v0 = k.at * a.slice, size = min(a.slice, a.vocab - v0);
-            const Pick v = draw(size, [&](int i) { return !all && v0 + i == out ? 0.0 : weight(row[v0 + i], p.top, heat); },
-                                [&](double) { return goal - k.base; }, sh.part, sh.found, &sh.base);
-            token = v0 + max(v.at, 0);
+    if (DRAFT) {
+        const bool rest = some && !greedy && m < n && s_row[n + 1 + m].top > -INFINITY;
+        if (tid == 0) {
+            const Stat q = s_row[rest ? n + 1 + m : m];
+            a.rests[seq] = Rest{1.0 / p.sum, 1.0 / q.sum, heat, p.top, q.top, rest ? m : -1};
         }
+        if (rest) return;  // uniform
+    }
+    const float *row = target_row(a, seq, m);
+    int token = p.at;  // (0 where the row has nothing)
+    if (some && !greedy) {
+        // the target's own weights, without the rejected token of a draft by lookup
+        const Stat *of = stats + static_cast<size_t>(m) * a.slices;
+        const int out = !DRAFT && m < n && s_rejected < a.vocab ? s_rejected : -1;
+        const double taken = out >= 0 ? weight(number(row[out]), p.top, heat, sh.steps) : 0.0;
+        token = draw_row<kDecideThreads, U>(a, u, [&](int k, bool all) {
+            const double w = of[k].sum * weight(of[k].top, p.top, heat, sh.steps);
+            return !all && out >= 0 && out / a.slice == k ? fmax(w - taken, 0.0) : w;
+        }, [&](int v0, int i, int size, bool all, double (&w)[U]) {
+            float l[U];
+            logits_of(row + v0, i, size, l);
+#pragma unroll
+            for (int e = 0; e < U; ++e) w[e] = !all && v0 + i + e == out ? 0.0 : weight(l[e], p.top, heat, sh.steps);
+        }, sh);
     }
     if (tid == 0) {
-        if (a.draft) a.rests[seq] = rest;
-        if (rest.row < 0) {
-            a.tokens[static_cast<size_t>(seq) * (D + 1) + m] = token;
-            if (a.logprobs) {
-                const double t = row[token] == p.top ? 0.0 : (static_cast<double>(row[token]) - static_cast<double>(p.top)) * heat;
-                a.logprobs[static_cast<size_t>(seq) * (D + 1) + m] = !some ? -INFINITY : greedy ? 0.0f : static_cast<float>(t - log(p.sum));
-            }
+        a.tokens[static_cast<size_t>(seq) * (D + 1) + m] = token;
+        if (a.logprobs) {
+            const float log_p = static_cast<float>(log_of(number(row[token]), p.top, t) - log(p.sum));
+            a.logprobs[static_cast<size_t>(seq) * (D + 1) + m] = !some ? -INFINITY : greedy ? 0.0f : log_p;
         }
     }
 }
 
-__device__ __forceinline__ double rest_weight(const Rest &r, float p, float q) {
-    return fmax(weight(p, r.top_p, r.heat) * r.inv_p - weight(q, r.top_q, r.heat) * r.inv_q, 0.0);
+__device__ __forceinline__ double rest_weight(const Rest &r, float p, float q, const double *steps) {
+    return fmax(weight(p, r.top_p, r.heat, steps) * r.inv_p - weight(q, r.top_q, r.heat, steps) * r.inv_q, 0.0);
 }
 
 template <int U>
 __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
-    __shared__ double s_sum[kWaves];
+    __shared__ double s_sum[kWaves], s_steps[32];
     const int slice = blockIdx.x % a.slices, seq = blockIdx.x / a.slices, tid = threadIdx.x;
     const Rest r = a.rests[seq];
     if (r.row < 0) return;  // uniform
@@ -345,61 +430,48 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
     f32x4v x[U], y[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int i = 4 * (u * kThreads + tid);
-        x[u] = y[u] = f32x4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i + 4 <= n) {
-            __builtin_memcpy(&x[u], __builtin_assume_aligned(p + i, 4), 16);
-            __builtin_memcpy(&y[u], __builtin_assume_aligned(q + i, 4), 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i + e < n) {
-                    x[u][e] = p[i + e];
-                    y[u][e] = q[i + e];
-                }
-        }
+        x[u] = logits_at(p, 4 * (u * kThreads + tid), n);
+        y[u] = logits_at(q, 4 * (u * kThreads + tid), n);
     }
+    if (tid < 32) s_steps[tid] = step_of(tid);
+    __syncthreads();
     double sum = 0.0;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += rest_weight(r, x[u][e], y[u][e]);
+        for (int e = 0; e < 4; ++e) sum += rest_weight(r, number(x[u][e]), number(y[u][e]), s_steps);
     sum = wave_sum_f64(sum);
     if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
     __syncthreads();
-    if (tid == 0) {
-        sum = 0.0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
-        a.rest_sums[static_cast<size_t>(seq) * a.slices + slice] = sum;
-    }
+    if (tid == 0) a.rest_sums[static_cast<size_t>(seq) * a.slices + slice] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
 }
 
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
-    __shared__ Shared sh;
+template <int U>  // tokens a thread
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a) {
+    __shared__ Shared<kDrawThreads> sh;
     const int seq = blockIdx.x, D = a.max_drafts;
     const Rest r = a.rests[seq];
     if (r.row < 0) return;  // uniform
+    if (threadIdx.x < 32) sh.steps[threadIdx.x] = step_of(threadIdx.x);
     const float *p = target_row(a, seq, r.row), *q = draft_row(a, seq, r.row);
     const double *sums = a.rest_sums + static_cast<size_t>(seq) * a.slices;
-    const double u = static_cast<double>(uniform_at(a.uniform + static_cast<size_t>(seq) * (D + 1) + D));
+    const double u = static_cast<double>(uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + D]));
+    const float t = temperature_of(a, seq);
     const Stat *of = a.stats + (static_cast<size_t>(seq) * (2 * D + 1) + r.row) * a.slices;
-    double goal = 0.0;
-    bool rest = true;
-    Pick k = draw(a.slices, [&](int i) { return sums[i]; }, [&](double total) { return goal = u * total; }, sh.part, sh.found, &sh.base);
-    if (k.at < 0) {  // uniform: p is nowhere above q
-        rest = false;
-        k = draw(a.slices, [&](int i) { return of[i].sum * weight(of[i].top, r.top_p, r.heat); },
-                 [&](double total) { return goal = u * total; }, sh.part, sh.found, &sh.base);
-    }
-    const int v0 = max(k.at, 0) * a.slice, size = min(a.slice, a.vocab - v0);
-    const Pick v = draw(size, [&](int i) { return rest ? rest_weight(r, p[v0 + i], q[v0 + i]) : weight(p[v0 + i], r.top_p, r.heat); },
-                        [&](double) { return goal - k.base; }, sh.part, sh.found, &sh.base);
+    __syncthreads();
+    // all: where p is nowhere above q
+    const int token = draw_row<kDrawThreads, U>(a, u, [&](int k, bool all) {
+        return all ? of[k].sum * weight(of[k].top, r.top_p, r.heat, sh.steps) : sums[k];
+    }, [&](int v0, int i, int size, bool all, double (&w)[U]) {
+        float x[U], y[U];
+        logits_of(p + v0, i, size, x);
+        logits_of(q + v0, i, size, y);
+#pragma unroll
+        for (int e = 0; e < U; ++e) w[e] = all ? weight(x[e], r.top_p, r.heat, sh.steps) : rest_weight(r, x[e], y[e], sh.steps);
+    }, sh);
     if (threadIdx.x == 0) {
-        const int token = v0 + max(v.at, 0);
         a.tokens[static_cast<size_t>(seq) * (D + 1) + r.row] = token;
-        const double t = p[token] == r.top_p ? 0.0 : (static_cast<double>(p[token]) - static_cast<double>(r.top_p)) * r.heat;
-        if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + r.row] = static_cast<float>(t + log(r.inv_p));
+        if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + r.row] = static_cast<float>(log_of(number(p[token]), r.top_p, t) + log(r.inv_p));
     }
 }
 
@@ -408,7 +480,7 @@ int slices_of(int vocab, int slice) { return (vocab + slice - 1) / slice; }
 // Runs per thread.
 int runs_of(int64_t rows, int vocab) {
     for (int u = 4; u > 1; u /= 2)
-        if (rows * slices_of(vocab, u * kMinSlice) >= 1024) return u;
+        if (slices_of(vocab, u / 2 * kMinSlice) > kDrawThreads || rows * slices_of(vocab, u * kMinSlice) >= 1024) return u;
     return 1;
 }
 struct Layout {
@@ -436,7 +508,7 @@ bool al4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 extern "C" {
 
 size_t qlin_verify_drafts_workspace_bytes(int n_seqs, int max_drafts, int vocab) {
-    if (n_seqs <= 0 || max_drafts < 0 || max_drafts > qlin::kMostDrafts || vocab <= 0 || vocab > 1 << 28) return 0;
+    if (n_seqs <= 0 || max_drafts < 0 || max_drafts > qlin::kMostDrafts || vocab <= 0 || vocab > qlin::kMostVocab) return 0;
     return qlin::layout_of(n_seqs, max_drafts, vocab).bytes;
 }
 
@@ -445,7 +517,7 @@ int qlin_launch_verify_drafts(const float *target, size_t target_stride, const f
                               int *tokens, int *accepted, float *logprobs, float *rates, int n_seqs, int max_drafts,
                               int vocab, void *workspace, size_t workspace_bytes) {
     if (n_seqs < 0 || max_drafts < 0 || vocab < 0) return QLIN_ERR_SHAPE;
-    if (vocab > (1 << 28) || max_drafts > qlin::kMostDrafts) return QLIN_ERR_LIMIT;
+    if (vocab > qlin::kMostVocab || max_drafts > qlin::kMostDrafts) return QLIN_ERR_LIMIT;
     if (n_seqs == 0) return QLIN_OK;
     if (vocab == 0) return QLIN_ERR_SHAPE;  // (there is no token to draw)
     if (target_stride < static_cast<size_t>(vocab) || (draft && max_drafts > 0 && draft_stride < static_cast<size_t>(vocab))) return QLIN_ERR_SHAPE;
@@ -468,19 +540,22 @@ int qlin_launch_verify_drafts(const float *target, size_t target_stride, const f
                                 reinterpret_cast<qlin::Stat *>(ws + l.stats), reinterpret_cast<double *>(ws + l.sums),
                                 reinterpret_cast<qlin::Rest *>(ws + l.rests)};
     const hipStream_t s = static_cast<hipStream_t>(qlin_get_stream());
-    auto go = [&](auto stats, auto rest) {
+    auto go = [&](auto stats, auto decide, auto decide_drafts, auto rest, auto draw) {
         hipLaunchKernelGGL(stats, dim3(static_cast<unsigned>(grid)), dim3(qlin::kThreads), 0, s, a);
-        hipLaunchKernelGGL(qlin::verify_decide_kernel, dim3(n_seqs), dim3(qlin::kThreads), 0, s, a);
-        if (draft) {
+        if (!draft) {
+            hipLaunchKernelGGL(decide, dim3(n_seqs), dim3(qlin::kDecideThreads), 0, s, a);
+        } else {
+            hipLaunchKernelGGL(decide_drafts, dim3(n_seqs), dim3(qlin::kDecideThreads), 0, s, a);
             hipLaunchKernelGGL(rest, dim3(static_cast<unsigned>(n_seqs) * l.slices), dim3(qlin::kThreads), 0, s, a);
-            hipLaunchKernelGGL(qlin::verify_draw_kernel, dim3(n_seqs), dim3(qlin::kThreads), 0, s, a);
+            hipLaunchKernelGGL(draw, dim3(n_seqs), dim3(qlin::kDrawThreads), 0, s, a);
         }
         return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
     };
+    using namespace qlin;
     switch (l.runs) {
-        case 4: return go(qlin::verify_stats_kernel<4>, qlin::verify_rest_kernel<4>);
-        case 2: return go(qlin::verify_stats_kernel<2>, qlin::verify_rest_kernel<2>);
-        default: return go(qlin::verify_stats_kernel<1>, qlin::verify_rest_kernel<1>);
+        case 4: return go(verify_stats_kernel<4>, verify_decide_kernel<4, false>, verify_decide_kernel<4, true>, verify_rest_kernel<4>, verify_draw_kernel<8>);
+        case 2: return go(verify_stats_kernel<2>, verify_decide_kernel<2, false>, verify_decide_kernel<2, true>, verify_rest_kernel<2>, verify_draw_kernel<4>);
+        default: return go(verify_stats_kernel<1>, verify_decide_kernel<1, false>, verify_decide_kernel<1, true>, verify_rest_kernel<1>, verify_draw_kernel<2>);
     }
 }
 

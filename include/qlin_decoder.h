@@ -229,7 +229,7 @@ typedef struct qlin_lora {
  * below 1; NaN: 0).  A logit that is NaN counts as -inf; tokens at +inf share a row's probability.  A row without any
  * logit above -inf accepts nothing; where y would come from it, y is 0 with logprob -inf.  A drafted token outside
  * [0, vocab) is not accepted (and by lookup takes nothing from p).
- * vocab <= 1 << 28 and max_drafts <= 63 (else QLIN_ERR_LIMIT).  Pointers 4-byte aligned, the workspace 16-byte
+ * vocab <= 1 << 21 and max_drafts <= 63 (else QLIN_ERR_LIMIT).  Pointers 4-byte aligned, the workspace 16-byte
  * (qlin_verify_drafts_workspace_bytes(...) bytes; rules as qlin_launch_lora_add's).
  */
 

@@ -100,7 +100,7 @@ def test_validation():
         return qlin.status("qlin_launch_verify_drafts", target, ts, draft, ds, drafts, n_drafts, temp, uni, tok, acc, logs, rates, n, d, vocab, ws, nws)
     assert run(n=-1) == SHAPE and run(d=-1) == SHAPE and run(vocab=-1) == SHAPE and run(vocab=0) == SHAPE
     assert run(ts=99) == SHAPE and run(ds=99) == SHAPE
-    assert run(d=64) == LIMIT and run(vocab=(1 << 28) + 1, ts=1 << 29, ds=1 << 29) == LIMIT
+    assert run(d=64) == LIMIT and run(vocab=(1 << 21) + 1, ts=1 << 29, ds=1 << 29) == LIMIT
     assert run(n=1 << 22, vocab=151936, ts=151936, ds=151936, nws=1 << 60) == LIMIT
     for name in ("target", "uni", "tok", "acc", "drafts", "ws"):
         assert run(**{name: 0}) == NULL, name
@@ -110,7 +110,7 @@ def test_validation():
     need = qlin.verify_drafts_workspace_bytes(2, 3, 100)
     assert need > 0 and run(nws=need - 1) == LIMIT
     assert run(n=0, target=0) == OK
-    for bad in ((0, 3, 100), (2, -1, 100), (2, 64, 100), (2, 3, 0), (2, 3, (1 << 28) + 1)):
+    for bad in ((0, 3, 100), (2, -1, 100), (2, 64, 100), (2, 3, 0), (2, 3, (1 << 21) + 1)):
         assert qlin.verify_drafts_workspace_bytes(*bad) == 0
 
 
@@ -196,7 +196,8 @@ def test_verify(vocab, n, d, with_draft):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,d,vocab,with_draft", [(1, 4, 151936, False), (24, 4, 151936, True), (150, 0, 102400, False), (40, 2, 60001, True)])
+@pytest.mark.parametrize("n,d,vocab,with_draft", [(1, 4, 151936, False), (24, 4, 151936, True), (150, 0, 102400, False), (40, 2, 60001, True),
+                                                (1, 1, 1 << 21, True), (2, 1, 600000, False)])
 def test_verify_large(n, d, vocab, with_draft):
     torch = _gpu()
     from gpu_util import banner
