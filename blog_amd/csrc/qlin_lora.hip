@@ -5,16 +5,24 @@
 //
 // Rows of one adapter stand in tiles, of 16 rows (up to 256 rows in all, where each workgroup of the first launch groups the
 // ids by itself) or of 64 (a launch of one workgroup before it).  Weights are the A operand of the matrix cores, rows of x and
-// z the B operand; a lane loads 8 consecutive values of both, so that nothing goes through LDS on the way in.
+// z the B operand.
 // 1. lora_down_kernel: z of a tile, up to 64 ranks and a slice of x: 4 waves take parts of the slice and meet in LDS.  Slices
 //    are stored apart and added up by the second launch, in order: no atomics.
 // 2. lora_up_kernel: a tile and a run of outputs, scale z in LDS.
-// Everything is multiplied on v_mfma_f32_16x16x4_f32: f32's products and sums, whatever the values are.
+//
+// Products are exact.  bf16 and f16 weights go to v_mfma_f32_16x16x32_bf16: an f16 weight is the sum of two bf16 values, and
+// 2^26 v of an f32 value v is the sum of three (8 bits each; with the factor, which leaves with the sum, all parts of any v are
+// normal numbers).  Where a |v| is 2^60 or more (or infinite) these would overflow, and what is left goes to
+// v_mfma_f32_16x16x4_f32, a uniform and rare branch; f32 weights go there always.  (All types there: 613 rows of 18944 to 3584
+// at rank 64 63.3 and 57.4 us in the two launches, where they now take 26.2 and 17.4.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "qlin.h"
 #include "qlin_decoder.h"
+#include "qlin_bf16x3.hpp"
 #include "qlin_device.hpp"
 #include "qlin_internal.hpp"
 
@@ -25,10 +33,10 @@ constexpr int kMostMats = 4;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFewRows = 256;   // grouped by each workgroup; with more, a launch groups them
 constexpr int kTile = 64;       // the most rows of a tile
+constexpr int kUpThreads = 512;  // of lora_up_kernel over tiles of 64 rows
+constexpr int kPart = 32;       // of a workgroup of lora_down_kernel
 constexpr int kRanks = 64;      // of a workgroup of lora_down_kernel
 constexpr int kMostAdapters = 1024;
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Rows that have one adapter (-1: none), in the workspace.
 struct Tile {
@@ -56,15 +64,37 @@ __device__ __forceinline__ int slot_of(const LoraArgs &a, int row) {
 }
 __device__ __forceinline__ int rank_of(const LoraArgs &a, int id) { return a.ranks ? min(max(a.ranks[id], 0), a.max_rank) : a.max_rank; }
 
-// 8 weights of a type (0 bf16, 1 f16, 2 f32) as loaded, and as f32 values
+// Loads and stores.  Eight lanes take a line of 128 bytes, a wave 8 rows, so that no line is met by two instructions: the second
+// would wait in the first level cache for the first one's miss, with all that comes after it.  (The lanes as the matrix cores
+// take them, row l % 16 and the values 8 (l / 16) .., 2011 rows of 4096 to 14336 at rank 64 took 19.5 and 78.6 us, with the cache
+// stalled for two thirds of it; four lanes to half a line 20.1 and 73.3.)  What is loaded changes lanes through LDS of the
+// wave's own, rows 144 bytes apart, so that 16 lanes with 16 bytes of 16 rows meet all banks.
+constexpr int kLine = 128, kRowBytes = kLine + 16;
+
+// what the wave has written to LDS is read by other lanes of it, or the other way round
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// rows 8 i + lane / 8, 16 bytes each lane
+template <int N, class V>
+__device__ __forceinline__ void put_rows(char *lds, const V (&v)[N], int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<V *>(lds + (8 * i + (lane >> 3)) * kRowBytes + 16 * (lane & 7)) = v[i];
+}
+
+constexpr float kUp = 0x1p26f, kDown = 0x1p-26f, kWide = 0x1p60f;
+
+// 8 weights of a type (0 bf16, 1 f16, 2 f32), and as f32 values
 template <int T>
 struct Weights {
+    static constexpr int kBytes = T == 2 ? 4 : 2, kValues = kLine / kBytes;  // of a line
     u32x4 v[T == 2 ? 2 : 1];
-    __device__ __forceinline__ void load(const void *p, size_t i, bool there) {
-        const u32x4 zero = {0u, 0u, 0u, 0u};
-        const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p) + i * (T == 2 ? 4 : 2));
+    // values 8 i .. of a row in LDS
+    __device__ __forceinline__ void get(const char *row, int i) {
 #pragma unroll
-        for (int h = 0; h < (T == 2 ? 2 : 1); ++h) v[h] = there ? q[h] : zero;
+        for (int h = 0; h < (T == 2 ? 2 : 1); ++h) v[h] = *reinterpret_cast<const u32x4 *>(row + 8 * kBytes * i + 16 * h);
     }
     __device__ __forceinline__ float at(int j) const {
         if constexpr (T == 2) {
@@ -75,33 +105,55 @@ struct Weights {
             else return f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xffffu);
         }
     }
-    // only the first n count
-    __device__ __forceinline__ void keep(int n) {
-#pragma unroll
-        for (int h = 0; h < (T == 2 ? 2 : 1); ++h)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                if constexpr (T == 2) {
-                    if (4 * h + d >= n) v[h][d] = 0u;
-                } else {
-                    if (2 * d >= n) v[h][d] = 0u;
-                    else if (2 * d + 1 >= n) v[h][d] &= 0xffffu;
-                }
-            }
-    }
 };
+// only the first n values of the 16 bytes at v count (no choice that would be a branch: a wait would come with it)
+template <int T>
+__device__ __forceinline__ void keep_weights(u32x4 &v, int n) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        if constexpr (T == 2) v[d] &= static_cast<uint32_t>((d - n) >> 31);
+        else v[d] &= (static_cast<uint32_t>((2 * d - n) >> 31) & 0xffffu) | (static_cast<uint32_t>((2 * d + 1 - n) >> 31) & 0xffff0000u);
+    }
+}
 
-struct Values {  // 8 values of x
-    f32x4 v[2];
-    __device__ __forceinline__ void load(const float *p, bool there) {
-        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        v[0] = v[1] = zero;
-        if (there) {
-            __builtin_memcpy(&v[0], __builtin_assume_aligned(p, 4), 16);
-            __builtin_memcpy(&v[1], __builtin_assume_aligned(p + 4, 4), 16);
+__device__ __forceinline__ f32x4 mfma_bf16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// The bf16 operands of 8 bf16 or f16 weights: the weights, or what their 8 leading bits are and the rest.
+template <int T>
+struct Operands {
+    u32x4 hi, lo;
+    __device__ __forceinline__ explicit Operands(const Weights<T> &w) {
+        if constexpr (T == 0) {
+            hi = w.v[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = w.at(2 * i), b = w.at(2 * i + 1);
+                hi[i] = bf16_tops(a, b);
+                lo[i] = bf16_tops(a - bf16_hi_val(__builtin_bit_cast(uint32_t, a)), b - bf16_hi_val(__builtin_bit_cast(uint32_t, b)));
+            }
         }
     }
+    // acc += weights times the three parts of 8 values; the large products first
+    __device__ __forceinline__ f32x4 times(const u32x4 &h, const u32x4 &m, const u32x4 &l, f32x4 acc) const {
+        acc = mfma_bf16(hi, h, acc);
+        acc = mfma_bf16(hi, m, acc);
+        if constexpr (T == 1) acc = mfma_bf16(lo, h, acc);
+        acc = mfma_bf16(hi, l, acc);
+        if constexpr (T == 1) {
+            acc = mfma_bf16(lo, m, acc);
+            acc = mfma_bf16(lo, l, acc);
+        }
+        return acc;
+    }
 };
+template <int T>
+__device__ __forceinline__ f32x4 mfma_f32(const Weights<T> &w, const f32x4 (&v)[2], f32x4 acc) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.at(e), v[e >> 2][e & 3], acc, 0, 0, 0);
+    return acc;
+}
 
 // The tile of number `tile` among up to 256 rows, a row a thread: tiles are numbered by their first rows, and a tile's rows are in
 // order, so that every workgroup finds the same.  Gives the number of tiles.
@@ -147,55 +199,74 @@ __device__ __forceinline__ int group_rows(const LoraArgs &a, int tile, Tile &t, 
 
 // More rows: one workgroup counts each adapter's rows, gives it its tiles and puts the rows into them.  (In what order does
 // not matter: a row's results do not depend on its tile.)
-constexpr int kGroupThreads = 1024;
+constexpr int kGroupThreads = 1024, kKept = 4;  // rows a thread whose places are kept in registers
 __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
-    __shared__ int s_count[kMostAdapters + 1], s_tile[kMostAdapters + 1], s_wave[kGroupThreads / 64], s_total;
-    const int tid = threadIdx.x, lane = tid & 63;
-    for (int i = tid; i <= kMostAdapters; i += kGroupThreads) s_count[i] = 0;
-    if (tid == 0) s_total = 0;
+    __shared__ int s_count[kMostAdapters + 1], s_tile[kMostAdapters + 1], s_wave[kGroupThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, kinds = a.n_adapters + 1;
+    int slot[kKept], place[kKept];
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) slot[i] = tid + i * kGroupThreads < a.rows ? slot_of(a, tid + i * kGroupThreads) : -1;
+    for (int i = tid; i < kinds; i += kGroupThreads) s_count[i] = 0;
     __syncthreads();
-    for (int r = tid; r < a.rows; r += kGroupThreads) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) place[i] = slot[i] >= 0 ? atomicAdd(&s_count[slot[i]], 1) : 0;
+    __syncthreads();  // (the kept rows' places are the first ones, those of the rest come after them all)
+    const int rest = tid + kKept * kGroupThreads;
+    for (int r = rest; r < a.rows; r += kGroupThreads) {
         const int id = slot_of(a, r);
         if (id >= 0) atomicAdd(&s_count[id], 1);
     }
     __syncthreads();
-    for (int base = 0; base <= a.n_adapters; base += kGroupThreads) {
-        const int id = base + tid;
-        const int n = id <= a.n_adapters ? (s_count[id] + kTile - 1) / kTile : 0;
-        int run = n;
+    // (kinds <= 1025: the last one, the rows without an adapter, is thread 1023's second)
+    const int count = tid < kinds ? s_count[tid] : 0, last = kinds > kGroupThreads ? s_count[kGroupThreads] : 0;
+    const int n = (count + kTile - 1) / kTile;
+    int run = n;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(run, o, 64);
-            if (lane >= o) run += up;
-        }
-        if (lane == 63) s_wave[tid >> 6] = run;
-        __syncthreads();
-        int start = s_total + run - n;
-        for (int w = 0; w < (tid >> 6); ++w) start += s_wave[w];
-        if (id <= a.n_adapters) s_tile[id] = start;
-        for (int t = 0; t < n; ++t) {
-            a.tiles[start + t].adapter = id == a.n_adapters ? -1 : id;
-            a.tiles[start + t].count = min(kTile, s_count[id] - t * kTile);
-        }
-        __syncthreads();
-        if (tid == kGroupThreads - 1) s_total = start + n;
-        if (id <= a.n_adapters) s_count[id] = 0;
-        __syncthreads();
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(run, o, 64);
+        if (lane >= o) run += up;
     }
-    for (int r = tid; r < a.rows; r += kGroupThreads) {
-        const int id = slot_of(a, r);
-        if (id < 0) continue;
-        const int at = atomicAdd(&s_count[id], 1);
-        a.tiles[s_tile[id] + at / kTile].rows[at % kTile] = r;
+    if (lane == 63) s_wave[tid >> 6] = run;
+    __syncthreads();
+    int start = run - n, total = 0;
+#pragma unroll
+    for (int w = 0; w < kGroupThreads / 64; ++w) {
+        const int v = s_wave[w];
+        if (w < (tid >> 6)) start += v;
+        total += v;
     }
-    if (tid == 0) *a.n_tiles = s_total;
+    auto head = [&](int id, int at, int rows) {
+        s_tile[id] = at;
+        for (int t = 0; t * kTile < rows; ++t) {
+            a.tiles[at + t].adapter = id == a.n_adapters ? -1 : id;
+            a.tiles[at + t].count = min(kTile, rows - t * kTile);
+        }
+    };
+    if (tid < kinds) head(tid, start, count);
+    if (last > 0 && tid == 0) head(kGroupThreads, total, last);
+    if (tid == 0) *a.n_tiles = total + (last + kTile - 1) / kTile;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+        if (slot[i] >= 0) a.tiles[s_tile[slot[i]] + place[i] / kTile].rows[place[i] % kTile] = tid + i * kGroupThreads;
+    if (a.rows > kKept * kGroupThreads) {  // uniform; the rest are counted again, downwards
+        for (int r = rest; r < a.rows; r += kGroupThreads) {
+            const int id = slot_of(a, r);
+            if (id < 0) continue;
+            const int at = atomicSub(&s_count[id], 1) - 1;
+            a.tiles[s_tile[id] + at / kTile].rows[at % kTile] = r;
+        }
+    }
 }
 
-// z of one tile, one projection, one group of ranks and one slice of x.  NT: tiles of 16 rows.
+// z of 16 NT rows of a tile from its row `first` on, one projection, one group of ranks and one slice of x.  lds: at least
+// kDownBytes<NT>() for the workgroup.
+template <int NT>
+constexpr int kDownBytes = kWaves * (kRanks / 16 * NT * 64 * 16 > 16 * NT * kRowBytes ? kRanks / 16 * NT * 64 * 16 : 16 * NT * kRowBytes);
 template <int T, int NT>
-__device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int mat, int group, int split, f32x4 *s_z) {
-    constexpr int RT = kRanks / 16;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int first, int mat, int group, int split, char *lds) {
+    constexpr int RT = kRanks / 16, K = Weights<T>::kValues, H = K / 32;  // a step: a line of weights, H lines of x
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int rank = rank_of(a, t.adapter) - group * kRanks;
     if (rank <= 0) return;  // uniform
     const int tiles = min((rank + 15) / 16, RT);
@@ -206,67 +277,154 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int mat, 
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = zero;
     // (rows past the tile's or the rank's end are others again; what comes of them is not stored)
-    const float *x[NT];
+    const float *x[2 * NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j] = a.x + t.rows[min(16 * j + n, t.count - 1)] * a.x_stride;
-    size_t w[RT];
+    for (int j = 0; j < 2 * NT; ++j) x[j] = a.x + t.rows[min(first + 8 * j + (lane >> 3), t.count - 1)] * a.x_stride;
+    const char *w[2 * RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-        w[i] = (static_cast<size_t>(t.adapter) * a.max_rank + group * kRanks + min(16 * i + n, rank - 1)) * a.in_dim;
-    const void *weights = a.mats[mat].a;
-    const int steps = (a.in_dim + 31) / 32, parts = a.splits * kWaves, part = split * kWaves + wave;
+    for (int i = 0; i < 2 * RT; ++i)
+        w[i] = static_cast<const char *>(a.mats[mat].a) +
+               (static_cast<size_t>(t.adapter) * a.max_rank + group * kRanks + min(8 * i + (lane >> 3), rank - 1)) * a.in_dim * Weights<T>::kBytes;
+    const int steps = (a.in_dim + K - 1) / K, parts = a.splits * kWaves, part = split * kWaves + wave;
     const int from = static_cast<int>(static_cast<int64_t>(steps) * part / parts), to = static_cast<int>(static_cast<int64_t>(steps) * (part + 1) / parts);
     struct Step {
-        Weights<T> w[RT];
-        Values x[NT];
+        u32x4 w[RT][2];
+        f32x4 x[H][2 * NT];
     };
+    // (past the end of x: its last values once more, as zeros)
     auto load = [&](Step &s, int at) {
-        const int k = 32 * at + 8 * g;
-        const bool there = at < to && k < a.in_dim;
+        const int kx = K * at + 4 * (lane & 7), kw = min(K * at + (16 / Weights<T>::kBytes) * (lane & 7), a.in_dim - 16 / Weights<T>::kBytes);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) s.x[j].load(x[j] + k, there);
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-            if (i < tiles) s.w[i].load(weights, w[i] + k, there);
-    };
-    auto multiply = [&](const Step &s) {
+            for (int j = 0; j < 2 * NT; ++j) __builtin_memcpy(&s.x[h][j], __builtin_assume_aligned(x[j] + min(kx + 32 * h, a.in_dim - 4), 4), 16);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
             if (i < tiles) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s.w[i].at(e), s.x[j].v[e >> 2][e & 3], acc[i][j], 0, 0, 0);
+                for (int h = 0; h < 2; ++h) s.w[i][h] = *reinterpret_cast<const u32x4 *>(w[2 * i + h] + kw * Weights<T>::kBytes);
             }
     };
-    constexpr int U = NT == 1 ? 4 : 2;  // steps in flight
-    Step s[U];
+    // A lane's operands: row n of 16, the values 8 g .. of 32.
+    char *mine = lds + wave * (16 * NT * kRowBytes);
+    const int n = lane & 15, g = lane >> 4;
+    auto multiply = [&](Step &s, int at, auto wide) {
+        if (K * at + K > a.in_dim) {  // uniform
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(s[u], from + u);
-    for (int at = from; at < to; at += U) {
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const Step now = s[u];
-            load(s[u], at + U + u);
-            multiply(now);
+                for (int j = 0; j < 2 * NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s.x[h][j][e] = K * at + 32 * h + 4 * (lane & 7) < a.in_dim ? s.x[h][j][e] : 0.0f;
+        }
+        f32x4 v[H][NT][2];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            wave_sync();
+            put_rows(mine, s.x[h], lane);
+            wave_sync();
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) v[h][j][i] = *reinterpret_cast<const f32x4 *>(mine + (16 * j + n) * kRowBytes + 32 * g + 16 * i);
+        }
+        if constexpr (decltype(wide)::value) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                if (i < tiles) {
+                    wave_sync();
+                    put_rows(mine, s.w[i], lane);
+                    wave_sync();
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        Weights<T> o;
+                        o.get(mine + n * kRowBytes, 4 * h + g);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[i][j] = mfma_f32(o, v[h][j], acc[i][j]);
+                    }
+                }
+            return true;
+        } else {
+            float top = 0.0f;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) top = max3_abs(v[h][j][e >> 2][e & 3], v[h][j][e >> 2][(e & 3) + 1], top);
+            if (__any(!(top < kWide))) return false;
+            u32x4 hi[H][NT], mid[H][NT], lo[H][NT];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) split3(v[h][j][0] * kUp, v[h][j][1] * kUp, hi[h][j], mid[h][j], lo[h][j]);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                if (i < tiles) {
+                    wave_sync();
+                    put_rows(mine, s.w[i], lane);
+                    wave_sync();
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        Weights<T> r;
+                        r.get(mine + n * kRowBytes, 4 * h + g);
+                        const Operands<T> o(r);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[i][j] = o.times(hi[h][j], mid[h][j], lo[h][j], acc[i][j]);
+                    }
+                }
+            return true;
+        }
+    };
+    Step s;
+    int at = from;
+    if (at < to) load(s, at);
+    if constexpr (T != 2) {
+        // (acc is 2^26 z)
+        bool fits = true;
+#pragma unroll 1
+        while (at < to) {
+            Step now = s;
+            if (at + 1 < to) load(s, at + 1);
+            fits = multiply(now, at, std::false_type());
+            if (!fits) break;  // uniform: a value that is too large
+            ++at;
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] *= kDown;
+#pragma unroll 1
+        for (; at < to; ++at) {
+            load(s, at);
+            multiply(s, at, std::true_type());
+        }
+    } else {
+#pragma unroll 1
+        for (; at < to; ++at) {
+            Step now = s;
+            if (at + 1 < to) load(s, at + 1);
+            multiply(now, at, std::true_type());
         }
     }
+    __syncthreads();  // (the waves' rows are read)
+    f32x4 *s_z = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
             if (i < tiles) s_z[((wave * RT + i) * NT + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    // a lane's 4 values are ranks 4 g .. 4 g + 3 of row n
+    // a lane takes ranks 4 (l % 4) .. of row l / 4
+    const int of = 16 * (lane & 3) + (lane >> 2);
 #pragma unroll
     for (int i = 0; i < RT * NT; i += kWaves) {
-        const int at = i + wave, rt = at / NT, j = at % NT;
+        const int tile = i + wave, rt = tile / NT, j = tile % NT;
         if (rt >= tiles) continue;
-        f32x4 sum = s_z[at * 64 + lane];
+        f32x4 sum = s_z[tile * 64 + of];
 #pragma unroll
-        for (int v = 1; v < kWaves; ++v) sum += s_z[(v * RT * NT + at) * 64 + lane];
-        const int row = 16 * j + n, k = group * kRanks + 16 * rt + 4 * g;
+        for (int v = 1; v < kWaves; ++v) sum += s_z[(v * RT * NT + tile) * 64 + of];
+        const int row = first + 16 * j + (lane >> 2), k = group * kRanks + 16 * rt + 4 * (lane & 3);
         if (row < t.count && k < a.max_rank)
             *reinterpret_cast<f32x4 *>(a.z + ((static_cast<size_t>(split) * a.n_mats + mat) * a.rows + t.rows[row]) * a.max_rank + k) = sum;
     }
@@ -274,10 +432,10 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int mat, 
 
 // FEW: at most 256 rows in tiles of 16, a workgroup for each tile that there can be; else the tiles that there are in turn.
 template <int T, bool FEW>
-__global__ __launch_bounds__(kThreads) void lora_down_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void lora_down_kernel(LoraArgs a) {
     __shared__ Tile t;
-    __shared__ __attribute__((aligned(16))) f32x4 s_z[kWaves * (kRanks / 16) * (FEW ? 1 : kTile / 16) * 64];
-    const int groups = (a.max_rank + kRanks - 1) / kRanks, units = a.n_mats * groups * a.splits;
+    __shared__ __attribute__((aligned(16))) char s_z[kDownBytes<FEW ? 1 : kPart / 16>];
+    const int groups = (a.max_rank + kRanks - 1) / kRanks, units = a.n_mats * groups * a.splits * (FEW ? 1 : kTile / kPart);
     if constexpr (FEW) {
         __shared__ __attribute__((aligned(16))) int s_ids[kFewRows];
         __shared__ int s_first[kWaves], s_chunk;
@@ -295,7 +453,7 @@ __global__ __launch_bounds__(kThreads) void lora_down_kernel(LoraArgs a) {
         }
         if (tile >= n || t.adapter < 0) return;  // uniform
         const int split = unit % a.splits, rest = unit / a.splits;
-        down<T, 1>(a, t, rest % a.n_mats, rest / a.n_mats, split, s_z);
+        down<T, 1>(a, t, 0, rest % a.n_mats, rest / a.n_mats, split, s_z);
     } else {
         const int total = *a.n_tiles * units;
         for (int item = blockIdx.x; item < total; item += gridDim.x) {
@@ -307,10 +465,10 @@ __global__ __launch_bounds__(kThreads) void lora_down_kernel(LoraArgs a) {
                 t.count = a.tiles[tile].count;
             }
             __syncthreads();
-            if (t.adapter < 0) continue;  // uniform
-            const int split = unit % a.splits, rest = unit / a.splits;
-            if (t.count <= 16) down<T, 1>(a, t, rest % a.n_mats, rest / a.n_mats, split, s_z);
-            else down<T, kTile / 16>(a, t, rest % a.n_mats, rest / a.n_mats, split, s_z);
+            const int split = unit % a.splits, part = unit / a.splits % (kTile / kPart) * kPart, rest = unit / a.splits / (kTile / kPart);
+            if (t.adapter < 0 || part >= t.count) continue;  // uniform
+            if (t.count - part <= 16) down<T, 1>(a, t, part, rest % a.n_mats, rest / a.n_mats, split, s_z);
+            else down<T, kPart / 16>(a, t, part, rest % a.n_mats, rest / a.n_mats, split, s_z);
         }
     }
 }
@@ -336,74 +494,154 @@ __device__ __forceinline__ void store_values(float *p, int i, int n, const f32x4
     }
 }
 
-// y of one tile and one run of outputs.  s_z: [16 NT][stride] scale z, 0 past the rank.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// scale z of a tile in LDS: the three bf16 parts of 2^26 of it (Z of bf16 and f16 weights), or f32 values; 0 past the rank.
+struct Staged {
+    int stride, part;  // bytes from a row to the next one, and from a part
+    bool wide;
+};
+
+// y of 16 NT rows of a tile from its row `from` on, 32 outputs at a time: a line of each row.
+// (Rows past the tile's end, ranks past the slot's and outputs past the last one are others again; what comes of them is not
+// stored.)
 template <int T, int NT>
-__device__ __forceinline__ void up(const LoraArgs &a, const Tile &t, int mat, int first, const float *s_z, int stride, int rank) {
-    const qlin_lora &m = a.mats[mat];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int last = min(first + a.chunk, m.out_dim);
-    const float *base[NT];
-    float *y[NT];
-    bool there[NT];
+struct Up {
+    static constexpr int K = Weights<T>::kValues, H = K / 32;  // a line of weights
+    const qlin_lora &m;
+    const float *base[2 * NT];
+    float *y[2 * NT];
+    bool there[2 * NT];
+    f32x4 was[2 * NT];
+    u32x4 ahead[4];  // the first line of weights of the next outputs
+    const char *b;
+    char *mine;
+    int lane, rank, max_rank;
+
+    __device__ __forceinline__ Up(const LoraArgs &a, const Tile &t, int mat, int from, int rank, char *mine)
+        : m(a.mats[mat]), mine(mine), lane(threadIdx.x & 63), rank(rank), max_rank(a.max_rank) {
+        b = static_cast<const char *>(m.b) + static_cast<size_t>(max(t.adapter, 0)) * m.out_dim * max_rank * Weights<T>::kBytes;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int row = t.rows[min(16 * j + n, t.count - 1)];
-        there[j] = 16 * j + n < t.count;
-        base[j] = m.base + row * m.base_stride;
-        y[j] = m.y + row * m.y_stride;
+        for (int j = 0; j < 2 * NT; ++j) {
+            const int at = from + 8 * j + (lane >> 3), row = t.rows[min(at, t.count - 1)];
+            there[j] = at < t.count;
+            base[j] = m.base + row * m.base_stride + 4 * (lane & 7);
+            y[j] = m.y + row * m.y_stride + 4 * (lane & 7);
+        }
     }
-    const size_t w = static_cast<size_t>(max(t.adapter, 0)) * m.out_dim;
-    const int chunks = (rank + 31) / 32;  // 0 without an adapter
-    // 32 outputs at a time, so that a row's 128 bytes are met together
-    for (int o = first + 32 * wave; o < last; o += 32 * kWaves) {
-        f32x4 acc[2][NT];
+    // Weights come before the base: loads arrive in order, and the products can go ahead of it.
+    __device__ __forceinline__ void load(int o) {
+        if (rank > 0) weights(ahead, o, 0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int j = 0; j < 2 * NT; ++j) {
+            if (o + 32 <= m.out_dim) __builtin_memcpy(&was[j], __builtin_assume_aligned(base[j] + o, 4), 16);  // uniform
+            else was[j] = values_at(base[j], o, m.out_dim - 4 * (lane & 7));
+        }
+    }
+    __device__ __forceinline__ void weights(u32x4 (&w)[4], int o, int c) const {
+        constexpr int each = 16 / Weights<T>::kBytes;
+        const int k = min(K * c + each * (lane & 7), max_rank - each);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[h][j] = values_at(base[j], o + 16 * h + 4 * g, there[j] ? last : 0);
-        f32x4 sum[2][NT];
+        for (int i = 0; i < 4; ++i)
+            w[i] = *reinterpret_cast<const u32x4 *>(b + (static_cast<size_t>(min(o + 8 * i + (lane >> 3), m.out_dim - 1)) * max_rank + k) * Weights<T>::kBytes);
+    }
+    template <bool WIDE>
+    __device__ __forceinline__ void multiply(f32x4 (&sum)[2][NT], u32x4 (&w)[4], int c, const Staged &z, const char *first) const {
+        constexpr int each = 16 / Weights<T>::kBytes;
+        if (K * c + K > rank) {  // uniform
+#pragma unroll
+            for (int i = 0; i < 4; ++i) keep_weights<T>(w[i], rank - K * c - each * (lane & 7));
+        }
+        wave_sync();
+        put_rows(mine, w, lane);
+        wave_sync();
+        const int n = lane & 15, g = lane >> 4;
+        first += n * z.stride;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            if (K * c + 32 * h >= rank) break;  // uniform
+            const int k = K * c + 32 * h + 8 * g;
+            Weights<T> r[2];
+            r[0].get(mine + n * kRowBytes, 4 * h + g);
+            r[1].get(mine + (16 + n) * kRowBytes, 4 * h + g);
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    f32x4 v[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) v[i] = *reinterpret_cast<const f32x4 *>(first + 16 * j * z.stride + 4 * k + 16 * i);
+                    sum[0][j] = mfma_f32(r[0], v, sum[0][j]);
+                    sum[1][j] = mfma_f32(r[1], v, sum[1][j]);
+                }
+            } else {
+                const Operands<T> b0(r[0]), b1(r[1]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    u32x4 v[3];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) v[i] = *reinterpret_cast<const u32x4 *>(first + 16 * j * z.stride + 2 * k + i * z.part);
+                    sum[0][j] = b0.times(v[0], v[1], v[2], sum[0][j]);
+                    sum[1][j] = b1.times(v[0], v[1], v[2], sum[1][j]);
+                }
+            }
+        }
+    }
+    // y of outputs o .. o + 31, whose loads are on their way; those of next (if < last) follow before anything waits for
+    // these.  z: the first row's.
+    template <bool WIDE>
+    __device__ __forceinline__ void add(int o, int next, int last, const Staged &z, const char *first) {
         const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 sum[2][NT];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < NT; ++j) sum[h][j] = zero;
-        for (int c = 0; c < chunks; ++c) {
-            const int k = 32 * c + 8 * g;
-            Weights<T> b[2];
+        f32x4 now[2 * NT];
+        u32x4 w[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                b[h].load(m.b, (w + min(o + 16 * h + n, m.out_dim - 1)) * a.max_rank + k, k < rank);
-                if (32 * c + 32 > rank) b[h].keep(rank - k);  // uniform
+        for (int j = 0; j < 2 * NT; ++j) now[j] = was[j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = ahead[i];
+        if (next < last) load(next);
+        if (rank > 0) multiply<WIDE>(sum, w, 0, z, first);
+#pragma unroll 1
+        for (int c = 1; K * c < rank; ++c) {
+            weights(w, o, c);
+            multiply<WIDE>(sum, w, c, z, first);
+        }
+        if (rank > 0) {
+            wave_sync();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    *reinterpret_cast<f32x4 *>(mine + (16 * j + (lane & 15)) * kRowBytes + 64 * h + 16 * (lane >> 4)) = sum[h][j];
+            wave_sync();
+#pragma unroll
+            for (int j = 0; j < 2 * NT; ++j) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(mine + (8 * j + (lane >> 3)) * kRowBytes + 16 * (lane & 7));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) now[j][e] = fmaf(v[e], WIDE ? 1.0f : kDown, now[j][e]);
             }
-            f32x4 z[NT][2];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const f32x4 *p = reinterpret_cast<const f32x4 *>(s_z + (16 * j + n) * stride + k);
-                z[j][0] = p[0];
-                z[j][1] = p[1];
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        sum[h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[h].at(e), z[j][e >> 2][e & 3], sum[h][j], 0, 0, 0);
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                store_values(y[j], o + 16 * h + 4 * g, there[j] ? last : 0, chunks ? acc[h][j] + sum[h][j] : acc[h][j]);
+        for (int j = 0; j < 2 * NT; ++j)
+            if (there[j]) {
+                if (o + 32 <= m.out_dim) __builtin_memcpy(__builtin_assume_aligned(y[j] + o, 4), &now[j], 16);  // uniform
+                else store_values(y[j], o, m.out_dim - 4 * (lane & 7), now[j]);
+            }
     }
-}
+};
+constexpr int kUpBytes = 32 * kRowBytes;  // of a wave
 
 template <int T, bool FEW>
-__global__ __launch_bounds__(kThreads) void lora_up_kernel(LoraArgs a) {
-    constexpr int M = FEW ? 16 : kTile;
-    extern __shared__ __attribute__((aligned(16))) float s_z[];  // [M][stride]
+__global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel(LoraArgs a) {
+    constexpr int M = FEW ? 16 : kTile, N = FEW ? kThreads : kUpThreads;
+    extern __shared__ __attribute__((aligned(16))) char s_z[];  // the waves' own rows, then z
     __shared__ Tile t;
-    const int stride = (a.max_rank + 31) / 32 * 32 + 4;  // (rows 4 banks apart)
+    __shared__ int s_wide;
+    char *const s_parts = s_z + N / 64 * kUpBytes;
+    const int width = (a.max_rank + 31) / 32 * 32;
     const int runs = a.chunks[a.n_mats - 1], total = *a.n_tiles * runs;
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
         const int tile = item / runs;
@@ -415,27 +653,80 @@ __global__ __launch_bounds__(kThreads) void lora_up_kernel(LoraArgs a) {
         if (threadIdx.x == 0) {
             t.adapter = a.tiles[tile].adapter;
             t.count = a.tiles[tile].count;
+            s_wide = 0;
         }
         __syncthreads();
         if (t.adapter < 0 && a.mats[mat].y == a.mats[mat].base) continue;  // uniform
+        const int first = run * a.chunk, last = min(first + a.chunk, a.mats[mat].out_dim), wave = threadIdx.x >> 6;
+        // a wave takes 32 rows (16 of few): where there are more, waves go two by two
+        constexpr int NT = FEW ? 1 : 2;
+        const bool both = t.count > 16 * NT;
+        const int from = both ? 16 * NT * (wave & 1) : 0, step = 32 * (N / 64) / (both ? 2 : 1);
+        int o = first + 32 * (both ? wave >> 1 : wave);
         const int rank = t.adapter < 0 ? 0 : rank_of(a, t.adapter);
+        Up<T, NT> up(a, t, mat, from, rank, s_z + wave * kUpBytes);
+        if (o < last) up.load(o);  // (requested before z is staged)
         const int quads = (rank + 31) / 32 * 8;  // of a row
         const float scale = t.adapter >= 0 && a.scales ? a.scales[t.adapter] : 1.0f;
         const int rows = (t.count + 15) / 16 * 16;
-        for (int i = threadIdx.x; i < rows * quads; i += kThreads) {
-            const int r = i / quads, k = 4 * (i % quads);
+        const size_t split = static_cast<size_t>(a.n_mats) * a.rows * a.max_rank;
+        auto z_of = [&](int r, int k) {  // scale z, 4 values
             f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
             if (r < t.count && k < rank) {
                 const float *p = a.z + (static_cast<size_t>(mat) * a.rows + t.rows[r]) * a.max_rank + k;
-                for (int s = 0; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + static_cast<size_t>(s) * a.n_mats * a.rows * a.max_rank);
+                int s = 0;
+                for (; s + 4 <= a.splits; s += 4) {
+                    f32x4 v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4 *>(p + (s + i) * split);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum += v[i];
+                }
+                for (; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + s * split);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] = k + e < rank ? sum[e] * scale : 0.0f;
             }
-            *reinterpret_cast<f32x4 *>(s_z + r * stride + k) = sum;
+            return sum;
+        };
+        // (rows 16 bytes more than a multiple of 64 apart: 16 lanes meet 16 times 4 banks)
+        Staged z = {2 * width + 16, M * (2 * width + 16), T == 2};
+        if constexpr (T != 2) {
+            bool wide = false;
+            for (int i = threadIdx.x; i < rows * quads; i += N) {
+                const int r = i / quads, k = 4 * (i % quads);
+                const f32x4 v = z_of(r, k);
+                wide |= !(max3_abs(v[0], v[1], fmaxf(fabsf(v[2]), fabsf(v[3]))) < kWide);
+                uint2 h, m, l;
+                split3(v[0] * kUp, v[1] * kUp, h.x, m.x, l.x);
+                split3(v[2] * kUp, v[3] * kUp, h.y, m.y, l.y);
+                char *at = s_parts + r * z.stride + 2 * k;
+                *reinterpret_cast<uint2 *>(at) = h;
+                *reinterpret_cast<uint2 *>(at + z.part) = m;
+                *reinterpret_cast<uint2 *>(at + 2 * z.part) = l;
+            }
+            if (wide) s_wide = 1;
+            __syncthreads();
+            z.wide = s_wide != 0;
         }
-        __syncthreads();
-        if (FEW || t.count <= 16) up<T, 1>(a, t, mat, run * a.chunk, s_z, stride, rank);
-        else up<T, M / 16>(a, t, mat, run * a.chunk, s_z, stride, rank);
+        if (z.wide) {  // uniform
+            z.stride = 4 * width + 16;
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * quads; i += N) {
+                const int r = i / quads, k = 4 * (i % quads);
+                *reinterpret_cast<f32x4 *>(s_parts + r * z.stride + 4 * k) = z_of(r, k);
+            }
+            __syncthreads();
+        }
+        const char *rows_z = s_parts + from * z.stride;
+        if constexpr (T != 2) {
+            if (!z.wide) {  // uniform
+#pragma unroll 1
+                for (; o < last; o += step) up.template add<false>(o, o + step, last, z, rows_z);
+                continue;
+            }
+        }
+#pragma unroll 1
+        for (; o < last; o += step) up.template add<true>(o, o + step, last, z, rows_z);
     }
 }
 
@@ -454,10 +745,10 @@ Layout layout_of(int rows, int n_mats, int n_adapters, int max_rank, int in_dim)
     l.groups = (max_rank + kRanks - 1) / kRanks;
     // slices of x: as many as give about 512 workgroups, each wave 2 steps of 32 at least
     const int steps = (in_dim + 31) / 32;
-    int64_t tiles = few ? l.most_tiles : (rows + m - 1) / m;
+    int64_t tiles = few ? l.most_tiles : (rows + kPart - 1) / kPart;
     l.splits = static_cast<int>(512 / (tiles * n_mats * l.groups));
-    if (l.splits > steps / (2 * kWaves)) l.splits = steps / (2 * kWaves);
-    if (l.splits > 8) l.splits = 8;
+    if (l.splits > steps / (2 * kWaves)) l.splits = steps / (2 * kWaves);  // (steps of 32)
+    if (l.splits > 16) l.splits = 16;
     if (l.splits < 1) l.splits = 1;
     l.tiles = 16;
     l.z = l.tiles + sizeof(Tile) * l.most_tiles;
@@ -515,16 +806,22 @@ int qlin_launch_lora_add(const qlin_lora *mats, int n_mats, int weight_type, int
     a.n_tiles = reinterpret_cast<int *>(ws), a.tiles = reinterpret_cast<qlin::Tile *>(ws + l.tiles), a.z = reinterpret_cast<float *>(ws + l.z);
     a.n_mats = kept, a.n_adapters = n_adapters, a.max_rank = max_rank, a.in_dim = in_dim, a.rows = rows, a.splits = l.splits;
     const bool few = rows <= qlin::kFewRows;
-    a.chunk = few ? 256 : 1024;
+    // outputs of a workgroup: as many as leave 128 of them, each stages z again
+    int64_t outputs = 0;
+    for (int i = 0; i < kept; ++i) outputs += a.mats[i].out_dim;
+    const int64_t tiles = few ? l.most_tiles : (rows + qlin::kTile - 1) / qlin::kTile;
+    a.chunk = 4096;
+    while (a.chunk > 128 && tiles * outputs < static_cast<int64_t>(128) * a.chunk) a.chunk /= 2;
     int runs = 0;
     for (int i = 0; i < kept; ++i) a.chunks[i] = runs += (a.mats[i].out_dim + a.chunk - 1) / a.chunk;
-    const int64_t downs = static_cast<int64_t>(l.most_tiles) * kept * l.groups * l.splits, ups = static_cast<int64_t>(l.most_tiles) * runs;
+    const int64_t downs = static_cast<int64_t>(l.most_tiles) * kept * l.groups * l.splits * (few ? 1 : qlin::kTile / qlin::kPart), ups = static_cast<int64_t>(l.most_tiles) * runs;
     const hipStream_t s = static_cast<hipStream_t>(qlin_get_stream());
-    const size_t lds = sizeof(float) * (few ? 16 : qlin::kTile) * ((max_rank + 31) / 32 * 32 + 4);
+    const size_t width = (max_rank + 31) / 32 * 32, m = few ? 16 : qlin::kTile;
+    const size_t lds = (few ? qlin::kThreads : qlin::kUpThreads) / 64 * qlin::kUpBytes + (weight_type == 2 ? m * (4 * width + 16) : 3 * m * (2 * width + 16));
     auto go = [&](auto down, auto up) {
         if (!few) hipLaunchKernelGGL(qlin::lora_group_kernel, dim3(1), dim3(qlin::kGroupThreads), 0, s, a);
         hipLaunchKernelGGL(down, dim3(static_cast<unsigned>(few ? downs : downs < 2048 ? downs : 2048)), dim3(qlin::kThreads), 0, s, a);
-        hipLaunchKernelGGL(up, dim3(static_cast<unsigned>(ups < 2048 ? ups : 2048)), dim3(qlin::kThreads), lds, s, a);
+        hipLaunchKernelGGL(up, dim3(static_cast<unsigned>(ups < 2048 ? ups : 2048)), dim3(few ? qlin::kThreads : qlin::kUpThreads), lds, s, a);
         return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
     };
     using namespace qlin;

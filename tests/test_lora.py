@@ -224,6 +224,17 @@ def test_many_rows(rows, slots, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", [0, 1, 2], ids=TYPES)
+@pytest.mark.parametrize("rank", [72, 200, 256])
+def test_many_rows_of_large_ranks(rank, kind):
+    torch = _gpu()
+    from gpu_util import banner
+    banner(f"lora_add rows=300 rank={rank} {TYPES[kind]}")
+    _check(torch, _case(torch, rank, 300, 1000, [200, 31], 3, rank, kind))
+    _check(torch, _case(torch, rank, 300, 1000, [200, 31], 3, rank, kind, whole=True), in_place=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [0, 1, 2], ids=TYPES)
 def test_wide_ranges(kind):
     """Values of one row far apart, subnormal weights, and rows of infinities and NaN, which stay in their rows."""
     torch = _gpu()
