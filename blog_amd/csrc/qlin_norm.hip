@@ -7,7 +7,10 @@
 //
 // A row is taken by W waves, 4 consecutive values a lane and U such runs in registers, so that x is read once; 8 lanes hold
 // one Q8_1 block.  Rows that do not fit (U = 0) are read a second time, each value by the lane that wrote or read it before, so
-// that outputs may take the inputs' place.
+// that outputs may take the inputs' place.  Many rows are bound by HBM: 2011 rows of 4096 with their sum and blocks of 128 and
+// the blocks read back, 151 MB, take 35.8 us in a graph (4.2 TB/s; 4 waves of 4 runs 38.0, 16 of one 36.9), 42.1 with f32 results
+// through the caches: from 16 MB on they leave as streaming stores.  Few rows are bound by latency, and 16 waves take a row of
+// 3584 in 3.0 us, 4 waves in 4.9 (each with the read back).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -45,9 +48,12 @@ __device__ __forceinline__ f32x4v values_at(const float *p, int i, int n) {
     }
     return v;
 }
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+template <bool STREAM>  // (a choice while it runs would be one plain store to the compiler)
 __device__ __forceinline__ void store_values(float *p, int i, int n, const f32x4v &v) {
     if (i + 4 <= n) {
-        __builtin_memcpy(__builtin_assume_aligned(p + i, 4), &v, 16);
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<f32x4u *>(p + i));
+        else *reinterpret_cast<f32x4u *>(p + i) = v;
     } else {
         if (i < n) p[i] = v[0];
         if (i + 1 < n) p[i + 1] = v[1];
@@ -74,7 +80,7 @@ __device__ __forceinline__ double weight_of(uint2 w, int e, int type, int one_pl
     return one_plus ? static_cast<double>(v) + 1.0 : static_cast<double>(v);
 }
 
-template <int W, int U>
+template <int W, int U, bool STREAM>
 __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(NormArgs a) {
     constexpr int R = W < 4 ? 4 / W : 1, N = 64 * W;  // rows a workgroup, lanes a row
     __shared__ double red[W > 1 ? R * W : 1];
@@ -91,7 +97,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(Norm
         return s;
     };
     auto count = [&](int i, const f32x4v &s) {
-        if (sum) store_values(sum, i, a.hidden, s);
+        if (sum) store_values<STREAM>(sum, i, a.hidden, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ss += static_cast<double>(s[e]) * static_cast<double>(s[e]);
     };
@@ -122,7 +128,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(Norm
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             y[e] = i + e < a.hidden ? static_cast<float>(static_cast<double>(v[e]) * inv * weight_of(wv, e, a.norm_type, a.one_plus)) : 0.0f;
-        if (normed) store_values(normed, i, a.hidden, f32x4v{y[0], y[1], y[2], y[3]});
+        if (normed) store_values<STREAM>(normed, i, a.hidden, f32x4v{y[0], y[1], y[2], y[3]});
         if (a.q8) {
             const int b = i / 32, j = t & 7;
             if (a.mmq) {
@@ -146,6 +152,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(Norm
 }
 
 // 4 values a lane; a lane past the row's end has none.
+template <bool STREAM>
 __global__ __launch_bounds__(256) void dequantize_q8_1_kernel(const uint8_t *__restrict__ xq, float *__restrict__ x,
                                                               int in_dim, int m, int quads, int64_t total, int mmq) {
     const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
@@ -166,9 +173,12 @@ __global__ __launch_bounds__(256) void dequantize_q8_1_kernel(const uint8_t *__r
         f32x4v v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = d * static_cast<float>(static_cast<int8_t>(codes >> (8 * e)));
-        store_values(x + r * in_dim, i, in_dim, v);
+        store_values<STREAM>(x + r * in_dim, i, in_dim, v);
     }
 }
+
+// results of so many values are not kept in the caches
+bool streamed(int64_t values) { return values * 4 >= 16 << 20; }
 
 hipStream_t current_stream() { return static_cast<hipStream_t>(qlin_get_stream()); }
 bool al(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -176,7 +186,9 @@ bool al(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (
 template <int W, int U>
 void launch(const NormArgs &a) {
     constexpr int R = W < 4 ? 4 / W : 1;
-    hipLaunchKernelGGL((add_rms_norm_kernel<W, U>), dim3((a.rows + R - 1) / R), dim3(W < 4 ? 256 : 64 * W), 0, current_stream(), a);
+    const dim3 grid((a.rows + R - 1) / R), block(W < 4 ? 256 : 64 * W);
+    if (streamed(static_cast<int64_t>(a.rows) * a.hidden)) hipLaunchKernelGGL((add_rms_norm_kernel<W, U, true>), grid, block, 0, current_stream(), a);
+    else hipLaunchKernelGGL((add_rms_norm_kernel<W, U, false>), grid, block, 0, current_stream(), a);
 }
 
 }  // namespace
@@ -208,7 +220,8 @@ int qlin_launch_add_rms_norm(const float *x, size_t x_stride, const float *delta
     if (a.padded <= 256) qlin::launch<1, 1>(a);
     else if (a.padded <= 1024) qlin::launch<4, 1>(a);
     else if (a.padded <= 2048) qlin::launch<4, 2>(a);
-    else if (a.padded <= 4096) qlin::launch<4, 4>(a);
+    else if (a.padded <= 4096 && rows < 512) qlin::launch<16, 1>(a);
+    else if (a.padded <= 4096) qlin::launch<8, 2>(a);
     else if (a.padded <= 8192) qlin::launch<16, 2>(a);
     else if (a.padded <= 16384) qlin::launch<16, 4>(a);
     else qlin::launch<16, 0>(a);
@@ -224,8 +237,12 @@ int qlin_launch_dequantize_q8_1(const uint8_t *x_q8_1, float *x, int in_dim, int
     const int quads = (in_dim + 3) / 4;
     const int64_t total = static_cast<int64_t>(m) * quads;
     const int64_t groups = (total + 255) / 256;
-    hipLaunchKernelGGL(qlin::dequantize_q8_1_kernel, dim3(static_cast<unsigned>(groups < 8192 ? groups : 8192)), dim3(256), 0,
-                       qlin::current_stream(), x_q8_1, x, in_dim, m, quads, total, mmq != 0);
+    const dim3 grid(static_cast<unsigned>(groups < 8192 ? groups : 8192));
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, qlin::current_stream(), x_q8_1, x, in_dim, m, quads, total, mmq != 0);
+    };
+    if (qlin::streamed(total * 4)) go(qlin::dequantize_q8_1_kernel<true>);
+    else go(qlin::dequantize_q8_1_kernel<false>);
     return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
 }
 
