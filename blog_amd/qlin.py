@@ -532,8 +532,14 @@ def logits_controls(logits, out, rows, vocab, *, history=None, history_lens=None
 # These take tensors of one GPU (the current device's, whose stream set_stream was given) and refuse others, and types,
 # shapes and layouts that would be read as something else.
 
-def _rows_of(t, rows, width, name, device):
-    """The address and the row stride of t: f32 [>= rows, >= width] whose rows are contiguous."""
+# (A launch takes about 2 us of the host, looking at a tensor from all sides as much again: the usual layouts are told by few
+# looks, and what one function would do for all tensors is written out where there are many.)
+
+def _rows_of(t, shape, name, device):
+    """The address and the row stride of t: f32 of at least shape whose rows are contiguous."""
+    if t.shape == shape and t.is_contiguous() and t.dtype is _F32 and t.get_device() == device:
+        return t.data_ptr(), shape[1]
+    rows, width = shape
     n, have = t.shape
     row, one = t.stride()
     if t.dtype is not _F32 or n < rows or have < width or one != 1 and width > 1 or t.get_device() != device:
@@ -543,9 +549,7 @@ def _rows_of(t, rows, width, name, device):
 
 
 def _values_of(t, n, dtype, name, device):
-    """The address of at least n contiguous values of dtype (None: none)."""
-    if t is None:
-        return 0
+    """The address of at least n contiguous values of dtype."""
     if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != device:
         raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device}, not {n} contiguous values of {dtype} on device {device}")
     return t.data_ptr()
@@ -566,15 +570,15 @@ def q8_1_bytes(in_dim, rows, mmq=False):
 def add_rms_norm(x, delta, sum, weight, norm_type, eps, one_plus, *, normed=None, q8_1=None, mmq=False, raw_sum=False):
     """sum = x + delta, and its RMSNorm into normed [rows, hidden], into Q8_1 blocks (uint8), or both.  x, delta, sum and normed
     are float32 [rows, hidden] with contiguous rows; delta and sum may be None, sum may be x or delta."""
-    library, device = _lib or lib(), _device_of(x, "x")
-    rows, hidden = x.shape
-    p_x, n_x = _rows_of(x, rows, hidden, "x", device)
-    p_delta, n_delta = (0, 0) if delta is None else _rows_of(delta, rows, hidden, "delta", device)
-    p_sum, n_sum = (0, 0) if sum is None else _rows_of(sum, rows, hidden, "sum", device)
-    p_normed, n_normed = (0, 0) if normed is None else _rows_of(normed, rows, hidden, "normed", device)
+    library, device, shape = _lib or lib(), _device_of(x, "x"), x.shape
+    rows, hidden = shape
+    p_x, n_x = _rows_of(x, shape, "x", device)
+    p_delta, n_delta = (0, 0) if delta is None else _rows_of(delta, shape, "delta", device)
+    p_sum, n_sum = (0, 0) if sum is None else _rows_of(sum, shape, "sum", device)
+    p_normed, n_normed = (0, 0) if normed is None else _rows_of(normed, shape, "normed", device)
     if weight.element_size() != 2 or weight.numel() < hidden or not weight.is_contiguous() or weight.get_device() != device:
         raise ValueError(f"weight: {tuple(weight.shape)} of {weight.dtype} on {weight.device}, not {hidden} contiguous values of 16 bits")
-    p_q8 = _values_of(q8_1, q8_1_bytes(hidden, rows, mmq), _U8, "q8_1", device)
+    p_q8 = 0 if q8_1 is None else _values_of(q8_1, q8_1_bytes(hidden, rows, mmq), _U8, "q8_1", device)
     rc = library.qlin_launch_add_rms_norm(p_x, n_x, p_delta, n_delta, p_sum, n_sum, weight.data_ptr(), norm_type, eps, int(one_plus),
                                           p_normed, n_normed, p_q8, int(mmq), int(raw_sum), rows, hidden)
     if rc != 0:
@@ -603,15 +607,17 @@ class Lora:
             raise ValueError("a and b are contiguous")
         self.a, self.b, self.type = a, b, _LORA_TYPES[a.dtype]
         self.n_adapters, self.max_rank, self.in_dim, self.out_dim = n, rank, n_in, out
+        self.like, self.device = (self.type, n, rank, n_in), a.get_device()
+        self.addresses = a.data_ptr(), b.data_ptr()
 
 
 def lora_workspace_bytes(rows, n_mats, n_adapters, max_rank, in_dim):
     return int(lib().qlin_lora_workspace_bytes(rows, n_mats, n_adapters, max_rank, in_dim))
 
 
-# struct qlin_lora, packed (filling ctypes structures takes several times as long)
-_LORA = struct.Struct("@4PNNi4x")
-assert _LORA.size == C.sizeof(LoraArgs)
+# structs qlin_lora, packed (filling ctypes structures takes several times as long)
+_LORAS = [struct.Struct("@" + "4PNNi4x" * n) for n in range(5)]
+assert _LORAS[1].size == C.sizeof(LoraArgs) and _LORAS[3].size == 3 * C.sizeof(LoraArgs)
 
 
 def lora_add(x, adapter_ids, mats, *, ranks=None, scales=None, workspace=None):
@@ -622,23 +628,26 @@ def lora_add(x, adapter_ids, mats, *, ranks=None, scales=None, workspace=None):
     library, device = _lib or lib(), _device_of(x, "x")
     if not 1 <= len(mats) <= 4:
         raise ValueError(f"{len(mats)} projections: 1 to 4")
-    first, rows = mats[0][0], x.shape[0]
-    p_x, n_x = _rows_of(x, rows, first.in_dim, "x", device)
-    packed = b""
+    like, rows = mats[0][0].like, x.shape[0]
+    kind, slots, rank, width = like
+    p_x, n_x = _rows_of(x, (rows, width), "x", device)
+    each = []
     for w, base, y in mats:
-        if w.type != first.type or w.n_adapters != first.n_adapters or w.max_rank != first.max_rank or w.in_dim != first.in_dim:
+        if w.like != like:
             raise ValueError("the projections' adapters have one type, number of slots, rank and input")
-        if w.a.get_device() != device:
+        if w.device != device:
             raise ValueError(f"adapters on {w.a.device}, x on device {device}")
-        p_base, n_base = _rows_of(base, rows, w.out_dim, "base", device)
-        p_y, n_y = (p_base, n_base) if y is base else _rows_of(y, rows, w.out_dim, "y", device)
-        packed += _LORA.pack(w.a.data_ptr(), w.b.data_ptr(), p_base, p_y, n_base, n_y, w.out_dim)
-    p_ws = _values_of(workspace, 0, _U8, "workspace", device)
-    rc = library.qlin_launch_lora_add(packed, len(mats), first.type, first.n_adapters, first.max_rank, first.in_dim,
-                                      _values_of(ranks, first.n_adapters, _I32, "ranks", device),
-                                      _values_of(scales, first.n_adapters, _F32, "scales", device), p_x, n_x,
-                                      _values_of(adapter_ids, rows, _I32, "adapter_ids", device), rows, p_ws,
-                                      0 if workspace is None else workspace.numel())
+        shape = rows, w.out_dim
+        p_base, n_base = _rows_of(base, shape, "base", device)
+        p_y, n_y = (p_base, n_base) if y is base else _rows_of(y, shape, "y", device)
+        each += (*w.addresses, p_base, p_y, n_base, n_y, w.out_dim)
+    p_ws = ws_bytes = 0
+    if workspace is not None:
+        p_ws, ws_bytes = _values_of(workspace, 0, _U8, "workspace", device), workspace.numel()
+    rc = library.qlin_launch_lora_add(_LORAS[len(mats)].pack(*each), len(mats), kind, slots, rank, width,
+                                      0 if ranks is None else _values_of(ranks, slots, _I32, "ranks", device),
+                                      0 if scales is None else _values_of(scales, slots, _F32, "scales", device), p_x, n_x,
+                                      _values_of(adapter_ids, rows, _I32, "adapter_ids", device), rows, p_ws, ws_bytes)
     if rc != 0:
         raise QlinError("qlin_launch_lora_add", rc)
 
@@ -660,11 +669,12 @@ def moe_route(how, logits, ids, weights):
     weights float32, both [tokens, k] and contiguous."""
     library, device = _lib or lib(), _device_of(logits, "logits")
     tokens, n_experts = logits.shape
-    p_logits, stride = _rows_of(logits, tokens, n_experts, "logits", device)
-    k = ids.shape[1]
+    p_logits, stride = _rows_of(logits, logits.shape, "logits", device)
+    shape = ids.shape
+    k = shape[1]
     if how.bias is not None and (how.bias.numel() < n_experts or how.bias.get_device() != device):
         raise ValueError(f"a bias of {how.bias.numel()} values on {how.bias.device} for {n_experts} experts on device {device}")
-    if ids.shape[0] < tokens or tuple(weights.shape) != tuple(ids.shape):
+    if shape[0] < tokens or weights.shape != shape:
         raise ValueError(f"ids {tuple(ids.shape)} and weights {tuple(weights.shape)} for {tokens} tokens")
     rc = library.qlin_launch_moe_route(how.address, p_logits, stride, _values_of(ids, 0, _I32, "ids", device),
                                        _values_of(weights, 0, _F32, "weights", device), tokens, n_experts, k)
@@ -676,14 +686,17 @@ def verify_drafts_workspace_bytes(n_seqs, max_drafts, vocab):
     return int(lib().qlin_verify_drafts_workspace_bytes(n_seqs, max_drafts, vocab))
 
 
-def _logits_of(t, n, rows, name, device):
-    """The address, the row stride and the vocabulary of [n, rows, vocab] logits that lie row after row."""
-    a, b, vocab = t.shape
-    seq, row, one = t.stride()
-    if t.dtype is not _F32 or a != n or b != rows or t.get_device() != device or one != 1 and vocab > 1 or a > 1 and b > 0 and seq != b * row:
-        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype}, strides {t.stride()}, on {t.device}, not float32 [{n}, {rows}, vocab] "
-                         f"row after row on device {device}")
-    return t.data_ptr(), row if b > 1 else seq if a > 1 else max(row, vocab), vocab
+def _logits_of(t, shape, name, device):
+    """The address and the row stride of [n, rows, vocab] logits that lie row after row."""
+    if t.shape == shape and t.is_contiguous() and t.dtype is _F32 and t.get_device() == device:
+        return t.data_ptr(), shape[2]
+    n, rows, vocab = shape
+    seq, row, one = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.dtype is not _F32 or tuple(t.shape) != tuple(shape) or t.get_device() != device or one != 1 and vocab > 1 or (
+            n > 1 and rows > 0 and seq != rows * row):
+        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype}, strides {t.stride()}, on {t.device}, not float32 [{n}, {rows}, "
+                         f"{vocab}] row after row on device {device}")
+    return t.data_ptr(), row if rows > 1 else seq if n > 1 else max(row, vocab)
 
 
 def verify_drafts(target, drafts, uniform, tokens, accepted, *, draft_logits=None, n_drafts=None, temperature=None, logprobs=None,
@@ -694,21 +707,21 @@ def verify_drafts(target, drafts, uniform, tokens, accepted, *, draft_logits=Non
     temperature float32 [n_seqs] or None.  Into tokens int32 [n_seqs, max_drafts + 1], accepted int32 [n_seqs], and, where given,
     logprobs float32 [n_seqs, max_drafts + 1] and rates float32 [n_seqs, max_drafts].  workspace: a uint8 tensor of
     verify_drafts_workspace_bytes(...)."""
-    library, device = _lib or lib(), _device_of(target, "target")
-    n, rows, vocab = target.shape
+    library, device, shape = _lib or lib(), _device_of(target, "target"), target.shape
+    n, rows, vocab = shape
     d = rows - 1
-    p_target, target_stride, _ = _logits_of(target, n, rows, "target", device)
-    p_draft = draft_stride = 0
+    p_target, target_stride = _logits_of(target, shape, "target", device)
+    p_draft = draft_stride = p_ws = ws_bytes = 0
     if draft_logits is not None:
-        p_draft, draft_stride, width = _logits_of(draft_logits, n, d, "draft_logits", device)
-        if width != vocab:
-            raise ValueError(f"draft logits of {width} tokens, the target's of {vocab}")
+        p_draft, draft_stride = _logits_of(draft_logits, (n, d, vocab), "draft_logits", device)
+    if workspace is not None:
+        p_ws, ws_bytes = _values_of(workspace, 0, _U8, "workspace", device), workspace.numel()
     rc = library.qlin_launch_verify_drafts(
-        p_target, target_stride, p_draft if d else 0, draft_stride, _values_of(drafts, n * d, _I32, "drafts", device),
-        _values_of(n_drafts, n, _I32, "n_drafts", device), _values_of(temperature, n, _F32, "temperature", device),
+        p_target, target_stride, p_draft if d else 0, draft_stride, 0 if drafts is None else _values_of(drafts, n * d, _I32, "drafts", device),
+        0 if n_drafts is None else _values_of(n_drafts, n, _I32, "n_drafts", device),
+        0 if temperature is None else _values_of(temperature, n, _F32, "temperature", device),
         _values_of(uniform, n * rows, _F32, "uniform", device), _values_of(tokens, n * rows, _I32, "tokens", device),
-        _values_of(accepted, n, _I32, "accepted", device), _values_of(logprobs, n * rows, _F32, "logprobs", device),
-        _values_of(rates, n * d, _F32, "rates", device), n, d, vocab, _values_of(workspace, 0, _U8, "workspace", device),
-        0 if workspace is None else workspace.numel())
+        _values_of(accepted, n, _I32, "accepted", device), 0 if logprobs is None else _values_of(logprobs, n * rows, _F32, "logprobs", device),
+        0 if rates is None else _values_of(rates, n * d, _F32, "rates", device), n, d, vocab, p_ws, ws_bytes)
     if rc != 0:
         raise QlinError("qlin_launch_verify_drafts", rc)
