@@ -15,7 +15,8 @@ torch provides the device memory and the streams.
 
 Two variations of the architecture: ``qk_norm`` norms every query and key head before the rotation (weights ``q_norm``
 and ``k_norm`` [head_dim] in each layer), and ``kv8`` keeps keys and values in the 8-bit cache of blocks.  With
-``set_controls`` the pick goes by the logits after penalties for repeated tokens, biases and a mask.
+``set_controls`` the pick goes by the logits after penalties for repeated tokens, biases and a mask; with ``set_adapters``
+low-rank adapters stand beside the linears; ``step_drafts`` checks drafted tokens against the model's probabilities in one pass.
 """
 from __future__ import annotations
 
@@ -129,6 +130,7 @@ class Qwen2Decoder:
         self.zero = torch.zeros(1, dtype=i32, device=dev)
         self.L = qlin.lib()
         self.controls, self.captured = None, []
+        self.adapters = None
         self.stream, self.controlled_on = None, set()  # the calls' stream, and those whose picks read the controls
         if cfg.qk_norm or cfg.kv8:
             qlin.set_stream(torch.cuda.current_stream())
@@ -176,6 +178,50 @@ class Qwen2Decoder:
                 bias_ids=torch.tensor([list(bias)], dtype=torch.int32, device="cuda"),
                 bias_values=torch.tensor([list(bias.values())], dtype=torch.float32, device="cuda"))
 
+    LINEARS = (("wq", "wk", "wv"), ("wo",), ("wd",))  # that can have adapters, as they read the same input
+
+    def set_adapters(self, layers, slot, ranks=None, scales=None) -> None:
+        """From the next call on: low-rank adapters beside the linears.  layers: for each layer a dict with a qlin.Lora for any of
+        wq, wk, wv (of one type, number of slots and rank), wo and wd; slot: the one to use (a number, rewritten by another
+        call, or an int32 tensor [1] on the device, which a graph reads at each replay; < 0: none).  ranks int32 and scales
+        float32 of the slots, or None.  None instead of layers: no adapters."""
+        torch, c = self.torch, self.cfg
+        if self.adapters is not None:
+            torch.cuda.synchronize()  # (steps on other streams may still read those before)
+        if layers is None:
+            self.adapters = None
+            return
+        if len(layers) != c.layers:
+            raise ValueError(f"adapters for {len(layers)} layers of {c.layers}")
+        dims = {"wq": (c.hidden, c.q_dim), "wk": (c.hidden, c.kv_dim), "wv": (c.hidden, c.kv_dim), "wo": (c.q_dim, c.hidden),
+                "wd": (c.ffn, c.hidden)}
+        need = 16
+        for L in layers:
+            for name, w in L.items():
+                if name not in dims or (w.in_dim, w.out_dim) != dims[name]:
+                    raise ValueError(f"an adapter {name} of {w.in_dim} to {w.out_dim}")
+            for names in self.LINEARS:
+                there = [L[n] for n in names if n in L]
+                if any(w.like != there[0].like for w in there):
+                    raise ValueError("the adapters of wq, wk and wv have one type, number of slots and rank")
+                # (also for fewer rows, which can take more workspace)
+                need = max([need] + [qlin.lora_workspace_bytes(rows, len(there), *w.like[1:]) for w in there[:1]
+                                     for rows in range(1, self.max_prompt + 1)])
+        ids = torch.empty(self.max_prompt, dtype=torch.int32, device="cuda")
+        if not torch.is_tensor(slot):
+            slot = torch.full((1,), slot, dtype=torch.int32, device="cuda")
+        elif slot.dtype != torch.int32 or slot.numel() != 1 or slot.device != ids.device:
+            raise ValueError("slot: a number, or int32 [1] on the decoder's device")
+        self.adapters = dict(layers=layers, slot=slot, ids=ids, ranks=ranks, scales=scales,
+                             ws=torch.empty(need, dtype=torch.uint8, device="cuda"))
+
+    def _adapt(self, layer, x, rows, outs):
+        """Adds the layer's adapters of the linears in outs (name: output), which read x."""
+        A = self.adapters
+        mats = [(A["layers"][layer][n], y[:rows]) for n, y in outs.items() if n in A["layers"][layer]]
+        if mats:
+            qlin.lora_add(x[:rows], A["ids"], [(w, y, y) for w, y in mats], ranks=A["ranks"], scales=A["scales"], workspace=A["ws"])
+
     # ---- the calls -------------------------------------------------------------------------------
 
     def _ok(self, name, rc):
@@ -192,9 +238,17 @@ class Qwen2Decoder:
         H, F, QD, KD = c.hidden, c.ffn, c.q_dim, c.kv_dim
         h, xn, q, k, v, attn, act = (t(self.h), t(self.xn), t(self.q), t(self.k), t(self.v), t(self.attn),
                                      t(self.act))
-        fuse = rows == 1 and self.fuse
+        A = self.adapters
+        if A is not None:
+            # (the slot stands on the device: captured with what follows)
+            A["ids"].copy_(A["slot"].expand(self.max_prompt))
+            if self.torch.cuda.is_current_stream_capturing():
+                self.captured.append(A)  # (the graph reads these tensors)
         for i, W in enumerate(self.w["layers"]):
-            if fuse:
+            # (adapters of q, k and v read the normed rows, which the fused launch does not write)
+            fuse = rows == 1 and self.fuse
+            seen = A is not None and any(name in A["layers"][i] for name in self.LINEARS[0])
+            if fuse and not seen:
                 qlin.rms_norm_quant_gemv_multi(c.wtype, [W["wq"], W["wk"], W["wv"]], self.rb_h, h, W["attn_norm"], 0,
                                                c.eps, 0, [q, k, v], [QD, KD, KD], H)
             elif rows == 1:
@@ -204,6 +258,8 @@ class Qwen2Decoder:
                 self._norm(h, xn, W["attn_norm"], rows)
                 for name, y, n in (("wq", q, QD), ("wk", k, KD), ("wv", v, KD)):
                     self._ok("matmul", L.qlin_launch_quant_matmul(c.wtype, t(W[name]), self.rb_h, xn, y, n, H, rows))
+            if seen:
+                self._adapt(i, self.xn, rows, {"wq": self.q, "wk": self.k, "wv": self.v})
             if c.kv8:
                 qlin.qk_norm_rope_store_kv8(self.how[i], self.kv8[i], q, QD, k, KD, v, KD, q, rows, c.n_heads, pos_ptr)
                 qlin.attend_kv8(self.kv8[i], q, attn, rows, c.n_heads, pos_ptr, None, c.head_dim ** -0.5, self.attend_ws)
@@ -222,7 +278,9 @@ class Qwen2Decoder:
                 self._ok("attend", L.qlin_launch_attend(q, t(self.kc[i]), t(self.vc[i]), attn, rows, c.n_heads,
                                                         c.kv_heads, c.head_dim, self.max_seq, pos_ptr))
             self._ok("o", L.qlin_launch_quant_matmul_add(c.wtype, t(W["wo"]), self.rb_q, attn, h, H, QD, rows))
-            if fuse:
+            if A is not None:
+                self._adapt(i, self.attn, rows, {"wo": self.h})
+            if fuse:  # (its gate and up have no adapters)
                 self._ok("norm_swiglu", L.qlin_launch_rms_norm_quant_swiglu(c.wtype, t(W["wg"]), t(W["wu"]), self.rb_h,
                                                                             h, t(W["ffn_norm"]), 0, c.eps, 0, act, F,
                                                                             H))
@@ -235,6 +293,8 @@ class Qwen2Decoder:
                 self._ok("swiglu", L.qlin_launch_quant_swiglu_rows(c.wtype, t(W["wg"]), t(W["wu"]), self.rb_h,
                                                                    self.rb_h, xn, act, F, H, rows))
             self._ok("down", L.qlin_launch_quant_matmul_add(c.wtype, t(W["wd"]), self.rb_f, act, h, H, F, rows))
+            if A is not None:
+                self._adapt(i, self.act, rows, {"wd": self.h})
 
     def _head(self, row: int):
         """Final norm of residual row `row`, the tied output head, and the greedy pick into token."""
@@ -305,6 +365,46 @@ class Qwen2Decoder:
             self.torch.add(self.pos, 1, out=self.history_len)
         self._head(0)
         self.pos.add_(1)
+
+    def drafts(self, n: int) -> dict:
+        """What a call of step_drafts with n drafted tokens works on, for as long as it is used: drafts int32 [1, n] and
+        uniform float32 [1, n + 1] (numbers in [0, 1)), which the caller fills, and n_drafts int32 [1] (at first n) and
+        temperature float32 [1] (at first 0: greedy); tokens int32 [1, n + 1] (-1 after the last), accepted int32 [1], logprobs
+        and rates, which the call fills."""
+        torch, c, dev = self.torch, self.cfg, "cuda"
+        if not 0 <= n < min(self.max_prompt, qlin.KV8_BLOCK):  # (as far as the 8-bit cache takes positions back)
+            raise ValueError(f"{n} drafted tokens: at most {min(self.max_prompt, qlin.KV8_BLOCK) - 1}")
+        f = lambda *shape: torch.zeros(*shape, dtype=torch.float32, device=dev)
+        i = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)
+        return dict(drafts=i(1, n), uniform=f(1, n + 1), n_drafts=torch.full((1,), n, dtype=torch.int32, device=dev), temperature=f(1),
+                    tokens=i(1, n + 1), accepted=i(1), logprobs=f(1, n + 1), rates=f(1, n), logits=f(1, n + 1, c.vocab),
+                    ws=torch.empty(max(16, qlin.verify_drafts_workspace_bytes(1, n, c.vocab)), dtype=torch.uint8, device=dev))
+
+    def step_drafts(self, d: dict, draft_logits=None) -> None:
+        """Decode tokens by drafts (of self.drafts(n)): the next token and the n drafted ones after it in one pass, those
+        that the model's probabilities accept and one more; leaves pos after them and the last one as the next token (no host
+        synchronisation).  draft_logits float32 [1, n, vocab], or None for drafts by lookup.  The positions pos .. pos + n
+        are below max_seq; controls of the pick do not go with it."""
+        c, t, torch = self.cfg, c_ptr, self.torch
+        if self.controls is not None:
+            raise ValueError("drafts are not checked under controls")
+        rows = d["tokens"].shape[1]
+        self.stream = torch.cuda.current_stream()
+        qlin.set_stream(self.stream)
+        self.prompt_ids[:1].copy_(self.token)
+        # (a draft past n_drafts may be anything)
+        self.prompt_ids[1:rows].copy_(d["drafts"][0].clamp(0, c.vocab - 1))
+        self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.prompt_ids), t(self.h), t(self.w["table"]),
+                                                                 self.rb_h, c.hidden, rows))
+        self._layers(rows, t(self.pos))
+        self._norm(t(self.h), t(self.xn), self.w["final_norm"], rows)
+        self._ok("lm_head", self.L.qlin_launch_quant_matmul(c.wtype, t(self.w["table"]), self.rb_h, t(self.xn), t(d["logits"]),
+                                                            c.vocab, c.hidden, rows))
+        qlin.verify_drafts(d["logits"], d["drafts"], d["uniform"], d["tokens"], d["accepted"], draft_logits=draft_logits,
+                           n_drafts=d["n_drafts"], temperature=d["temperature"], logprobs=d["logprobs"], rates=d["rates"],
+                           workspace=d["ws"])
+        torch.index_select(d["tokens"][0], 0, d["accepted"], out=self.token)
+        self.pos.add_(d["accepted"]).add_(1)
 
     def generate(self, prompt, n_new: int, logits_out=None):
         """Greedy decode of n_new tokens after the prompt, eagerly; returns the token ids (host list).
