@@ -3,8 +3,8 @@
 //
 // Mathematics: z = A x, y = base + B (scale z), A and B those of the row's adapter.
 //
-// Rows of one adapter stand in tiles, of 16 rows (up to 256 rows in all, where each workgroup of the first launch groups the
-// ids by itself) or of 64 (a launch of one workgroup before it).  Weights are the A operand of the matrix cores, rows of x and
+// Rows of one adapter stand in tiles, of 16 rows (up to 256 rows in all, where each wave groups the ids by itself) or of 64 (a
+// launch of one workgroup before the others).  Weights are the A operand of the matrix cores, rows of x and
 // z the B operand.
 // 1. lora_down_kernel: z of a tile, up to 64 ranks and a slice of x: 4 waves take parts of the slice and meet in LDS.  Slices
 //    are stored apart and added up by the second launch, in order: no atomics.
@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kMostMats = 4;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kFewRows = 256;   // grouped by each workgroup; with more, a launch groups them
+constexpr int kFewRows = 256;   // grouped by each wave; with more, a launch groups them
 constexpr int kTile = 64;       // the most rows of a tile
 constexpr int kUpThreads = 512;  // of lora_up_kernel over tiles of 64 rows
 constexpr int kPart = 32;       // of a workgroup of lora_down_kernel
@@ -155,47 +155,66 @@ __device__ __forceinline__ f32x4 mfma_f32(const Weights<T> &w, const f32x4 (&v)[
     return acc;
 }
 
-// The tile of number `tile` among up to 256 rows, a row a thread: tiles are numbered by their first rows, and a tile's rows are in
-// order, so that every workgroup finds the same.  Gives the number of tiles.
-__device__ __forceinline__ int group_rows(const LoraArgs &a, int tile, Tile &t, int *s_ids, int *s_first, int *s_chunk) {
-    const int r = threadIdx.x;
-    const int mine = r < a.rows ? slot_of(a, r) : -1;
-    s_ids[r] = mine;
-    if (r == 0) {
-        t.count = 0;
-        t.adapter = -1;
-        *s_chunk = -1;
-    }
-    __syncthreads();
-    int before = 0;  // rows before this one that have its adapter
-    for (int i = 0; i < (r & ~63) + 64; i += 4) {  // (uniform in a wave)
-        const int4 v = *reinterpret_cast<const int4 *>(s_ids + i);
-        before += (v.x == mine && i < r) + (v.y == mine && i + 1 < r) + (v.z == mine && i + 2 < r) + (v.w == mine && i + 3 < r);
-    }
-    const bool first = mine >= 0 && before % 16 == 0;
-    const uint64_t firsts = __ballot(first);
-    if ((r & 63) == 0) s_first[r >> 6] = static_cast<int>(__popcll(firsts));
-    __syncthreads();
-    int at = static_cast<int>(__popcll(firsts & ((1ull << (r & 63)) - 1))), n = 0;
+// A tile's rows: in LDS, or of up to 16 in lanes 0 .. 15 of each wave.
+struct TileRows {
+    const int *rows;
+    __device__ __forceinline__ int operator()(int i) const { return rows[i]; }
+};
+struct LaneRows {
+    int row;
+    __device__ __forceinline__ int operator()(int i) const { return __builtin_amdgcn_ds_bpermute(4 * i, row); }
+};
+struct Group {
+    int adapter, count;  // -1: no adapter; no rows: no such tile
+};
+// The tile of number `tile` among up to 256 rows, by each wave for itself, 64 rows at a time: adapters in the order of their
+// first rows, an adapter's rows in order, so that every wave finds the same.  No LDS, no barrier: with both and a row a
+// thread one row of 896 to 896, 128 and 128 took 15.3 us in the two launches, so 9.6.
+__device__ __forceinline__ Group find_tile(const LoraArgs &a, int tile, LaneRows &rows) {
+    constexpr int I = kFewRows / 64;
+    const int lane = threadIdx.x & 63;
+    const uint64_t below = (1ull << lane) - 1;
+    int slot[I];
+    uint64_t todo[I], mine[I];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < (r >> 6)) at += s_first[w];
-        n += s_first[w];
+    for (int i = 0; i < I; ++i) {
+        slot[i] = -1;
+        if (64 * i < a.rows && 64 * i + lane < a.rows) slot[i] = slot_of(a, 64 * i + lane);
     }
-    if (first && at == tile) {
-        t.adapter = mine;
-        *s_chunk = before / 16;
+#pragma unroll
+    for (int i = 0; i < I; ++i) todo[i] = __ballot(slot[i] >= 0);
+    int id = 0, count = 0;
+#pragma unroll 1
+    for (;;) {  // uniform
+        if (todo[0]) id = __builtin_amdgcn_readlane(slot[0], __builtin_ctzll(todo[0]));
+        else if (todo[1]) id = __builtin_amdgcn_readlane(slot[1], __builtin_ctzll(todo[1]));
+        else if (todo[2]) id = __builtin_amdgcn_readlane(slot[2], __builtin_ctzll(todo[2]));
+        else if (todo[3]) id = __builtin_amdgcn_readlane(slot[3], __builtin_ctzll(todo[3]));
+        else return Group{-1, 0};
+        count = 0;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            mine[i] = __ballot(slot[i] == id);
+            todo[i] &= ~mine[i];
+            count += static_cast<int>(__popcll(mine[i]));
+        }
+        const int n = (count + 15) / 16;
+        if (tile < n) break;
+        tile -= n;
     }
-    __syncthreads();
-    if (mine >= 0 && mine == t.adapter && before / 16 == *s_chunk) {
-        t.rows[before % 16] = r;
-        atomicMax(&t.count, before % 16 + 1);
+    // each row to the lane of its place, plus one; lanes that nothing comes to get 0
+    int before = -16 * tile, row = 0;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int place = before + static_cast<int>(__popcll(mine[i] & below));
+        const bool in = (mine[i] >> lane & 1) && place >= 0 && place < 16;
+        row = max(row, __builtin_amdgcn_ds_permute(4 * (in ? place : 63), in ? 64 * i + lane + 1 : 0));
+        before += static_cast<int>(__popcll(mine[i]));
     }
-    __syncthreads();
-    if (r == 0 && t.adapter == a.n_adapters) t.adapter = -1;
-    __syncthreads();
-    return n;
+    rows.row = max(row - 1, 0);  // (lanes past the last row: another)
+    return Group{id < a.n_adapters ? id : -1, min(16, count - 16 * tile)};
 }
+static_assert(kFewRows == 256, "find_tile has four registers of rows");
 
 // More rows: one workgroup counts each adapter's rows, gives it its tiles and puts the rows into them.  (In what order does
 // not matter: a row's results do not depend on its tile.)
@@ -263,8 +282,8 @@ __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
 // kDownBytes<NT>() for the workgroup.
 template <int NT>
 constexpr int kDownBytes = kWaves * (kRanks / 16 * NT * 64 * 16 > 16 * NT * kRowBytes ? kRanks / 16 * NT * 64 * 16 : 16 * NT * kRowBytes);
-template <int T, int NT>
-__device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int first, int mat, int group, int split, char *lds) {
+template <int T, int NT, class R>
+__device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R &rows, int first, int mat, int group, int split, char *lds) {
     constexpr int RT = kRanks / 16, K = Weights<T>::kValues, H = K / 32;  // a step: a line of weights, H lines of x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int rank = rank_of(a, t.adapter) - group * kRanks;
@@ -279,7 +298,7 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int first
     // (rows past the tile's or the rank's end are others again; what comes of them is not stored)
     const float *x[2 * NT];
 #pragma unroll
-    for (int j = 0; j < 2 * NT; ++j) x[j] = a.x + t.rows[min(first + 8 * j + (lane >> 3), t.count - 1)] * a.x_stride;
+    for (int j = 0; j < 2 * NT; ++j) x[j] = a.x + rows(min(first + 8 * j + (lane >> 3), t.count - 1)) * a.x_stride;
     const char *w[2 * RT];
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i)
@@ -424,51 +443,36 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Tile &t, int first
         f32x4 sum = s_z[tile * 64 + of];
 #pragma unroll
         for (int v = 1; v < kWaves; ++v) sum += s_z[(v * RT * NT + tile) * 64 + of];
-        const int row = first + 16 * j + (lane >> 2), k = group * kRanks + 16 * rt + 4 * (lane & 3);
-        if (row < t.count && k < a.max_rank)
-            *reinterpret_cast<f32x4 *>(a.z + ((static_cast<size_t>(split) * a.n_mats + mat) * a.rows + t.rows[row]) * a.max_rank + k) = sum;
+        const int at = first + 16 * j + (lane >> 2), row = rows(min(at, t.count - 1)), k = group * kRanks + 16 * rt + 4 * (lane & 3);
+        if (at < t.count && k < a.max_rank)
+            *reinterpret_cast<f32x4 *>(a.z + ((static_cast<size_t>(split) * a.n_mats + mat) * a.rows + row) * a.max_rank + k) = sum;
     }
 }
 
-// FEW: at most 256 rows in tiles of 16, a workgroup for each tile that there can be; else the tiles that there are in turn.
+// FEW: tiles of 16 that each wave finds, a workgroup for each that there can be; else those that there are, in turn.
 template <int T, bool FEW>
 __global__ __launch_bounds__(kThreads, 2) void lora_down_kernel(LoraArgs a) {
-    __shared__ Tile t;
     __shared__ __attribute__((aligned(16))) char s_z[kDownBytes<FEW ? 1 : kPart / 16>];
     const int groups = (a.max_rank + kRanks - 1) / kRanks, units = a.n_mats * groups * a.splits * (FEW ? 1 : kTile / kPart);
     if constexpr (FEW) {
-        __shared__ __attribute__((aligned(16))) int s_ids[kFewRows];
-        __shared__ int s_first[kWaves], s_chunk;
-        const int tile = blockIdx.x / units, unit = blockIdx.x % units;
-        const int n = group_rows(a, tile, t, s_ids, s_first, &s_chunk);
-        if (unit == 0) {  // for lora_up_kernel
-            if (tile < n) {
-                if (threadIdx.x < 16) a.tiles[tile].rows[threadIdx.x] = t.rows[threadIdx.x];
-                if (threadIdx.x == 0) {
-                    a.tiles[tile].adapter = t.adapter;
-                    a.tiles[tile].count = t.count;
-                }
-            }
-            if (tile == 0 && threadIdx.x == 0) *a.n_tiles = n;
-        }
-        if (tile >= n || t.adapter < 0) return;  // uniform
-        const int split = unit % a.splits, rest = unit / a.splits;
-        down<T, 1>(a, t, 0, rest % a.n_mats, rest / a.n_mats, split, s_z);
+        const int unit = blockIdx.x % units, split = unit % a.splits, rest = unit / a.splits;
+        LaneRows rows;
+        const Group t = find_tile(a, blockIdx.x / units, rows);
+        if (t.adapter >= 0) down<T, 1>(a, t, rows, 0, rest % a.n_mats, rest / a.n_mats, split, s_z);
     } else {
+        __shared__ Tile t;
+        const TileRows rows = {t.rows};
         const int total = *a.n_tiles * units;
         for (int item = blockIdx.x; item < total; item += gridDim.x) {
             const int tile = item / units, unit = item % units;
             __syncthreads();  // (the tile and the sums of before are read)
             if (threadIdx.x < kTile) t.rows[threadIdx.x] = a.tiles[tile].rows[threadIdx.x];
-            if (threadIdx.x == 0) {
-                t.adapter = a.tiles[tile].adapter;
-                t.count = a.tiles[tile].count;
-            }
+            const Group of = {a.tiles[tile].adapter, a.tiles[tile].count};
             __syncthreads();
             const int split = unit % a.splits, part = unit / a.splits % (kTile / kPart) * kPart, rest = unit / a.splits / (kTile / kPart);
-            if (t.adapter < 0 || part >= t.count) continue;  // uniform
-            if (t.count - part <= 16) down<T, 1>(a, t, part, rest % a.n_mats, rest / a.n_mats, split, s_z);
-            else down<T, kPart / 16>(a, t, part, rest % a.n_mats, rest / a.n_mats, split, s_z);
+            if (of.adapter < 0 || part >= of.count) continue;  // uniform
+            if (of.count - part <= 16) down<T, 1>(a, of, rows, part, rest % a.n_mats, rest / a.n_mats, split, s_z);
+            else down<T, kPart / 16>(a, of, rows, part, rest % a.n_mats, rest / a.n_mats, split, s_z);
         }
     }
 }
@@ -518,12 +522,13 @@ struct Up {
     char *mine;
     int lane, rank, max_rank;
 
-    __device__ __forceinline__ Up(const LoraArgs &a, const Tile &t, int mat, int from, int rank, char *mine)
+    template <class R>
+    __device__ __forceinline__ Up(const LoraArgs &a, const Group &t, const R &rows, int mat, int from, int rank, char *mine)
         : m(a.mats[mat]), mine(mine), lane(threadIdx.x & 63), rank(rank), max_rank(a.max_rank) {
         b = static_cast<const char *>(m.b) + static_cast<size_t>(max(t.adapter, 0)) * m.out_dim * max_rank * Weights<T>::kBytes;
 #pragma unroll
         for (int j = 0; j < 2 * NT; ++j) {
-            const int at = from + 8 * j + (lane >> 3), row = t.rows[min(at, t.count - 1)];
+            const int at = from + 8 * j + (lane >> 3), row = rows(min(at, t.count - 1));
             there[j] = at < t.count;
             base[j] = m.base + row * m.base_stride + 4 * (lane & 7);
             y[j] = m.y + row * m.y_stride + 4 * (lane & 7);
@@ -634,103 +639,125 @@ struct Up {
 };
 constexpr int kUpBytes = 32 * kRowBytes;  // of a wave
 
+// One run of outputs of one tile, by N threads.  s_z: the waves' own rows, then z of at most M rows.
+template <int T, int N, int M, class R>
+__device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &rows, int run, char *s_z, int &s_wide) {
+    int mat = 0;
+    while (run >= a.chunks[mat]) ++mat;
+    if (mat > 0) run -= a.chunks[mat - 1];
+    if (t.adapter < 0 && a.mats[mat].y == a.mats[mat].base) return;  // uniform
+    char *const s_parts = s_z + N / 64 * kUpBytes;
+    const int width = (a.max_rank + 31) / 32 * 32, wave = threadIdx.x >> 6;
+    const int first = run * a.chunk, last = min(first + a.chunk, a.mats[mat].out_dim);
+    // a wave takes 32 rows (16 of few): where there are more, waves go two by two
+    constexpr int NT = M > 16 ? 2 : 1;
+    const bool both = t.count > 16 * NT;
+    const int from = both ? 16 * NT * (wave & 1) : 0, step = 32 * (N / 64) / (both ? 2 : 1);
+    int o = first + 32 * (both ? wave >> 1 : wave);
+    const int rank = t.adapter < 0 ? 0 : rank_of(a, t.adapter);
+    Up<T, NT> up(a, t, rows, mat, from, rank, s_z + wave * kUpBytes);
+    if (o < last) up.load(o);  // (requested before z is staged)
+    const int quads = (rank + 31) / 32 * 8;  // of a row
+    const float scale = t.adapter >= 0 && a.scales ? a.scales[t.adapter] : 1.0f;
+    const int staged = (t.count + 15) / 16 * 16 * quads;
+    const size_t split = static_cast<size_t>(a.n_mats) * a.rows * a.max_rank;
+    auto z_of = [&](int row, int k) {  // scale z, 4 values; row < 0: none
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (row >= 0 && k < rank) {
+            const float *p = a.z + (static_cast<size_t>(mat) * a.rows + row) * a.max_rank + k;
+            int s = 0;
+#pragma unroll 1
+            for (; s + 4 <= a.splits; s += 4) {
+                f32x4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4 *>(p + (s + i) * split);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += v[i];
+            }
+#pragma unroll 1
+            for (; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + s * split);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = k + e < rank ? sum[e] * scale : 0.0f;
+        }
+        return sum;
+    };
+    auto each = [&](auto put) {  // (whole waves, as rows may stand in their lanes)
+#pragma unroll 1
+        for (int i0 = wave * 64; i0 < staged; i0 += N) {
+            const int i = i0 + (threadIdx.x & 63), r = i / quads;
+            const int row = rows(min(r, t.count - 1));
+            if (i < staged) put(r, r < t.count ? row : -1, 4 * (i % quads));
+        }
+    };
+    // (rows 16 bytes more than a multiple of 64 apart: 16 lanes meet 16 times 4 banks)
+    Staged z = {2 * width + 16, M * (2 * width + 16), T == 2};
+    if constexpr (T != 2) {
+        bool wide = false;
+        each([&](int r, int row, int k) {
+            const f32x4 v = z_of(row, k);
+            wide |= !(max3_abs(v[0], v[1], fmaxf(fabsf(v[2]), fabsf(v[3]))) < kWide);
+            uint2 h, m, l;
+            split3(v[0] * kUp, v[1] * kUp, h.x, m.x, l.x);
+            split3(v[2] * kUp, v[3] * kUp, h.y, m.y, l.y);
+            char *at = s_parts + r * z.stride + 2 * k;
+            *reinterpret_cast<uint2 *>(at) = h;
+            *reinterpret_cast<uint2 *>(at + z.part) = m;
+            *reinterpret_cast<uint2 *>(at + 2 * z.part) = l;
+        });
+        if (wide) s_wide = 1;
+        __syncthreads();
+        z.wide = s_wide != 0;
+    }
+    if (z.wide) {  // uniform
+        z.stride = 4 * width + 16;
+        if (T != 2) __syncthreads();
+        each([&](int r, int row, int k) { *reinterpret_cast<f32x4 *>(s_parts + r * z.stride + 4 * k) = z_of(row, k); });
+        __syncthreads();
+    }
+    const char *rows_z = s_parts + from * z.stride;
+    if constexpr (T != 2) {
+        if (!z.wide) {  // uniform
+#pragma unroll 1
+            for (; o < last; o += step) up.template add<false>(o, o + step, last, z, rows_z);
+            return;
+        }
+    }
+#pragma unroll 1
+    for (; o < last; o += step) up.template add<true>(o, o + step, last, z, rows_z);
+}
+
 template <int T, bool FEW>
 __global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel(LoraArgs a) {
-    constexpr int M = FEW ? 16 : kTile, N = FEW ? kThreads : kUpThreads;
-    extern __shared__ __attribute__((aligned(16))) char s_z[];  // the waves' own rows, then z
-    __shared__ Tile t;
+    extern __shared__ __attribute__((aligned(16))) char s_z[];
     __shared__ int s_wide;
-    char *const s_parts = s_z + N / 64 * kUpBytes;
-    const int width = (a.max_rank + 31) / 32 * 32;
-    const int runs = a.chunks[a.n_mats - 1], total = *a.n_tiles * runs;
-    for (int item = blockIdx.x; item < total; item += gridDim.x) {
-        const int tile = item / runs;
-        int run = item % runs, mat = 0;
-        while (run >= a.chunks[mat]) ++mat;
-        if (mat > 0) run -= a.chunks[mat - 1];
-        __syncthreads();  // (the tile of before is read)
-        if (threadIdx.x < M) t.rows[threadIdx.x] = a.tiles[tile].rows[threadIdx.x];
-        if (threadIdx.x == 0) {
-            t.adapter = a.tiles[tile].adapter;
-            t.count = a.tiles[tile].count;
-            s_wide = 0;
-        }
+    const int runs = a.chunks[a.n_mats - 1];
+    if constexpr (FEW) {
+        LaneRows rows;
+        const Group t = find_tile(a, blockIdx.x / runs, rows);
+        if (t.count == 0) return;  // uniform
+        if (threadIdx.x == 0) s_wide = 0;
         __syncthreads();
-        if (t.adapter < 0 && a.mats[mat].y == a.mats[mat].base) continue;  // uniform
-        const int first = run * a.chunk, last = min(first + a.chunk, a.mats[mat].out_dim), wave = threadIdx.x >> 6;
-        // a wave takes 32 rows (16 of few): where there are more, waves go two by two
-        constexpr int NT = FEW ? 1 : 2;
-        const bool both = t.count > 16 * NT;
-        const int from = both ? 16 * NT * (wave & 1) : 0, step = 32 * (N / 64) / (both ? 2 : 1);
-        int o = first + 32 * (both ? wave >> 1 : wave);
-        const int rank = t.adapter < 0 ? 0 : rank_of(a, t.adapter);
-        Up<T, NT> up(a, t, mat, from, rank, s_z + wave * kUpBytes);
-        if (o < last) up.load(o);  // (requested before z is staged)
-        const int quads = (rank + 31) / 32 * 8;  // of a row
-        const float scale = t.adapter >= 0 && a.scales ? a.scales[t.adapter] : 1.0f;
-        const int rows = (t.count + 15) / 16 * 16;
-        const size_t split = static_cast<size_t>(a.n_mats) * a.rows * a.max_rank;
-        auto z_of = [&](int r, int k) {  // scale z, 4 values
-            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (r < t.count && k < rank) {
-                const float *p = a.z + (static_cast<size_t>(mat) * a.rows + t.rows[r]) * a.max_rank + k;
-                int s = 0;
-                for (; s + 4 <= a.splits; s += 4) {
-                    f32x4 v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4 *>(p + (s + i) * split);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum += v[i];
-                }
-                for (; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + s * split);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] = k + e < rank ? sum[e] * scale : 0.0f;
-            }
-            return sum;
-        };
-        // (rows 16 bytes more than a multiple of 64 apart: 16 lanes meet 16 times 4 banks)
-        Staged z = {2 * width + 16, M * (2 * width + 16), T == 2};
-        if constexpr (T != 2) {
-            bool wide = false;
-            for (int i = threadIdx.x; i < rows * quads; i += N) {
-                const int r = i / quads, k = 4 * (i % quads);
-                const f32x4 v = z_of(r, k);
-                wide |= !(max3_abs(v[0], v[1], fmaxf(fabsf(v[2]), fabsf(v[3]))) < kWide);
-                uint2 h, m, l;
-                split3(v[0] * kUp, v[1] * kUp, h.x, m.x, l.x);
-                split3(v[2] * kUp, v[3] * kUp, h.y, m.y, l.y);
-                char *at = s_parts + r * z.stride + 2 * k;
-                *reinterpret_cast<uint2 *>(at) = h;
-                *reinterpret_cast<uint2 *>(at + z.part) = m;
-                *reinterpret_cast<uint2 *>(at + 2 * z.part) = l;
-            }
-            if (wide) s_wide = 1;
+        up<T, kThreads, 16>(a, t, rows, blockIdx.x % runs, s_z, s_wide);
+    } else {
+        __shared__ Tile t;
+        const TileRows rows = {t.rows};
+        const int total = *a.n_tiles * runs;
+        for (int item = blockIdx.x; item < total; item += gridDim.x) {
+            const int tile = item / runs;
+            __syncthreads();  // (the tile of before is read)
+            if (threadIdx.x < kTile) t.rows[threadIdx.x] = a.tiles[tile].rows[threadIdx.x];
+            if (threadIdx.x == 0) s_wide = 0;
+            const Group of = {a.tiles[tile].adapter, a.tiles[tile].count};
             __syncthreads();
-            z.wide = s_wide != 0;
+            up<T, kUpThreads, kTile>(a, of, rows, item % runs, s_z, s_wide);
         }
-        if (z.wide) {  // uniform
-            z.stride = 4 * width + 16;
-            __syncthreads();
-            for (int i = threadIdx.x; i < rows * quads; i += N) {
-                const int r = i / quads, k = 4 * (i % quads);
-                *reinterpret_cast<f32x4 *>(s_parts + r * z.stride + 4 * k) = z_of(r, k);
-            }
-            __syncthreads();
-        }
-        const char *rows_z = s_parts + from * z.stride;
-        if constexpr (T != 2) {
-            if (!z.wide) {  // uniform
-#pragma unroll 1
-                for (; o < last; o += step) up.template add<false>(o, o + step, last, z, rows_z);
-                continue;
-            }
-        }
-#pragma unroll 1
-        for (; o < last; o += step) up.template add<true>(o, o + step, last, z, rows_z);
     }
 }
 
 bool al(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Whether each wave groups the rows: what that takes grows with the adapters in use, 64 rows at a time, a launch for it takes 4 us.
+bool few_of(int rows, int n_adapters) { return rows <= 64 || (rows <= kFewRows && n_adapters < 64); }
 
 struct Layout {
     int most_tiles, groups, splits;
@@ -738,7 +765,7 @@ struct Layout {
 };
 Layout layout_of(int rows, int n_mats, int n_adapters, int max_rank, int in_dim) {
     Layout l;
-    const bool few = rows <= kFewRows;
+    const bool few = few_of(rows, n_adapters);
     const int m = few ? 16 : kTile, kinds = rows < n_adapters + 1 ? rows : n_adapters + 1;
     l.most_tiles = rows / m + kinds;
     if (l.most_tiles > rows) l.most_tiles = rows;
@@ -805,7 +832,7 @@ int qlin_launch_lora_add(const qlin_lora *mats, int n_mats, int weight_type, int
     a.ranks = ranks, a.ids = adapter_ids, a.scales = scales, a.x = x, a.x_stride = x_stride;
     a.n_tiles = reinterpret_cast<int *>(ws), a.tiles = reinterpret_cast<qlin::Tile *>(ws + l.tiles), a.z = reinterpret_cast<float *>(ws + l.z);
     a.n_mats = kept, a.n_adapters = n_adapters, a.max_rank = max_rank, a.in_dim = in_dim, a.rows = rows, a.splits = l.splits;
-    const bool few = rows <= qlin::kFewRows;
+    const bool few = qlin::few_of(rows, n_adapters);
     // outputs of a workgroup: as many as leave 128 of them, each stages z again
     int64_t outputs = 0;
     for (int i = 0; i < kept; ++i) outputs += a.mats[i].out_dim;
@@ -821,7 +848,7 @@ int qlin_launch_lora_add(const qlin_lora *mats, int n_mats, int weight_type, int
     auto go = [&](auto down, auto up) {
         if (!few) hipLaunchKernelGGL(qlin::lora_group_kernel, dim3(1), dim3(qlin::kGroupThreads), 0, s, a);
         hipLaunchKernelGGL(down, dim3(static_cast<unsigned>(few ? downs : downs < 2048 ? downs : 2048)), dim3(qlin::kThreads), 0, s, a);
-        hipLaunchKernelGGL(up, dim3(static_cast<unsigned>(ups < 2048 ? ups : 2048)), dim3(few ? qlin::kThreads : qlin::kUpThreads), lds, s, a);
+        hipLaunchKernelGGL(up, dim3(static_cast<unsigned>(few || ups < 2048 ? ups : 2048)), dim3(few ? qlin::kThreads : qlin::kUpThreads), lds, s, a);
         return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
     };
     using namespace qlin;
