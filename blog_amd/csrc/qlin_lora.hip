@@ -228,7 +228,17 @@ __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
     for (int i = tid; i < kinds; i += kGroupThreads) s_count[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kKept; ++i) place[i] = slot[i] >= 0 ? atomicAdd(&s_count[slot[i]], 1) : 0;
+    for (int i = 0; i < kKept; ++i) {
+        place[i] = 0;
+        const int first = __builtin_amdgcn_readfirstlane(slot[i]);
+        if (__all(slot[i] == first)) {  // a run: one addition for 64 rows, where 64 would come one after the other
+            if (first < 0) continue;
+            if (lane == 0) place[i] = atomicAdd(&s_count[first], 64);
+            place[i] = __builtin_amdgcn_readfirstlane(place[i]) + lane;
+        } else if (slot[i] >= 0) {
+            place[i] = atomicAdd(&s_count[slot[i]], 1);
+        }
+    }
     __syncthreads();  // (the kept rows' places are the first ones, those of the rest come after them all)
     const int rest = tid + kKept * kGroupThreads;
     for (int r = rest; r < a.rows; r += kGroupThreads) {
@@ -757,7 +767,7 @@ __global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel
 bool al(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Whether each wave groups the rows: what that takes grows with the adapters in use, 64 rows at a time, a launch for it takes 4 us.
-bool few_of(int rows, int n_adapters) { return rows <= 64 || (rows <= kFewRows && n_adapters < 64); }
+bool few_of(int rows, int n_adapters) { return rows <= 64 || (rows <= kFewRows && n_adapters < 32); }
 
 struct Layout {
     int most_tiles, groups, splits;
@@ -770,11 +780,13 @@ Layout layout_of(int rows, int n_mats, int n_adapters, int max_rank, int in_dim)
     l.most_tiles = rows / m + kinds;
     if (l.most_tiles > rows) l.most_tiles = rows;
     l.groups = (max_rank + kRanks - 1) / kRanks;
-    // slices of x: as many as give about 512 workgroups, each wave 2 steps of 32 at least
-    const int steps = (in_dim + 31) / 32;
-    int64_t tiles = few ? l.most_tiles : (rows + kPart - 1) / kPart;
+    // slices of x: as many as give about 512 workgroups, but each is stored apart and read by every run of outputs, so that a
+    // wave has 8 steps of 32 values at least, 2 of few rows, where it is latency that counts (2011 rows of 4096 to 14336 in 8
+    // slices of 4 steps 85.0 us, in 4 of 8 82.2; 613 rows of 18944 to 3584 in 16 44.7, in 8 47.5)
+    const int steps = (in_dim + 31) / 32, least = few ? 2 : 8;
+    const int64_t tiles = few ? l.most_tiles : (rows + kPart - 1) / kPart;
     l.splits = static_cast<int>(512 / (tiles * n_mats * l.groups));
-    if (l.splits > steps / (2 * kWaves)) l.splits = steps / (2 * kWaves);  // (steps of 32)
+    if (l.splits > steps / (least * kWaves)) l.splits = steps / (least * kWaves);
     if (l.splits > 16) l.splits = 16;
     if (l.splits < 1) l.splits = 1;
     l.tiles = 16;
@@ -833,12 +845,13 @@ int qlin_launch_lora_add(const qlin_lora *mats, int n_mats, int weight_type, int
     a.n_tiles = reinterpret_cast<int *>(ws), a.tiles = reinterpret_cast<qlin::Tile *>(ws + l.tiles), a.z = reinterpret_cast<float *>(ws + l.z);
     a.n_mats = kept, a.n_adapters = n_adapters, a.max_rank = max_rank, a.in_dim = in_dim, a.rows = rows, a.splits = l.splits;
     const bool few = qlin::few_of(rows, n_adapters);
-    // outputs of a workgroup: as many as leave 128 of them, each stages z again
+    // outputs of a workgroup: as many as leave 256 workgroups, since each stages z again (128: 2048 rows of 4096 to 4096 at rank 16
+    // 40.8 us, 256: 37.0), but a step of its waves at least
     int64_t outputs = 0;
     for (int i = 0; i < kept; ++i) outputs += a.mats[i].out_dim;
     const int64_t tiles = few ? l.most_tiles : (rows + qlin::kTile - 1) / qlin::kTile;
     a.chunk = 4096;
-    while (a.chunk > 128 && tiles * outputs < static_cast<int64_t>(128) * a.chunk) a.chunk /= 2;
+        while (a.chunk > (few ? 128 : 256) && tiles * outputs < static_cast<int64_t>(256) * a.chunk) a.chunk /= 2;
     int runs = 0;
     for (int i = 0; i < kept; ++i) a.chunks[i] = runs += (a.mats[i].out_dim + a.chunk - 1) / a.chunk;
     const int64_t downs = static_cast<int64_t>(l.most_tiles) * kept * l.groups * l.splits * (few ? 1 : qlin::kTile / qlin::kPart), ups = static_cast<int64_t>(l.most_tiles) * runs;
