@@ -642,8 +642,12 @@ struct Up {
 #pragma unroll
         for (int j = 0; j < 2 * NT; ++j)
             if (there[j]) {
-                if (o + 32 <= m.out_dim) __builtin_memcpy(__builtin_assume_aligned(y[j] + o, 4), &now[j], 16);  // uniform
-                else store_values(y[j], o, m.out_dim - 4 * (lane & 7), now[j]);
+                if (o + 32 <= m.out_dim) {  // uniform
+                    if constexpr (NT > 1) __builtin_nontemporal_store(now[j], reinterpret_cast<f32x4u *>(y[j] + o));
+                    else __builtin_memcpy(__builtin_assume_aligned(y[j] + o, 4), &now[j], 16);
+                } else {
+                    store_values(y[j], o, m.out_dim - 4 * (lane & 7), now[j]);
+                }
             }
     }
 };
