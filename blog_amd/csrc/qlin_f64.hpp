@@ -37,6 +37,25 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return halves(h32[0], l32[0]) + halves(h32[1], l32[1]);
 }
 
+// The sums over lanes 0 .. l in lane l (every lane active): within rows of 16 lanes by shifts of 1, 2, 4 and 8, then the last
+// lane of a row to the row after it, and lane 31 to the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_from_f64(double x) {  // 0 in lanes that nothing comes to
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xf, false);
+    return halves(hi, lo);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+    v += dpp_from_f64<0x111, 0xf>(v);  // row_shr
+    v += dpp_from_f64<0x112, 0xf>(v);
+    v += dpp_from_f64<0x114, 0xf>(v);
+    v += dpp_from_f64<0x118, 0xf>(v);
+    v += dpp_from_f64<0x142, 0xa>(v);  // row_bcast15 to rows 1 and 3
+    v += dpp_from_f64<0x143, 0xc>(v);  // row_bcast31 to rows 2 and 3
+    return v;
+}
+
 // e^x: n = rint(x / ln 2), e^x = 2^n e^r with r = x - n ln 2, |r| <= ln 2 / 2, from ln 2 in two parts, and e^r by its
 // Taylor polynomial of degree 13 (the first term left out is below 5e-18).  1 to 2 units of the last place; 0 from about
 // -745 down, infinite from 710 up, 0 for NaN.

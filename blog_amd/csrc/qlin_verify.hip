@@ -205,12 +205,7 @@ __device__ __forceinline__ Pick draw(const double (&w)[U], int each, Goal goal_o
     double mine = 0.0;
 #pragma unroll
     for (int e = 0; e < U; ++e) mine += w[e];
-    double run = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(run, o, 64);
-        if (lane >= o) run += up;
-    }
+    double run = wave_scan_f64(mine);
     __syncthreads();  // (sh's readers of before are done)
     if (lane == 63) sh.part[wave] = run;
     if (tid == 0) {
@@ -279,8 +274,16 @@ __device__ __forceinline__ int draw_row(const VerifyArgs &a, double u, Slice sli
 }
 template <int U>
 __device__ __forceinline__ void logits_of(const float *p, int i, int n, float (&v)[U]) {
+    if constexpr (U % 4 == 0) {
 #pragma unroll
-    for (int e = 0; e < U; ++e) v[e] = i + e < n ? p[i + e] : -INFINITY;
+        for (int e = 0; e < U; e += 4) {
+            const f32x4v x = logits_at(p, i + e, n);
+            v[e] = x[0], v[e + 1] = x[1], v[e + 2] = x[2], v[e + 3] = x[3];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < U; ++e) v[e] = i + e < n ? p[i + e] : -INFINITY;
+    }
 #pragma unroll
     for (int e = 0; e < U; ++e) v[e] = number(v[e]);
 }
