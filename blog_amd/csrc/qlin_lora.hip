@@ -289,9 +289,10 @@ __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
 }
 
 // z of 16 NT rows of a tile from its row `first` on, one projection, one group of ranks and one slice of x.  lds: at least
-// kDownBytes<NT>() for the workgroup.
-template <int NT>
-constexpr int kDownBytes = kWaves * (kRanks / 16 * NT * 64 * 16 > 16 * NT * kRowBytes ? kRanks / 16 * NT * 64 * 16 : 16 * NT * kRowBytes);
+// kDownBytes for the workgroup.
+constexpr int kDownRows = 64;  // of LDS a wave: two lines of 32 rows of x, or a line of 64 rows of weights
+constexpr int kDownBytes = kWaves * kDownRows * kRowBytes;
+static_assert(kDownBytes >= kWaves * (kRanks / 16) * (kPart / 16) * 64 * 16, "the waves' sums");
 template <int T, int NT, class R>
 __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R &rows, int first, int mat, int group, int split, char *lds) {
     constexpr int RT = kRanks / 16, K = Weights<T>::kValues, H = K / 32;  // a step: a line of weights, H lines of x
@@ -335,7 +336,8 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
             }
     };
     // A lane's operands: row n of 16, the values 8 g .. of 32.
-    char *mine = lds + wave * (16 * NT * kRowBytes);
+    static_assert(H * 16 * NT <= kDownRows && 16 * RT <= kDownRows, "");
+    char *mine = lds + wave * (kDownRows * kRowBytes);
     const int n = lane & 15, g = lane >> 4;
     auto multiply = [&](Step &s, int at, auto wide) {
         if (K * at + K > a.in_dim) {  // uniform
@@ -347,27 +349,30 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
                     for (int e = 0; e < 4; ++e) s.x[h][j][e] = K * at + 32 * h + 4 * (lane & 7) < a.in_dim ? s.x[h][j][e] : 0.0f;
         }
         f32x4 v[H][NT][2];
+        wave_sync();
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            wave_sync();
-            put_rows(mine, s.x[h], lane);
-            wave_sync();
+        for (int h = 0; h < H; ++h) put_rows(mine + h * 16 * NT * kRowBytes, s.x[h], lane);
+        wave_sync();
+#pragma unroll
+        for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) v[h][j][i] = *reinterpret_cast<const f32x4 *>(mine + (16 * j + n) * kRowBytes + 32 * g + 16 * i);
-        }
+                for (int i = 0; i < 2; ++i)
+                    v[h][j][i] = *reinterpret_cast<const f32x4 *>(mine + (16 * (h * NT + j) + n) * kRowBytes + 32 * g + 16 * i);
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            if (i < tiles) put_rows(mine + 16 * i * kRowBytes, s.w[i], lane);
+        wave_sync();
         if constexpr (decltype(wide)::value) {
 #pragma unroll
             for (int i = 0; i < RT; ++i)
                 if (i < tiles) {
-                    wave_sync();
-                    put_rows(mine, s.w[i], lane);
-                    wave_sync();
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
                         Weights<T> o;
-                        o.get(mine + n * kRowBytes, 4 * h + g);
+                        o.get(mine + (16 * i + n) * kRowBytes, 4 * h + g);
 #pragma unroll
                         for (int j = 0; j < NT; ++j) acc[i][j] = mfma_f32(o, v[h][j], acc[i][j]);
                     }
@@ -390,13 +395,10 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
 #pragma unroll
             for (int i = 0; i < RT; ++i)
                 if (i < tiles) {
-                    wave_sync();
-                    put_rows(mine, s.w[i], lane);
-                    wave_sync();
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
                         Weights<T> r;
-                        r.get(mine + n * kRowBytes, 4 * h + g);
+                        r.get(mine + (16 * i + n) * kRowBytes, 4 * h + g);
                         const Operands<T> o(r);
 #pragma unroll
                         for (int j = 0; j < NT; ++j) acc[i][j] = o.times(hi[h][j], mid[h][j], lo[h][j], acc[i][j]);
@@ -462,7 +464,7 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
 // FEW: tiles of 16 that each wave finds, a workgroup for each that there can be; else those that there are, in turn.
 template <int T, bool FEW>
 __global__ __launch_bounds__(kThreads, 2) void lora_down_kernel(LoraArgs a) {
-    __shared__ __attribute__((aligned(16))) char s_z[kDownBytes<FEW ? 1 : kPart / 16>];
+    __shared__ __attribute__((aligned(16))) char s_z[kDownBytes];
     const int groups = (a.max_rank + kRanks - 1) / kRanks, units = a.n_mats * groups * a.splits * (FEW ? 1 : kTile / kPart);
     if constexpr (FEW) {
         const int unit = blockIdx.x % units, split = unit % a.splits, rest = unit / a.splits;

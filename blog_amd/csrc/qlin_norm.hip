@@ -10,7 +10,7 @@
 // that outputs may take the inputs' place.  Many rows are bound by HBM: 2011 rows of 4096 with their sum and blocks of 128 and
 // the blocks read back, 151 MB, take 35.8 us in a graph (4.2 TB/s; 4 waves of 4 runs 38.0, 16 of one 36.9), 42.1 with f32 results
 // through the caches: from 16 MB on they leave as streaming stores.  Few rows are bound by latency, and 16 waves take a row of
-// 3584 in 3.0 us, 4 waves in 4.9 (each with the read back).
+// 3584 in 4.5 us, 4 waves in 6.4.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -219,6 +219,7 @@ int qlin_launch_add_rms_norm(const float *x, size_t x_stride, const float *delta
                         one_plus, rows, hidden, (hidden + unit - 1) / unit * unit, mmq != 0, raw_sum != 0, eps};
     if (a.padded <= 256) qlin::launch<1, 1>(a);
     else if (a.padded <= 1024) qlin::launch<4, 1>(a);
+    else if (a.padded <= 2048 && rows < 512) qlin::launch<8, 1>(a);
     else if (a.padded <= 2048) qlin::launch<4, 2>(a);
     else if (a.padded <= 4096 && rows < 512) qlin::launch<16, 1>(a);
     else if (a.padded <= 4096) qlin::launch<8, 2>(a);

@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     const double heat = heat_of(t);
     int x = -1;
     float u_x = 0.0f, l_p = -INFINITY, l_q = -INFINITY;
-    if (wave == 0 && lane < n) {  // a draft a lane
+    if (wave == 0 && lane < D) {  // a draft a lane, also those that n_drafts leaves out: it is still on its way
         x = a.drafts[static_cast<size_t>(seq) * D + lane];
         u_x = uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + lane]);
         if (x >= 0 && x < a.vocab) {
@@ -313,10 +313,10 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     if (tid < 32) sh.steps[tid] = step_of(tid);
     __syncthreads();
     const Stat *stats = a.stats + static_cast<size_t>(seq) * (2 * D + 1) * a.slices;
-    const int rows = DRAFT ? 2 * n + 1 : n + 1;  // the target's n + 1, then the drafts'
+    // the target's rows, then the drafts' (of rows that are not there: anything, which is not used)
 #pragma unroll 1
-    for (int r = wave; r < rows; r += kDecideThreads / 64) {
-        const Stat *of = stats + static_cast<size_t>(r <= n ? r : D + r - n) * a.slices;
+    for (int r = wave; r < (DRAFT ? 2 * D + 1 : D + 1); r += kDecideThreads / 64) {
+        const Stat *of = stats + static_cast<size_t>(r) * a.slices;
         float top = -INFINITY;
         int at = 0;
         double sum = 0.0;
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
                 }
             }
             if (DRAFT && token) {
-                const Stat q = s_row[n + 1 + lane];
+                const Stat q = s_row[D + 1 + lane];
                 qx = !(q.top > -inf) ? 0.0 : greedy ? (x == q.at ? 1.0 : 0.0) : weight(l_q, q.top, heat, sh.steps) / q.sum;
             }
             ok = static_cast<double>(u_x) * qx < px;
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
             a.tokens[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? x : -1;
             if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? static_cast<float>(log_px) : 0.0f;
         }
-        const int rejected = __shfl(x, m, 64);  // (-1 where all were accepted)
+        const int rejected = __shfl(x, m, 64);  // (not used where all were accepted)
         if (lane == 0) {
             a.accepted[seq] = m;
             s_accepted = m;
@@ -385,9 +385,9 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     const Stat p = s_row[m];
     const bool some = p.top > -INFINITY;
     if (DRAFT) {
-        const bool rest = some && !greedy && m < n && s_row[n + 1 + m].top > -INFINITY;
+        const bool rest = some && !greedy && m < n && s_row[D + 1 + m].top > -INFINITY;
         if (tid == 0) {
-            const Stat q = s_row[rest ? n + 1 + m : m];
+            const Stat q = s_row[rest ? D + 1 + m : m];
             a.rests[seq] = Rest{1.0 / p.sum, 1.0 / q.sum, heat, p.top, q.top, rest ? m : -1};
         }
         if (rest) return;  // uniform
@@ -454,17 +454,18 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a)
     __shared__ Shared<kDrawThreads> sh;
     const int seq = blockIdx.x, D = a.max_drafts;
     const Rest r = a.rests[seq];
+    // (requested before it is known whether there is anything to draw)
+    const double sum = static_cast<int>(threadIdx.x) < a.slices ? a.rest_sums[static_cast<size_t>(seq) * a.slices + threadIdx.x] : 0.0;
     if (r.row < 0) return;  // uniform
     if (threadIdx.x < 32) sh.steps[threadIdx.x] = step_of(threadIdx.x);
     const float *p = target_row(a, seq, r.row), *q = draft_row(a, seq, r.row);
-    const double *sums = a.rest_sums + static_cast<size_t>(seq) * a.slices;
     const double u = static_cast<double>(uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + D]));
     const float t = temperature_of(a, seq);
     const Stat *of = a.stats + (static_cast<size_t>(seq) * (2 * D + 1) + r.row) * a.slices;
     __syncthreads();
     // all: where p is nowhere above q
     const int token = draw_row<kDrawThreads, U>(a, u, [&](int k, bool all) {
-        return all ? of[k].sum * weight(of[k].top, r.top_p, r.heat, sh.steps) : sums[k];
+        return all ? of[k].sum * weight(of[k].top, r.top_p, r.heat, sh.steps) : sum;
     }, [&](int v0, int i, int size, bool all, double (&w)[U]) {
         float x[U], y[U];
         logits_of(p + v0, i, size, x);

@@ -194,11 +194,14 @@ typedef struct qlin_logits_controls {
  * The adapters stand in slots of max_rank: a [n_adapters, max_rank, in_dim] and b [n_adapters, out_dim, max_rank] of
  * weight_type 0 (bf16), 1 (f16) or 2 (f32).  ranks [n_adapters] (NULL: max_rank each; clamped to 0 .. max_rank) says how
  * much of a slot counts: the rest is not used, whatever it holds.  scales [n_adapters] or NULL (1).
- * Accuracy: products of exact operands, sums in f32; A x is held in f32, then multiplied by the scale.
+ * Accuracy: exact products, sums in f32; A x is held in f32, then multiplied by the scale, and base is added to the sum in one
+ * step.  bf16 and f16 weights are below 2^30 in magnitude, and sums of |A x| and |B z| below 2^100 (f32 weights, or an x or z of 2^60
+ * or more: as far as f32 holds); an infinite weight gives NaN.  Infinities and NaN of x stay in their rows.
  * n_adapters >= 1, in_dim and max_rank are multiples of 8, from 8 on (else QLIN_ERR_SHAPE), max_rank <= 256, n_adapters <= 1024 and rows <= 65536 (else
  * QLIN_ERR_LIMIT); a and b 16-byte aligned, the rest 4-byte (else QLIN_ERR_ALIGN).  Strides in floats, >= the row.
  * workspace: qlin_lora_workspace_bytes(...) bytes, 16-byte aligned, used by nothing else while the launches run (calls
  * on one stream, or graphs that are not replayed at the same time, may share it); its contents do not matter before or after.
+ * Fewer rows can take more of it.
  */
 typedef struct qlin_lora {
     const void *a, *b;
