@@ -45,6 +45,7 @@ struct Rest {
     double heat;          // 32 / (T ln 2)
     float top_p, top_q;
     int row;              // -1: nothing is left
+    int whole;            // drawn from p alone
 };
 
 struct VerifyArgs {
@@ -247,10 +248,9 @@ __device__ __forceinline__ Pick draw(const double (&w)[U], int each, Goal goal_o
 // The whole draw of a row from given sums of its slices: slice_weight(k, all) and token_weights(first, i, n, all, w).  all: not
 // without what is taken out, where nothing else has a weight.
 template <int N, int U, class Slice, class Tokens>
-__device__ __forceinline__ int draw_row(const VerifyArgs &a, double u, Slice slice_weight, Tokens token_weights, Shared<N> &sh) {
+__device__ __forceinline__ int draw_row(const VerifyArgs &a, double u, Slice slice_weight, Tokens token_weights, Shared<N> &sh, bool all = false) {
     int slice = -1;
     double goal = 0.0;
-    bool all = false;
 #pragma unroll 1
     for (;;) {  // (in one piece of code: instructions that are met once cost more time than the arithmetic)
         double w[U];
@@ -385,29 +385,31 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     const Stat p = s_row[m];
     const bool some = p.top > -INFINITY;
     if (DRAFT) {
-        const bool rest = some && !greedy && m < n && s_row[D + 1 + m].top > -INFINITY;
+        const bool due = some && !greedy, rest = m < n && s_row[D + 1 + m].top > -INFINITY;
         if (tid == 0) {
             const Stat q = s_row[rest ? D + 1 + m : m];
-            a.rests[seq] = Rest{1.0 / p.sum, 1.0 / q.sum, heat, p.top, q.top, rest ? m : -1};
+            a.rests[seq] = Rest{1.0 / p.sum, 1.0 / q.sum, heat, p.top, q.top, due ? m : -1, !rest};
         }
-        if (rest) return;  // uniform
+        if (due) return;  // uniform
     }
     const float *row = target_row(a, seq, m);
     int token = p.at;  // (0 where the row has nothing)
-    if (some && !greedy) {
-        // the target's own weights, without the rejected token of a draft by lookup
-        const Stat *of = stats + static_cast<size_t>(m) * a.slices;
-        const int out = !DRAFT && m < n && s_rejected < a.vocab ? s_rejected : -1;
-        const double taken = out >= 0 ? weight(number(row[out]), p.top, heat, sh.steps) : 0.0;
-        token = draw_row<kDecideThreads, U>(a, u, [&](int k, bool all) {
-            const double w = of[k].sum * weight(of[k].top, p.top, heat, sh.steps);
-            return !all && out >= 0 && out / a.slice == k ? fmax(w - taken, 0.0) : w;
-        }, [&](int v0, int i, int size, bool all, double (&w)[U]) {
-            float l[U];
-            logits_of(row + v0, i, size, l);
+    if constexpr (!DRAFT) {
+        if (some && !greedy) {
+            // the target's own weights, without the rejected token of a draft by lookup
+            const Stat *of = stats + static_cast<size_t>(m) * a.slices;
+            const int out = m < n && s_rejected < a.vocab ? s_rejected : -1;
+            const double taken = out >= 0 ? weight(number(row[out]), p.top, heat, sh.steps) : 0.0;
+            token = draw_row<kDecideThreads, U>(a, u, [&](int k, bool all) {
+                const double w = of[k].sum * weight(of[k].top, p.top, heat, sh.steps);
+                return !all && out >= 0 && out / a.slice == k ? fmax(w - taken, 0.0) : w;
+            }, [&](int v0, int i, int size, bool all, double (&w)[U]) {
+                float l[U];
+                logits_of(row + v0, i, size, l);
 #pragma unroll
-            for (int e = 0; e < U; ++e) w[e] = !all && v0 + i + e == out ? 0.0 : weight(l[e], p.top, heat, sh.steps);
-        }, sh);
+                for (int e = 0; e < U; ++e) w[e] = !all && v0 + i + e == out ? 0.0 : weight(l[e], p.top, heat, sh.steps);
+            }, sh);
+        }
     }
     if (tid == 0) {
         a.tokens[static_cast<size_t>(seq) * (D + 1) + m] = token;
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
     __shared__ double s_sum[kWaves], s_steps[32];
     const int slice = blockIdx.x % a.slices, seq = blockIdx.x / a.slices, tid = threadIdx.x;
     const Rest r = a.rests[seq];
-    if (r.row < 0) return;  // uniform
+    if (r.row < 0 || r.whole) return;  // uniform
     const int v0 = slice * a.slice, n = min(a.slice, a.vocab - v0);
     const float *p = target_row(a, seq, r.row) + v0, *q = draft_row(a, seq, r.row) + v0;
     f32x4v x[U], y[U];
@@ -463,16 +465,16 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a)
     const float t = temperature_of(a, seq);
     const Stat *of = a.stats + (static_cast<size_t>(seq) * (2 * D + 1) + r.row) * a.slices;
     __syncthreads();
-    // all: where p is nowhere above q
+    // all: from p, as where p is nowhere above q
     const int token = draw_row<kDrawThreads, U>(a, u, [&](int k, bool all) {
         return all ? of[k].sum * weight(of[k].top, r.top_p, r.heat, sh.steps) : sum;
     }, [&](int v0, int i, int size, bool all, double (&w)[U]) {
         float x[U], y[U];
         logits_of(p + v0, i, size, x);
-        logits_of(q + v0, i, size, y);
+        if (!all) logits_of(q + v0, i, size, y);  // uniform
 #pragma unroll
         for (int e = 0; e < U; ++e) w[e] = all ? weight(x[e], r.top_p, r.heat, sh.steps) : rest_weight(r, x[e], y[e], sh.steps);
-    }, sh);
+    }, sh, r.whole != 0);
     if (threadIdx.x == 0) {
         a.tokens[static_cast<size_t>(seq) * (D + 1) + r.row] = token;
         if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + r.row] = static_cast<float>(log_of(number(p[token]), r.top_p, t) + log(r.inv_p));
