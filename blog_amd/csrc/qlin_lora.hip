@@ -14,7 +14,12 @@
 // 2^26 v of an f32 value v is the sum of three (8 bits each; with the factor, which leaves with the sum, all parts of any v are
 // normal numbers).  Where a |v| is 2^60 or more (or infinite) these would overflow, and what is left goes to
 // v_mfma_f32_16x16x4_f32, a uniform and rare branch; f32 weights go there always.  (All types there: 613 rows of 18944 to 3584
-// at rank 64 63.3 and 57.4 us in the two launches, where they now take 26.2 and 17.4.)
+// with 8 adapters of rank 64 in f16 63.3 and 57.4 us in the two launches, where they take 25.3 and 14.0.)
+//
+// Few rows are bound by latency: one row of 896 to 896, 128 and 128 at rank 16 takes 9.7 us in a graph, 48 rows of 3584 to 3584,
+// 512 and 512 with 15 adapters of rank 32 15.8.  Many are bound by memory in the second launch (2011 rows of 4096 to 14336 at rank
+// 64: 230 MB of base and y, 55.7 us, 4.1 TB/s, 77.2 in all) and in the first by what a wave has to do between its loads: x into
+// three parts and f16 weights into two take the vector unit 40 of 100 cycles, the products the matrix unit 20.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -67,7 +72,7 @@ __device__ __forceinline__ int rank_of(const LoraArgs &a, int id) { return a.ran
 // Loads and stores.  Eight lanes take a line of 128 bytes, a wave 8 rows, so that no line is met by two instructions: the second
 // would wait in the first level cache for the first one's miss, with all that comes after it.  (The lanes as the matrix cores
 // take them, row l % 16 and the values 8 (l / 16) .., 2011 rows of 4096 to 14336 at rank 64 took 19.5 and 78.6 us, with the cache
-// stalled for two thirds of it; four lanes to half a line 20.1 and 73.3.)  What is loaded changes lanes through LDS of the
+// stalled for two thirds of it; four lanes to half a line 20.1 and 73.3; so 16.9 and 61.)  What is loaded changes lanes through LDS of the
 // wave's own, rows 144 bytes apart, so that 16 lanes with 16 bytes of 16 rows meet all banks.
 constexpr int kLine = 128, kRowBytes = kLine + 16;
 
@@ -217,7 +222,7 @@ __device__ __forceinline__ Group find_tile(const LoraArgs &a, int tile, LaneRows
 static_assert(kFewRows == 256, "find_tile has four registers of rows");
 
 // More rows: one workgroup counts each adapter's rows, gives it its tiles and puts the rows into them.  (In what order does
-// not matter: a row's results do not depend on its tile.)
+// not matter: a row's results do not depend on its place.)
 constexpr int kGroupThreads = 1024, kKept = 4;  // rows a thread whose places are kept in registers
 __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
     __shared__ int s_count[kMostAdapters + 1], s_tile[kMostAdapters + 1], s_wave[kGroupThreads / 64];
@@ -792,7 +797,7 @@ Layout layout_of(int rows, int n_mats, int n_adapters, int max_rank, int in_dim)
     l.groups = (max_rank + kRanks - 1) / kRanks;
     // slices of x: as many as give about 512 workgroups, but each is stored apart and read by every run of outputs, so that a
     // wave has 8 steps of 32 values at least, 2 of few rows, where it is latency that counts (2011 rows of 4096 to 14336 in 8
-    // slices of 4 steps 85.0 us, in 4 of 8 82.2; 613 rows of 18944 to 3584 in 16 44.7, in 8 47.5)
+    // slices of 4 steps 85.0 us, in 4 of 8 82.2); 16 at most (613 rows of 18944 to 3584 in 8 47.5 us, in 16 43.1, in 18 to 32 45.5)
     const int steps = (in_dim + 31) / 32, least = few ? 2 : 8;
     const int64_t tiles = few ? l.most_tiles : (rows + kPart - 1) / kPart;
     l.splits = static_cast<int>(512 / (tiles * n_mats * l.groups));

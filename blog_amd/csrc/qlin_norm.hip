@@ -9,8 +9,8 @@
 // one Q8_1 block.  Rows that do not fit (U = 0) are read a second time, each value by the lane that wrote or read it before, so
 // that outputs may take the inputs' place.  Many rows are bound by HBM: 2011 rows of 4096 with their sum and blocks of 128 and
 // the blocks read back, 151 MB, take 35.8 us in a graph (4.2 TB/s; 4 waves of 4 runs 38.0, 16 of one 36.9), 42.1 with f32 results
-// through the caches: from 16 MB on they leave as streaming stores.  Few rows are bound by latency, and 16 waves take a row of
-// 3584 in 4.5 us, 4 waves in 6.4.
+// through the caches: from 16 MB on they leave as streaming stores.  Few rows are bound by latency: 16 waves take a row of 3584 in
+// 4.4 us, 4 waves in 6.4; 48 rows of 2048 with f32 results and blocks take 4.0 by 8 waves each, 5.0 by 4.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
