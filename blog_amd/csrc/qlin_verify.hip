@@ -314,22 +314,27 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
         }
     }
     const double u = static_cast<double>(uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + D]));
+    const Stat *stats = a.stats + static_cast<size_t>(seq) * (2 * D + 1) * a.slices;
+    const int rows = DRAFT ? 2 * D + 1 : D + 1;
+    const Stat none = {0.0, -INFINITY, 0};
+    Stat next = wave < rows && lane < a.slices ? stats[static_cast<size_t>(wave) * a.slices + lane] : none;
     if (tid < 32) sh.steps[tid] = step_of(tid);
     __syncthreads();
-    const Stat *stats = a.stats + static_cast<size_t>(seq) * (2 * D + 1) * a.slices;
     // the target's rows, then the drafts' (of rows that are not there: anything, which is not used)
 #pragma unroll 1
-    for (int r = wave; r < (DRAFT ? 2 * D + 1 : D + 1); r += kDecideThreads / 64) {
+    for (int r = wave; r < rows;) {
         const Stat *of = stats + static_cast<size_t>(r) * a.slices;
+        const Stat mine = next;
         float top = -INFINITY;
         int at = 0;
         double sum = 0.0;
         if (greedy) {
+            top = mine.top;
+            at = mine.at;
 #pragma unroll 1
-            for (int k = lane; k < a.slices; k += 64) better(top, at, of[k].top, of[k].at);
+            for (int k = lane + 64; k < a.slices; k += 64) better(top, at, of[k].top, of[k].at);
             wave_best(top, at);
         } else {
-            const Stat mine = lane < a.slices ? of[lane] : Stat{0.0, -INFINITY, 0};  // (read once)
             top = mine.top;
 #pragma unroll 1
             for (int k = lane + 64; k < a.slices; k += 64) top = fmaxf(top, of[k].top);
@@ -345,6 +350,8 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
             sum = wave_sum_f64(sum);
         }
         if (lane == 0) s_row[r] = Stat{sum, top, at};
+        r += kDecideThreads / 64;
+        next = r < rows && lane < a.slices ? stats[static_cast<size_t>(r) * a.slices + lane] : none;
     }
     __syncthreads();
     if (wave == 0) {
