@@ -191,62 +191,59 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
 
 template <int N>
 struct Shared {
-    double steps[32], part[N / 64], base;
-    int found[3];
+    double steps[32], part[2][N / 64], base[2];
+    int found[2];
 };
+__device__ __forceinline__ double of_lane(double v, int lane) {  // (uniform)
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return halves(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane)),
+                  static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), lane)));
+}
 
 // A draw by N threads: from the slices of a row, then from the tokens of a slice.  Thread t has the weights w (>= 0) of the
 // items t U .. t U + U - 1 (of a slice each one item, in w[0]).  The first item at which the running sum is above goal(total); where
 // rounding leaves none, the last one with a weight; -1 where there is no weight at all.  base: the running sum before it.
-// (A thread's sum and its walk add the same numbers from another start, so a goal can lie beyond the walk's end by a
+// Every wave finds the wave that has the item, from the waves' sums, and that wave finds the item: two barriers (a search by
+// all threads between four took 1 us more).  turn: draws that follow one another take the halves of sh in turn.
+// (A wave's, a thread's and a walk's sums add the same numbers from other starts, so that a goal can lie beyond the last one by a
 // rounding: then the last item with a weight.)
 struct Pick {
     int at;
     double base, total;
 };
 template <int N, int U, class Goal>
-__device__ __forceinline__ Pick draw(const double (&w)[U], int each, Goal goal_of, Shared<N> &sh) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ Pick draw(const double (&w)[U], int each, Goal goal_of, Shared<N> &sh, int turn) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     double mine = 0.0;
 #pragma unroll
     for (int e = 0; e < U; ++e) mine += w[e];
-    double run = wave_scan_f64(mine);
-    __syncthreads();  // (sh's readers of before are done)
-    if (lane == 63) sh.part[wave] = run;
-    if (tid == 0) {
-        sh.found[0] = 0x7fffffff;  // the first thread whose items pass the goal
-        sh.found[1] = -1;          // the last thread with a weight
-        sh.found[2] = -1;
-    }
+    const double run = wave_scan_f64(mine);
+    if (lane == 63) sh.part[turn][wave] = run;
     __syncthreads();
-    double start = 0.0, total = 0.0;
+    const double part = lane < N / 64 ? sh.part[turn][lane] : 0.0;
+    const double upto = wave_scan_f64(part);
+    const double total = of_lane(upto, 63), goal = goal_of(total);
+    const uint64_t some = __ballot(part > 0.0), past = __ballot(part > 0.0 && upto > goal);
+    if (!some) return Pick{-1, 0.0, total};  // (the same in every wave)
+    if (wave == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some))) {
+        const double before = wave > 0 ? of_lane(upto, wave - 1) : 0.0;
+        const uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && before + run > goal);
+        if (lane == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some))) {
+            double at = before + (run - mine);
+            bool done = false;
 #pragma unroll
-    for (int v = 0; v < N / 64; ++v) {
-        if (v < wave) start += sh.part[v];
-        total += sh.part[v];
-    }
-    start += run - mine;
-    const double goal = goal_of(total);
-    const uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && start + mine > goal);
-    if (past && lane == static_cast<int>(__ffsll(static_cast<long long>(past))) - 1) atomicMin(&sh.found[0], tid);
-    if (some && lane == 63 - static_cast<int>(__clzll(static_cast<long long>(some)))) atomicMax(&sh.found[1], tid);
-    __syncthreads();
-    const int who = sh.found[0] != 0x7fffffff ? sh.found[0] : sh.found[1];
-    if (who == tid) {
-        run = start;
-        bool done = false;
-#pragma unroll
-        for (int e = 0; e < U; ++e) {
-            if (w[e] > 0.0 && !done) {
-                sh.found[2] = tid * each + e;
-                sh.base = run;
-                done = run + w[e] > goal;
+            for (int e = 0; e < U; ++e) {
+                if (w[e] > 0.0 && !done) {
+                    sh.found[turn] = tid * each + e;
+                    sh.base[turn] = at;
+                    done = at + w[e] > goal;
+                }
+                at += w[e];
             }
-            run += w[e];
         }
     }
     __syncthreads();
-    return Pick{sh.found[2], sh.base, total};
+    return Pick{sh.found[turn], sh.base[turn], total};
 }
 
 // The whole draw of a row from given sums of its slices: slice_weight(k, all) and token_weights(first, i, n, all, w).  all: not
@@ -256,7 +253,7 @@ __device__ __forceinline__ int draw_row(const VerifyArgs &a, double u, Slice sli
     int slice = -1;
     double goal = 0.0;
 #pragma unroll 1
-    for (;;) {  // (in one piece of code: instructions that are met once cost more time than the arithmetic)
+    for (int turn = 0;; turn ^= 1) {  // (in one piece of code: instructions that are met once cost more time than the arithmetic)
         double w[U];
         if (slice < 0) {
 #pragma unroll
@@ -265,7 +262,7 @@ __device__ __forceinline__ int draw_row(const VerifyArgs &a, double u, Slice sli
         } else {
             token_weights(slice * a.slice, static_cast<int>(threadIdx.x) * U, min(a.slice, a.vocab - slice * a.slice), all, w);
         }
-        const Pick k = draw<N, U>(w, slice < 0 ? 1 : U, [&](double total) { return slice < 0 ? u * total : goal; }, sh);
+        const Pick k = draw<N, U>(w, slice < 0 ? 1 : U, [&](double total) { return slice < 0 ? u * total : goal; }, sh, turn);
         if (slice >= 0) return slice * a.slice + max(k.at, 0);
         if (k.at < 0) {  // uniform
             if (all) return 0;
