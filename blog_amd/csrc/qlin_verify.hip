@@ -313,42 +313,46 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     const double u = static_cast<double>(uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + D]));
     const Stat *stats = a.stats + static_cast<size_t>(seq) * (2 * D + 1) * a.slices;
     const int rows = DRAFT ? 2 * D + 1 : D + 1;
-    const Stat none = {0.0, -INFINITY, 0};
-    Stat next = wave < rows && lane < a.slices ? stats[static_cast<size_t>(wave) * a.slices + lane] : none;
+    constexpr int kAhead = U == 1 ? 3 : 1;  // slices of a row a lane; more are read one after the other
+    Stat next[kAhead];
+    auto load = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            next[i] = stats[static_cast<size_t>(min(r, rows - 1)) * a.slices + min(lane + 64 * i, a.slices - 1)];
+            if (lane + 64 * i >= a.slices) next[i] = Stat{0.0, -INFINITY, 0};
+        }
+    };
+    load(wave);
     if (tid < 32) sh.steps[tid] = step_of(tid);
     __syncthreads();
     // the target's rows, then the drafts' (of rows that are not there: anything, which is not used)
 #pragma unroll 1
     for (int r = wave; r < rows;) {
         const Stat *of = stats + static_cast<size_t>(r) * a.slices;
-        const Stat mine = next;
-        float top = -INFINITY;
-        int at = 0;
+        float top = next[0].top;
+        int at = next[0].at;
         double sum = 0.0;
         if (greedy) {
-            top = mine.top;
-            at = mine.at;
+#pragma unroll
+            for (int i = 1; i < kAhead; ++i) better(top, at, next[i].top, next[i].at);
 #pragma unroll 1
-            for (int k = lane + 64; k < a.slices; k += 64) better(top, at, of[k].top, of[k].at);
+            for (int k = lane + 64 * kAhead; k < a.slices; k += 64) better(top, at, of[k].top, of[k].at);
             wave_best(top, at);
         } else {
-            top = mine.top;
+#pragma unroll
+            for (int i = 1; i < kAhead; ++i) top = fmaxf(top, next[i].top);
 #pragma unroll 1
-            for (int k = lane + 64; k < a.slices; k += 64) top = fmaxf(top, of[k].top);
+            for (int k = lane + 64 * kAhead; k < a.slices; k += 64) top = fmaxf(top, of[k].top);
             top = wave_max_dpp(top);
-            Stat s = mine;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) sum += next[i].sum * weight(next[i].top, top, heat, sh.steps);
 #pragma unroll 1
-            for (int k = lane;;) {
-                sum += s.sum * weight(s.top, top, heat, sh.steps);
-                k += 64;
-                if (k >= a.slices) break;
-                s = of[k];
-            }
+            for (int k = lane + 64 * kAhead; k < a.slices; k += 64) sum += of[k].sum * weight(of[k].top, top, heat, sh.steps);
             sum = wave_sum_f64(sum);
         }
         if (lane == 0) s_row[r] = Stat{sum, top, at};
         r += kDecideThreads / 64;
-        next = r < rows && lane < a.slices ? stats[static_cast<size_t>(r) * a.slices + lane] : none;
+        load(r);
     }
     __syncthreads();
     if (wave == 0) {
