@@ -47,6 +47,7 @@ struct Stat {
 struct Rest {
     double inv_p, inv_q;  // one over the sums
     double heat;          // 32 / (T ln 2)
+    double log_p;         // of p's sum
     float top_p, top_q;
     int row;              // -1: nothing is left
     int whole;            // drawn from p alone
@@ -294,6 +295,7 @@ template <int U, bool DRAFT>
 __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArgs a) {
     __shared__ Stat s_row[2 * kMostDrafts + 1];
     __shared__ Shared<kDecideThreads> sh;
+    __shared__ double s_log[kMostDrafts + 1];  // of the sums
     __shared__ int s_accepted, s_rejected;
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = drafts_of(a, seq), D = a.max_drafts;
@@ -302,7 +304,8 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     const double heat = heat_of(t);
     int x = -1;
     float u_x = 0.0f, l_p = -INFINITY, l_q = -INFINITY;
-    if (wave == 0 && lane < D) {  // a draft a lane, also those that n_drafts leaves out: it is still on its way
+    double log_px = 0.0;
+    if (wave < 2 && lane < D) {  // a draft a lane, also those that n_drafts leaves out: it is still on its way
         x = a.drafts[static_cast<size_t>(seq) * D + lane];
         u_x = uniform_at(a.uniform[static_cast<size_t>(seq) * (D + 1) + lane]);
         if (x >= 0 && x < a.vocab) {
@@ -358,19 +361,12 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     if (wave == 0) {
         const float inf = INFINITY;
         bool ok = false;
-        double px = 0.0, log_px = 0.0;
+        double px = 0.0;
         if (lane < n) {
             const bool token = x >= 0 && x < a.vocab;
             const Stat p = s_row[lane];
             double qx = token ? 1.0 : 0.0;
-            if (token && p.top > -inf) {
-                if (greedy) {
-                    px = x == p.at ? 1.0 : 0.0;
-                } else {
-                    px = weight(l_p, p.top, heat, sh.steps) / p.sum;
-                    if (a.logprobs) log_px = log_of(l_p, p.top, t) - log(p.sum);
-                }
-            }
+            if (token && p.top > -inf) px = greedy ? (x == p.at ? 1.0 : 0.0) : weight(l_p, p.top, heat, sh.steps) / p.sum;
             if (DRAFT && token) {
                 const Stat q = s_row[D + 1 + lane];
                 qx = !(q.top > -inf) ? 0.0 : greedy ? (x == q.at ? 1.0 : 0.0) : weight(l_q, q.top, heat, sh.steps) / q.sum;
@@ -381,26 +377,32 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
             a.rates[static_cast<size_t>(seq) * D + lane] = 0.0f;
         }
         const int m = static_cast<int>(__ffsll(static_cast<long long>(~__ballot(ok)))) - 1;  // (lane 63 has no draft)
-        if (lane <= D && lane != m) {
-            a.tokens[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? x : -1;
-            if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? static_cast<float>(log_px) : 0.0f;
-        }
+        if (lane <= D && lane != m) a.tokens[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? x : -1;
         const int rejected = __shfl(x, m, 64);  // (not used where all were accepted)
         if (lane == 0) {
             a.accepted[seq] = m;
             s_accepted = m;
             s_rejected = rejected;
         }
+    } else if (wave == 1 && a.logprobs && !greedy) {  // (beside the above, which it would hold up)
+        if (lane <= n) {
+            const Stat p = s_row[lane];
+            const double log_sum = log(p.sum);
+            s_log[lane] = log_sum;
+            if (lane < n) log_px = log_of(l_p, p.top, t) - log_sum;  // (of an accepted draft, which p has)
+        }
     }
     __syncthreads();
     const int m = s_accepted;
+    if (wave == 1 && a.logprobs && lane <= D && lane != m)
+        a.logprobs[static_cast<size_t>(seq) * (D + 1) + lane] = lane < m ? static_cast<float>(log_px) : 0.0f;
     const Stat p = s_row[m];
     const bool some = p.top > -INFINITY;
     if (DRAFT) {
         const bool due = some && !greedy, rest = m < n && s_row[D + 1 + m].top > -INFINITY;
         if (tid == 0) {
             const Stat q = s_row[rest ? D + 1 + m : m];
-            a.rests[seq] = Rest{1.0 / p.sum, 1.0 / q.sum, heat, p.top, q.top, due ? m : -1, !rest};
+            a.rests[seq] = Rest{1.0 / p.sum, 1.0 / q.sum, heat, s_log[m], p.top, q.top, due ? m : -1, !rest};
         }
         if (due) return;  // uniform
     }
@@ -426,7 +428,7 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
     if (tid == 0) {
         a.tokens[static_cast<size_t>(seq) * (D + 1) + m] = token;
         if (a.logprobs) {
-            const float log_p = static_cast<float>(log_of(number(row[token]), p.top, t) - log(p.sum));
+            const float log_p = static_cast<float>(log_of(number(row[token]), p.top, t) - s_log[m]);
             a.logprobs[static_cast<size_t>(seq) * (D + 1) + m] = !some ? -INFINITY : greedy ? 0.0f : log_p;
         }
     }
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(VerifyArgs a)
     }, sh, r.whole != 0);
     if (threadIdx.x == 0) {
         a.tokens[static_cast<size_t>(seq) * (D + 1) + r.row] = token;
-        if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + r.row] = static_cast<float>(log_of(number(p[token]), r.top_p, t) + log(r.inv_p));
+        if (a.logprobs) a.logprobs[static_cast<size_t>(seq) * (D + 1) + r.row] = static_cast<float>(log_of(number(p[token]), r.top_p, t) - r.log_p);
     }
 }
 
