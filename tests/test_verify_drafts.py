@@ -209,6 +209,22 @@ def test_verify_large(n, d, vocab, with_draft):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [196608, 196609, 400003, 524288])
+@pytest.mark.parametrize("with_draft", [False, True])
+def test_few_rows_of_many_slices(vocab, with_draft):
+    torch = _gpu()
+    from gpu_util import banner
+    rng = np.random.default_rng(vocab)
+    banner(f"verify_drafts vocab={vocab} 2 sequences, draft logits={with_draft}")
+    a = _case(rng, 2, 1, vocab, with_draft)
+    for temperature in ([0.0, 0.8], [0.9, 0.0]):
+        a["temperature"] = np.array(temperature, np.float32)
+        for u in (0.0, 0.5, NEXT):
+            a["uniform"][:, 1] = u
+            _check(torch, a)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("with_draft", [False, True])
 def test_odd_values(with_draft):
     """Masked tokens, rows that a mask leaves empty, infinities and NaN, ties, drafts outside the vocabulary, random numbers at
