@@ -8,7 +8,7 @@
 // A row is taken by W waves, 4 consecutive values a lane and U such runs in registers, so that x is read once; 8 lanes hold
 // one Q8_1 block.  Rows that do not fit (U = 0) are read a second time, each value by the lane that wrote or read it before, so
 // that outputs may take the inputs' place.  Many rows are bound by HBM: 2011 rows of 4096 with their sum and blocks of 128 and
-// the blocks read back, 151 MB, take 35.8 us in a graph (4.2 TB/s; 4 waves of 4 runs 38.0, 16 of one 36.9), 42.1 with f32 results
+// the blocks read back, 150 MB, take 35.1 us in a graph (4.3 TB/s; 8 waves of 2 runs 35.5, 16 of one 37.3), 42 with f32 results
 // through the caches: from 16 MB on they leave as streaming stores.  Few rows are bound by latency: 16 waves take a row of 3584 in
 // 4.4 us, 4 waves in 6.4; 48 rows of 2048 with f32 results and blocks take 4.0 by 8 waves each, 5.0 by 4.
 #include <hip/hip_runtime.h>
@@ -91,12 +91,12 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(Norm
     float *sum = a.sum ? a.sum + row * a.sum_stride : nullptr;
     float *normed = a.normed ? a.normed + row * a.normed_stride : nullptr;
     double ss = 0.0;
-    auto take = [&](int i) {  // s of values i .. i + 3, stored and squared
+    auto take = [&](int i) {  // s of values i .. i + 3
         f32x4v s = values_at(x, i, a.hidden);
         if (delta) s += values_at(delta, i, a.hidden);
         return s;
     };
-    auto count = [&](int i, const f32x4v &s) {
+    auto count = [&](int i, const f32x4v &s) {  // stored and squared
         if (sum) store_values<STREAM>(sum, i, a.hidden, s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ss += static_cast<double>(s[e]) * static_cast<double>(s[e]);
@@ -106,7 +106,14 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void add_rms_norm_kernel(Norm
     uint2 w[K];
     if constexpr (U > 0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) s[u] = take(4 * (t + N * u));
+        for (int u = 0; u < U; ++u) s[u] = values_at(x, 4 * (t + N * u), a.hidden);
+        if (delta) {  // uniform; asked for all at once, as x
+            f32x4v d[K];
+#pragma unroll
+            for (int u = 0; u < U; ++u) d[u] = values_at(delta, 4 * (t + N * u), a.hidden);
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] += d[u];
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) w[u] = weights_at(a.w, 4 * (t + N * u), a.hidden);
 #pragma unroll
@@ -222,7 +229,7 @@ int qlin_launch_add_rms_norm(const float *x, size_t x_stride, const float *delta
     else if (a.padded <= 2048 && rows < 512) qlin::launch<8, 1>(a);
     else if (a.padded <= 2048) qlin::launch<4, 2>(a);
     else if (a.padded <= 4096 && rows < 512) qlin::launch<16, 1>(a);
-    else if (a.padded <= 4096) qlin::launch<8, 2>(a);
+    else if (a.padded <= 4096) qlin::launch<4, 4>(a);
     else if (a.padded <= 8192) qlin::launch<16, 2>(a);
     else if (a.padded <= 16384) qlin::launch<16, 4>(a);
     else qlin::launch<16, 0>(a);
