@@ -43,9 +43,13 @@ constexpr int kPart = 32;       // of a workgroup of lora_down_kernel
 constexpr int kRanks = 64;      // of a workgroup of lora_down_kernel
 constexpr int kMostAdapters = 1024;
 
-// Rows that have one adapter (-1: none), in the workspace.
-struct Tile {
-    int adapter, count, pad[2];
+// Rows that have one adapter (-1: none), with its rank and scale; no rows: no such tile.
+struct Group {
+    int adapter, count, rank;
+    float scale;
+};
+struct Tile {  // in the workspace
+    Group group;
     int rows[kTile];
 };
 
@@ -57,7 +61,7 @@ struct LoraArgs {
     int *n_tiles;
     float *z;  // [splits][n_mats][rows][max_rank]
     size_t x_stride;
-    int n_mats, n_adapters, max_rank, in_dim, rows, splits;
+    int n_mats, n_adapters, max_rank, in_dim, rows, splits, most_tiles;
     int copies;  // whether rows without an adapter are copied (somewhere y is not base)
     int chunk, chunks[kMostMats];  // outputs of a workgroup of lora_up_kernel, and their runs up to and with each projection
 };
@@ -68,6 +72,9 @@ __device__ __forceinline__ int slot_of(const LoraArgs &a, int row) {
     return id >= 0 && id < a.n_adapters ? id : a.copies ? a.n_adapters : -1;
 }
 __device__ __forceinline__ int rank_of(const LoraArgs &a, int id) { return a.ranks ? min(max(a.ranks[id], 0), a.max_rank) : a.max_rank; }
+__device__ __forceinline__ Group group_of(const LoraArgs &a, int id, int count) {
+    return id < a.n_adapters ? Group{id, count, rank_of(a, id), a.scales ? a.scales[id] : 1.0f} : Group{-1, count, 0, 1.0f};
+}
 
 // Loads and stores.  Eight lanes take a line of 128 bytes, a wave 8 rows, so that no line is met by two instructions: the second
 // would wait in the first level cache for the first one's miss, with all that comes after it.  (The lanes as the matrix cores
@@ -169,9 +176,6 @@ struct LaneRows {
     int row;
     __device__ __forceinline__ int operator()(int i) const { return __builtin_amdgcn_ds_bpermute(4 * i, row); }
 };
-struct Group {
-    int adapter, count;  // -1: no adapter; no rows: no such tile
-};
 // The tile of number `tile` among up to 256 rows, by each wave for itself, 64 rows at a time: adapters in the order of their
 // first rows, an adapter's rows in order, so that every wave finds the same.  No LDS, no barrier: with both and a row a
 // thread one row of 896 to 896, 128 and 128 took 15.3 us in the two launches, so 9.6.
@@ -195,7 +199,7 @@ __device__ __forceinline__ Group find_tile(const LoraArgs &a, int tile, LaneRows
         else if (todo[1]) id = __builtin_amdgcn_readlane(slot[1], __builtin_ctzll(todo[1]));
         else if (todo[2]) id = __builtin_amdgcn_readlane(slot[2], __builtin_ctzll(todo[2]));
         else if (todo[3]) id = __builtin_amdgcn_readlane(slot[3], __builtin_ctzll(todo[3]));
-        else return Group{-1, 0};
+        else return Group{-1, 0, 0, 1.0f};
         count = 0;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
@@ -217,7 +221,7 @@ __device__ __forceinline__ Group find_tile(const LoraArgs &a, int tile, LaneRows
         before += static_cast<int>(__popcll(mine[i]));
     }
     rows.row = max(row - 1, 0);  // (lanes past the last row: another)
-    return Group{id < a.n_adapters ? id : -1, min(16, count - 16 * tile)};
+    return group_of(a, id, min(16, count - 16 * tile));
 }
 static_assert(kFewRows == 256, "find_tile has four registers of rows");
 
@@ -228,6 +232,7 @@ __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
     __shared__ int s_count[kMostAdapters + 1], s_tile[kMostAdapters + 1], s_wave[kGroupThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, kinds = a.n_adapters + 1;
     int slot[kKept], place[kKept];
+    const Group mine = group_of(a, tid, 0);
 #pragma unroll
     for (int i = 0; i < kKept; ++i) slot[i] = tid + i * kGroupThreads < a.rows ? slot_of(a, tid + i * kGroupThreads) : -1;
     for (int i = tid; i < kinds; i += kGroupThreads) s_count[i] = 0;
@@ -269,15 +274,15 @@ __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
         if (w < (tid >> 6)) start += v;
         total += v;
     }
-    auto head = [&](int id, int at, int rows) {
+    auto head = [&](int id, Group of, int at, int rows) {
         s_tile[id] = at;
         for (int t = 0; t * kTile < rows; ++t) {
-            a.tiles[at + t].adapter = id == a.n_adapters ? -1 : id;
-            a.tiles[at + t].count = min(kTile, rows - t * kTile);
+            of.count = min(kTile, rows - t * kTile);
+            a.tiles[at + t].group = of;
         }
     };
-    if (tid < kinds) head(tid, start, count);
-    if (last > 0 && tid == 0) head(kGroupThreads, total, last);
+    if (tid < kinds) head(tid, mine, start, count);
+    if (last > 0 && tid == 0) head(kGroupThreads, Group{-1, 0, 0, 1.0f}, total, last);
     if (tid == 0) *a.n_tiles = total + (last + kTile - 1) / kTile;
     __syncthreads();
 #pragma unroll
@@ -293,6 +298,16 @@ __global__ __launch_bounds__(kGroupThreads) void lora_group_kernel(LoraArgs a) {
     }
 }
 
+// Tile number `tile`, its rows into LDS; no rows where there is no such tile.  (All of it is asked for at once: there is room for
+// most_tiles of them, of which the first n_tiles are filled.)
+__device__ __forceinline__ Group tile_at(const LoraArgs &a, int tile, int *s_rows) {
+    const int n = *a.n_tiles, t = min(tile, a.most_tiles - 1);
+    Group of = a.tiles[t].group;
+    if (threadIdx.x < kTile) s_rows[threadIdx.x] = a.tiles[t].rows[threadIdx.x];
+    if (tile >= n) of.count = 0;
+    return of;
+}
+
 // z of 16 NT rows of a tile from its row `first` on, one projection, one group of ranks and one slice of x.  lds: at least
 // kDownBytes for the workgroup.
 constexpr int kDownRows = 64;  // of LDS a wave: two lines of 32 rows of x, or a line of 64 rows of weights
@@ -302,7 +317,7 @@ template <int T, int NT, class R>
 __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R &rows, int first, int mat, int group, int split, char *lds) {
     constexpr int RT = kRanks / 16, K = Weights<T>::kValues, H = K / 32;  // a step: a line of weights, H lines of x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int rank = rank_of(a, t.adapter) - group * kRanks;
+    const int rank = t.rank - group * kRanks;
     if (rank <= 0) return;  // uniform
     const int tiles = min((rank + 15) / 16, RT);
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -477,14 +492,13 @@ __global__ __launch_bounds__(kThreads, 2) void lora_down_kernel(LoraArgs a) {
         const Group t = find_tile(a, blockIdx.x / units, rows);
         if (t.adapter >= 0) down<T, 1>(a, t, rows, 0, rest % a.n_mats, rest / a.n_mats, split, s_z);
     } else {
-        __shared__ Tile t;
-        const TileRows rows = {t.rows};
-        const int total = *a.n_tiles * units;
-        for (int item = blockIdx.x; item < total; item += gridDim.x) {
-            const int tile = item / units, unit = item % units;
+        __shared__ int s_rows[kTile];
+        const TileRows rows = {s_rows};
+        for (int item = blockIdx.x;; item += gridDim.x) {
+            const int unit = item % units;
             __syncthreads();  // (the tile and the sums of before are read)
-            if (threadIdx.x < kTile) t.rows[threadIdx.x] = a.tiles[tile].rows[threadIdx.x];
-            const Group of = {a.tiles[tile].adapter, a.tiles[tile].count};
+            const Group of = tile_at(a, item / units, s_rows);
+            if (of.count == 0) break;  // uniform
             __syncthreads();
             const int split = unit % a.splits, part = unit / a.splits % (kTile / kPart) * kPart, rest = unit / a.splits / (kTile / kPart);
             if (of.adapter < 0 || part >= of.count) continue;  // uniform
@@ -679,11 +693,10 @@ __device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &r
     const int start = first + 32 * (both ? wave >> 1 : wave);
     const int passes = start < last ? (last - start + step - 1) / step : 0, turn = both && (wave & 1) ? passes / 2 : 0;
     auto at = [&](int i) { i += turn; return start + step * (i < passes ? i : i - passes); };
-    const int rank = t.adapter < 0 ? 0 : rank_of(a, t.adapter);
+    const int rank = t.rank;
     Up<T, NT> up(a, t, rows, mat, from, rank, s_z + wave * kUpBytes);
     if (passes > 0) up.load(at(0));  // (requested before z is staged)
     const int quads = (rank + 31) / 32 * 8;  // of a row
-    const float scale = t.adapter >= 0 && a.scales ? a.scales[t.adapter] : 1.0f;
     const int staged = (t.count + 15) / 16 * 16 * quads;
     const size_t split = static_cast<size_t>(a.n_mats) * a.rows * a.max_rank;
     auto z_of = [&](int row, int k) {  // scale z, 4 values; row < 0: none
@@ -702,7 +715,7 @@ __device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &r
 #pragma unroll 1
             for (; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + s * split);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] = k + e < rank ? sum[e] * scale : 0.0f;
+            for (int e = 0; e < 4; ++e) sum[e] = k + e < rank ? sum[e] * t.scale : 0.0f;
         }
         return sum;
     };
@@ -764,15 +777,13 @@ __global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel
         __syncthreads();
         up<T, kThreads, 16>(a, t, rows, blockIdx.x % runs, s_z, s_wide);
     } else {
-        __shared__ Tile t;
-        const TileRows rows = {t.rows};
-        const int total = *a.n_tiles * runs;
-        for (int item = blockIdx.x; item < total; item += gridDim.x) {
-            const int tile = item / runs;
+        __shared__ int s_rows[kTile];
+        const TileRows rows = {s_rows};
+        for (int item = blockIdx.x;; item += gridDim.x) {
             __syncthreads();  // (the tile of before is read)
-            if (threadIdx.x < kTile) t.rows[threadIdx.x] = a.tiles[tile].rows[threadIdx.x];
+            const Group of = tile_at(a, item / runs, s_rows);
+            if (of.count == 0) break;  // uniform
             if (threadIdx.x == 0) s_wide = 0;
-            const Group of = {a.tiles[tile].adapter, a.tiles[tile].count};
             __syncthreads();
             up<T, kUpThreads, kTile>(a, of, rows, item % runs, s_z, s_wide);
         }
@@ -858,7 +869,7 @@ int qlin_launch_lora_add(const qlin_lora *mats, int n_mats, int weight_type, int
     char *ws = static_cast<char *>(workspace);
     a.ranks = ranks, a.ids = adapter_ids, a.scales = scales, a.x = x, a.x_stride = x_stride;
     a.n_tiles = reinterpret_cast<int *>(ws), a.tiles = reinterpret_cast<qlin::Tile *>(ws + l.tiles), a.z = reinterpret_cast<float *>(ws + l.z);
-    a.n_mats = kept, a.n_adapters = n_adapters, a.max_rank = max_rank, a.in_dim = in_dim, a.rows = rows, a.splits = l.splits;
+    a.n_mats = kept, a.n_adapters = n_adapters, a.max_rank = max_rank, a.in_dim = in_dim, a.rows = rows, a.splits = l.splits, a.most_tiles = l.most_tiles;
     const bool few = qlin::few_of(rows, n_adapters);
     // outputs of a workgroup: as many as leave 256 workgroups, since each stages z again (128: 2048 rows of 4096 to 4096 at rank 16
     // 40.8 us, 256: 37.0), but a step of its waves at least
