@@ -223,6 +223,19 @@ def test_many_rows(rows, slots, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("slots", [1, 1024])
+def test_most_rows(slots):
+    """More tiles than workgroups, with more projections; and no tile at all."""
+    torch = _gpu()
+    from gpu_util import banner
+    banner(f"lora_add rows=65536 slots={slots}")
+    c = _case(torch, slots, 65536, 64, [40, 8, 33], slots, 8, 0)
+    _check(torch, c)
+    c["ids"] = torch.full_like(c["ids"], -1)
+    _check(torch, c, in_place=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [0, 1, 2], ids=TYPES)
 @pytest.mark.parametrize("rank", [72, 200, 256])
 def test_many_rows_of_large_ranks(rank, kind):
