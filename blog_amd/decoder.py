@@ -128,6 +128,7 @@ class Qwen2Decoder:
         self.pos = torch.zeros(1, dtype=i32, device=dev)        # the next step's position
         self.at = torch.zeros(1, dtype=i32, device=dev)         # where a step is taken: past the last position, there
         self.zero = torch.zeros(1, dtype=i32, device=dev)
+        self.before = torch.zeros(1, dtype=i32, device=dev)     # rows of a step by drafts ahead of the one that completes a block
         self.L = qlin.lib()
         self.controls, self.captured = None, []
         self.adapters = None
@@ -232,8 +233,9 @@ class Qwen2Decoder:
         c = self.cfg
         self._ok("rms_norm", self.L.qlin_launch_rms_norm(x, out, w.data_ptr(), 0, rows, c.hidden, c.eps, 0))
 
-    def _layers(self, rows: int, pos_ptr: int):
-        """The decoder layers over `rows` tokens whose first position is *pos_ptr."""
+    def _layers(self, rows: int, pos_ptr: int, before: int = 0):
+        """The decoder layers over `rows` tokens whose first position is *pos_ptr.  before (an address): the first *before rows
+        see the 8-bit cache as it is without the rows after them."""
         c, L, t = self.cfg, self.L, c_ptr
         H, F, QD, KD = c.hidden, c.ffn, c.q_dim, c.kv_dim
         h, xn, q, k, v, attn, act = (t(self.h), t(self.xn), t(self.q), t(self.k), t(self.v), t(self.attn),
@@ -263,6 +265,8 @@ class Qwen2Decoder:
             if c.kv8:
                 qlin.qk_norm_rope_store_kv8(self.how[i], self.kv8[i], q, QD, k, KD, v, KD, q, rows, c.n_heads, pos_ptr)
                 qlin.attend_kv8(self.kv8[i], q, attn, rows, c.n_heads, pos_ptr, None, c.head_dim ** -0.5, self.attend_ws)
+                if before:  # (once more, in a cache that ends with them: their block is open there)
+                    qlin.attend_kv8(self.kv8[i], q, attn, rows, c.n_heads, pos_ptr, before, c.head_dim ** -0.5, self.attend_ws)
             elif c.qk_norm:
                 qlin.qk_norm_rope_store_kv(self.how[i], q, QD, k, KD, v, KD, q, self.kc[i], self.vc[i], rows, c.n_heads,
                                            c.kv_heads, c.head_dim, self.max_seq, pos_ptr)
@@ -383,7 +387,7 @@ class Qwen2Decoder:
     def step_drafts(self, d: dict, draft_logits=None) -> None:
         """Decode tokens by drafts (of self.drafts(n)): the next token and the n drafted ones after it in one pass, those
         that the model's probabilities accept and one more; leaves pos after them and the last one as the next token (no host
-        synchronisation).  draft_logits float32 [1, n, vocab], or None for drafts by lookup.  The positions pos .. pos + n
+        synchronisation).  A row's logits (d["logits"]) depend on no draft after it.  draft_logits float32 [1, n, vocab], or None for drafts by lookup.  The positions pos .. pos + n
         are below max_seq; controls of the pick do not go with it."""
         c, t, torch = self.cfg, c_ptr, self.torch
         if self.controls is not None:
@@ -396,7 +400,14 @@ class Qwen2Decoder:
         self.prompt_ids[1:rows].copy_(d["drafts"][0].clamp(0, c.vocab - 1))
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.prompt_ids), t(self.h), t(self.w["table"]),
                                                                  self.rb_h, c.hidden, rows))
-        self._layers(rows, t(self.pos))
+        before = 0
+        if c.kv8 and rows > 1:
+            # A block that ends at row b stands in codes, whose scale has all of its rows, also drafts that may be rejected: the
+            # rows before b see it as it was, open.  (At most 32 rows: one block ends among them, or none.)
+            torch.bitwise_and(torch.bitwise_not(self.pos), qlin.KV8_BLOCK - 1, out=self.before)
+            self.before.masked_fill_(self.before >= rows, 0)
+            before = t(self.before)
+        self._layers(rows, t(self.pos), before)
         self._norm(t(self.h), t(self.xn), self.w["final_norm"], rows)
         self._ok("lm_head", self.L.qlin_launch_quant_matmul(c.wtype, t(self.w["table"]), self.rb_h, t(self.xn), t(d["logits"]),
                                                             c.vocab, c.hidden, rows))

@@ -112,6 +112,9 @@ extern "C" {
  *   qlin_launch_attend_kv8      attn[s, r, h] = sum_j p_j v_j, p = softmax_j(softmax_scale * q . k_j) over the positions
  *                               j <= the row's that the cache holds, which ends at start_pos_dev[s] + the sequence's rows
  *                               (their keys and values are stored first); heads and key heads as in qlin_launch_attend.
+ *                               (A block that a later row of the call completes is seen in codes, whose scale is that of
+ *                               all its positions.  Rows that must not depend on later ones, as those of drafted tokens, are
+ *                               taken again by a second call whose n_rows_dev ends before the row that completes the block.)
  *                               A row that sees no position gives 0.  f32 accuracy: q softmax_scale log2(e) and p are
  *                               rounded to pairs of fp16 values, 22 bits and a sign each (what is below 2^-39 of a row's
  *                               largest q, or 2^-36 of its largest p, is lost), and their products with the codes are
