@@ -90,13 +90,16 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(const float *__r
 }
 
 // One wave per (row, head): query heads rotated in place; key heads rotated into the cache at the
-// row's position, with the row's value head beside them.
+// row's position, with the row's value head beside them.  Rows outside the cache are clamped to its ends, where a row of
+// the call may stand already: of those at one end only the nearest is stored (two would be written at once, in no order).
 __global__ __launch_bounds__(64) void rope_store_kernel(float *__restrict__ q, const float *__restrict__ k,
                                                         const float *__restrict__ v, float *__restrict__ kc,
                                                         float *__restrict__ vc, int n_heads, int kv_heads, int hd,
                                                         int max_seq, const int *__restrict__ start_pos, float theta) {
     const int row = blockIdx.x, head = blockIdx.y;
-    const int pos = min(max(*start_pos + row, 0), max_seq - 1);
+    const int64_t at = static_cast<int64_t>(*start_pos) + row;
+    const int pos = static_cast<int>(at < 0 ? 0 : at < max_seq ? at : max_seq - 1);
+    if (head >= n_heads && at != pos && row != (at < pos ? static_cast<int>(gridDim.x) - 1 : 0)) return;
     const int half = hd / 2;
     auto rotate = [&](const float *src, float *dst) {
         for (int i = threadIdx.x; i < half; i += 64) {

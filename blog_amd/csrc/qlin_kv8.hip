@@ -186,7 +186,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_store_kernel(qlin_qk_rope 
     Runs rr = r;
     rr.turned = rr.turned && live && (is_q || is_k);
     norm_and_turn<T>(x, y, rr, live, hd, is_q ? how.q_norm : how.k_norm, how, pos, max_seq);
-    if (live) {
+    // (of the rows outside the cache at one end of it only the nearest is stored: there two would be written at once)
+    if (live && (is_q || at == pos || row == (at < pos ? rows - 1 : 0))) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // (by value: a choice between vectors goes through memory)
             a[e] = is_q || is_k ? x[e] : a[e];

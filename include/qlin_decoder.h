@@ -20,7 +20,8 @@
  *   qlin_launch_attend         launch_full_attention_attend (kernel.cuh:186-189, kernel.cu:345-420) without
  *                              its output gate: attn[r, h] = softmax_j(q[r, h] . k[j, h / (n_heads /
  *                              kv_heads)] / sqrt(head_dim)) v[j, .] over positions j <= the row's.
- * A row's position is clamped to [0, max_seq_len - 1]; head_dim <= 256 and max_seq_len <= 32768
+ * A row's position is clamped to [0, max_seq_len - 1], and of the rows that a call has at one end then only the nearest is
+ * stored (the one whose own position it is, if there is one); head_dim <= 256 and max_seq_len <= 32768
  * (else QLIN_ERR_LIMIT); n_heads a multiple of kv_heads and head_dim of 4 (else QLIN_ERR_SHAPE);
  * qlin_launch_attend reads q, the caches and attn as 16-byte vectors (16-byte aligned, else
  * QLIN_ERR_ALIGN).
