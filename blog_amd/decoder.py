@@ -128,6 +128,7 @@ class Qwen2Decoder:
         self.pos = torch.zeros(1, dtype=i32, device=dev)        # the next step's position
         self.at = torch.zeros(1, dtype=i32, device=dev)         # where a step is taken: past the last position, there
         self.zero = torch.zeros(1, dtype=i32, device=dev)
+        self.room = torch.zeros(1, dtype=i32, device=dev)       # drafts that a step by drafts checks
         self.before = torch.zeros(1, dtype=i32, device=dev)     # rows of a step by drafts ahead of the one that completes a block
         self.L = qlin.lib()
         self.controls, self.captured = None, []
@@ -387,8 +388,9 @@ class Qwen2Decoder:
     def step_drafts(self, d: dict, draft_logits=None) -> None:
         """Decode tokens by drafts (of self.drafts(n)): the next token and the n drafted ones after it in one pass, those
         that the model's probabilities accept and one more; leaves pos after them and the last one as the next token (no host
-        synchronisation).  A row's logits (d["logits"]) depend on no draft after it.  draft_logits float32 [1, n, vocab], or None for drafts by lookup.  The positions pos .. pos + n
-        are below max_seq; controls of the pick do not go with it."""
+        synchronisation).  A row's logits (d["logits"]) depend on no draft after it.  draft_logits float32 [1, n, vocab], or
+        None for drafts by lookup.  Drafts that the cache has no position for are not checked, as if n_drafts left them out; from
+        the last position on that one is taken again, as step() does.  Controls of the pick do not go with it."""
         c, t, torch = self.cfg, c_ptr, self.torch
         if self.controls is not None:
             raise ValueError("drafts are not checked under controls")
@@ -400,19 +402,22 @@ class Qwen2Decoder:
         self.prompt_ids[1:rows].copy_(d["drafts"][0].clamp(0, c.vocab - 1))
         self._ok("embedding", self.L.qlin_launch_quant_embedding(c.wtype, t(self.prompt_ids), t(self.h), t(self.w["table"]),
                                                                  self.rb_h, c.hidden, rows))
+        # (drafts that there are positions for: the room is on the device, as the position is)
+        torch.clamp(self.pos, max=self.max_seq - 1, out=self.at)
+        torch.minimum(d["n_drafts"], (self.max_seq - 1) - self.at, out=self.room)
         before = 0
         if c.kv8 and rows > 1:
             # A block that ends at row b stands in codes, whose scale has all of its rows, also drafts that may be rejected: the
             # rows before b see it as it was, open.  (At most 32 rows: one block ends among them, or none.)
-            torch.bitwise_and(torch.bitwise_not(self.pos), qlin.KV8_BLOCK - 1, out=self.before)
+            torch.bitwise_and(torch.bitwise_not(self.at), qlin.KV8_BLOCK - 1, out=self.before)
             self.before.masked_fill_(self.before >= rows, 0)
             before = t(self.before)
-        self._layers(rows, t(self.pos), before)
+        self._layers(rows, t(self.at), before)
         self._norm(t(self.h), t(self.xn), self.w["final_norm"], rows)
         self._ok("lm_head", self.L.qlin_launch_quant_matmul(c.wtype, t(self.w["table"]), self.rb_h, t(self.xn), t(d["logits"]),
                                                             c.vocab, c.hidden, rows))
         qlin.verify_drafts(d["logits"], d["drafts"], d["uniform"], d["tokens"], d["accepted"], draft_logits=draft_logits,
-                           n_drafts=d["n_drafts"], temperature=d["temperature"], logprobs=d["logprobs"], rates=d["rates"],
+                           n_drafts=self.room, temperature=d["temperature"], logprobs=d["logprobs"], rates=d["rates"],
                            workspace=d["ws"])
         torch.index_select(d["tokens"][0], 0, d["accepted"], out=self.token)
         self.pos.add_(d["accepted"]).add_(1)
