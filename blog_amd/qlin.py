@@ -549,10 +549,30 @@ def _rows_of(t, shape, name, device):
 
 
 def _values_of(t, n, dtype, name, device):
-    """The address of at least n contiguous values of dtype."""
-    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != device:
-        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device}, not {n} contiguous values of {dtype} on device {device}")
+    """The address of n values of dtype, one for each row or adapter: contiguous, alone or the first ones of a longer line."""
+    have = t.numel()
+    if t.dtype is not dtype or have != n and (have < n or t.dim() > 1 and t.shape[-1] != 1) or not t.is_contiguous() or t.get_device() != device:
+        raise _not(t, f"{n} contiguous values of {dtype}", name, device)
     return t.data_ptr()
+
+
+def _table_of(t, n, width, dtype, name, device):
+    """The address of n rows of width values of dtype that stand one after the other: [>= n, width] (or a flat buffer of them)."""
+    if t.dtype is not dtype or t.numel() < n * width or n > 1 and width and t.dim() > 1 and t.shape[-1] != width or not t.is_contiguous() or (
+            t.get_device() != device):
+        raise _not(t, f"contiguous {dtype} [{n}, {width}]", name, device)
+    return t.data_ptr()
+
+
+def _bytes_of(t, n, name, device):
+    """The address of at least n bytes, in whatever shape."""
+    if t.dtype is not _U8 or t.numel() < n or not t.is_contiguous() or t.get_device() != device:
+        raise _not(t, f"{n} contiguous bytes (uint8)", name, device)
+    return t.data_ptr()
+
+
+def _not(t, what, name, device):
+    return ValueError(f"{name}: {tuple(t.shape)} of {t.dtype} on {t.device}, not {what} on device {device}")
 
 
 def _device_of(t, name):
@@ -576,9 +596,10 @@ def add_rms_norm(x, delta, sum, weight, norm_type, eps, one_plus, *, normed=None
     p_delta, n_delta = (0, 0) if delta is None else _rows_of(delta, shape, "delta", device)
     p_sum, n_sum = (0, 0) if sum is None else _rows_of(sum, shape, "sum", device)
     p_normed, n_normed = (0, 0) if normed is None else _rows_of(normed, shape, "normed", device)
-    if weight.element_size() != 2 or weight.numel() < hidden or not weight.is_contiguous() or weight.get_device() != device:
+    if weight.element_size() != 2 or weight.numel() != hidden and (weight.numel() < hidden or weight.dim() > 1) or not weight.is_contiguous() or (
+            weight.get_device() != device):
         raise ValueError(f"weight: {tuple(weight.shape)} of {weight.dtype} on {weight.device}, not {hidden} contiguous values of 16 bits")
-    p_q8 = 0 if q8_1 is None else _values_of(q8_1, q8_1_bytes(hidden, rows, mmq), _U8, "q8_1", device)
+    p_q8 = 0 if q8_1 is None else _bytes_of(q8_1, q8_1_bytes(hidden, rows, mmq), "q8_1", device)
     rc = library.qlin_launch_add_rms_norm(p_x, n_x, p_delta, n_delta, p_sum, n_sum, weight.data_ptr(), norm_type, eps, int(one_plus),
                                           p_normed, n_normed, p_q8, int(mmq), int(raw_sum), rows, hidden)
     if rc != 0:
@@ -586,10 +607,10 @@ def add_rms_norm(x, delta, sum, weight, norm_type, eps, one_plus, *, normed=None
 
 
 def dequantize_q8_1(x_q8_1, x, in_dim, m, mmq=False):
-    """The values that m rows of Q8_1 blocks (uint8) stand for, into x (float32, contiguous)."""
+    """The values that m rows of Q8_1 blocks (uint8) stand for, into x (float32 [m, in_dim], contiguous)."""
     library, device = _lib or lib(), _device_of(x, "x")
-    rc = library.qlin_launch_dequantize_q8_1(_values_of(x_q8_1, q8_1_bytes(in_dim, m, mmq), _U8, "x_q8_1", device),
-                                             _values_of(x, in_dim * m, _F32, "x", device), in_dim, m, int(mmq))
+    rc = library.qlin_launch_dequantize_q8_1(_bytes_of(x_q8_1, q8_1_bytes(in_dim, m, mmq), "x_q8_1", device),
+                                             _table_of(x, m, in_dim, _F32, "x", device), in_dim, m, int(mmq))
     if rc != 0:
         raise QlinError("qlin_launch_dequantize_q8_1", rc)
 
@@ -643,7 +664,7 @@ def lora_add(x, adapter_ids, mats, *, ranks=None, scales=None, workspace=None):
         each += (*w.addresses, p_base, p_y, n_base, n_y, w.out_dim)
     p_ws = ws_bytes = 0
     if workspace is not None:
-        p_ws, ws_bytes = _values_of(workspace, 0, _U8, "workspace", device), workspace.numel()
+        p_ws, ws_bytes = _bytes_of(workspace, 0, "workspace", device), workspace.numel()
     rc = library.qlin_launch_lora_add(_LORAS[len(mats)].pack(*each), len(mats), kind, slots, rank, width,
                                       0 if ranks is None else _values_of(ranks, slots, _I32, "ranks", device),
                                       0 if scales is None else _values_of(scales, slots, _F32, "scales", device), p_x, n_x,
@@ -672,12 +693,12 @@ def moe_route(how, logits, ids, weights):
     p_logits, stride = _rows_of(logits, logits.shape, "logits", device)
     shape = ids.shape
     k = shape[1]
-    if how.bias is not None and (how.bias.numel() < n_experts or how.bias.get_device() != device):
-        raise ValueError(f"a bias of {how.bias.numel()} values on {how.bias.device} for {n_experts} experts on device {device}")
+    if how.bias is not None:
+        _values_of(how.bias, n_experts, _F32, "the bias", device)
     if shape[0] < tokens or weights.shape != shape:
         raise ValueError(f"ids {tuple(ids.shape)} and weights {tuple(weights.shape)} for {tokens} tokens")
-    rc = library.qlin_launch_moe_route(how.address, p_logits, stride, _values_of(ids, 0, _I32, "ids", device),
-                                       _values_of(weights, 0, _F32, "weights", device), tokens, n_experts, k)
+    rc = library.qlin_launch_moe_route(how.address, p_logits, stride, _table_of(ids, tokens, k, _I32, "ids", device),
+                                       _table_of(weights, tokens, k, _F32, "weights", device), tokens, n_experts, k)
     if rc != 0:
         raise QlinError("qlin_launch_moe_route", rc)
 
@@ -715,13 +736,13 @@ def verify_drafts(target, drafts, uniform, tokens, accepted, *, draft_logits=Non
     if draft_logits is not None:
         p_draft, draft_stride = _logits_of(draft_logits, (n, d, vocab), "draft_logits", device)
     if workspace is not None:
-        p_ws, ws_bytes = _values_of(workspace, 0, _U8, "workspace", device), workspace.numel()
+        p_ws, ws_bytes = _bytes_of(workspace, 0, "workspace", device), workspace.numel()
     rc = library.qlin_launch_verify_drafts(
-        p_target, target_stride, p_draft if d else 0, draft_stride, 0 if drafts is None else _values_of(drafts, n * d, _I32, "drafts", device),
+        p_target, target_stride, p_draft if d else 0, draft_stride, 0 if drafts is None else _table_of(drafts, n, d, _I32, "drafts", device),
         0 if n_drafts is None else _values_of(n_drafts, n, _I32, "n_drafts", device),
         0 if temperature is None else _values_of(temperature, n, _F32, "temperature", device),
-        _values_of(uniform, n * rows, _F32, "uniform", device), _values_of(tokens, n * rows, _I32, "tokens", device),
-        _values_of(accepted, n, _I32, "accepted", device), 0 if logprobs is None else _values_of(logprobs, n * rows, _F32, "logprobs", device),
-        0 if rates is None else _values_of(rates, n * d, _F32, "rates", device), n, d, vocab, p_ws, ws_bytes)
+        _table_of(uniform, n, rows, _F32, "uniform", device), _table_of(tokens, n, rows, _I32, "tokens", device),
+        _values_of(accepted, n, _I32, "accepted", device), 0 if logprobs is None else _table_of(logprobs, n, rows, _F32, "logprobs", device),
+        0 if rates is None else _table_of(rates, n, d, _F32, "rates", device), n, d, vocab, p_ws, ws_bytes)
     if rc != 0:
         raise QlinError("qlin_launch_verify_drafts", rc)
