@@ -178,12 +178,12 @@ class QlinError(RuntimeError):
 
 _lib = None
 _F32 = _I32 = _U32 = _U8 = None  # torch's types
-_LORA_TYPES = {}
+_LORA_TYPES, _NOT_NORM_TYPE = {}, {}
 
 
 def lib() -> C.CDLL:
     """Loads the HIP library; raises if it has not been built (no fallback path exists)."""
-    global _lib, _F32, _I32, _U32, _U8, _LORA_TYPES
+    global _lib, _F32, _I32, _U32, _U8, _LORA_TYPES, _NOT_NORM_TYPE
     if _lib is None:
         # torch ships its own HIP runtime (torch/lib/libamdhip64.so, soname libamdhip64.so.7).  Loaded
         # first, it satisfies this library's libamdhip64.so.7 dependency, so the process has one HIP
@@ -193,6 +193,7 @@ def lib() -> C.CDLL:
             import torch
             _F32, _I32, _U32, _U8 = torch.float32, torch.int32, torch.uint32, torch.uint8
             _LORA_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+            _NOT_NORM_TYPE = {torch.float16: 0, torch.bfloat16: 1}  # (whole numbers are patterns of either type)
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -599,6 +600,8 @@ def add_rms_norm(x, delta, sum, weight, norm_type, eps, one_plus, *, normed=None
     if weight.element_size() != 2 or weight.numel() != hidden and (weight.numel() < hidden or weight.dim() > 1) or not weight.is_contiguous() or (
             weight.get_device() != device):
         raise ValueError(f"weight: {tuple(weight.shape)} of {weight.dtype} on {weight.device}, not {hidden} contiguous values of 16 bits")
+    if _NOT_NORM_TYPE.get(weight.dtype) == norm_type:
+        raise ValueError(f"weight: {weight.dtype} with norm_type {norm_type} (0 bfloat16, 1 float16)")
     p_q8 = 0 if q8_1 is None else _bytes_of(q8_1, q8_1_bytes(hidden, rows, mmq), "q8_1", device)
     rc = library.qlin_launch_add_rms_norm(p_x, n_x, p_delta, n_delta, p_sum, n_sum, weight.data_ptr(), norm_type, eps, int(one_plus),
                                           p_normed, n_normed, p_q8, int(mmq), int(raw_sum), rows, hidden)

@@ -105,3 +105,15 @@ def test_add_rms_norm_refuses_weights_of_several_rows(calls):
         with pytest.raises(ValueError):
             qlin.add_rms_norm(x, None, None, bad, 0, 1e-6, 0, normed=z(2, 64))
     assert len(calls) == 2
+
+
+def test_add_rms_norm_refuses_weights_of_the_other_type(calls):
+    x = z(2, 64)
+    run = lambda w, kind: qlin.add_rms_norm(x, None, None, w, kind, 1e-6, 0, normed=z(2, 64))
+    for w, kind in ((z(64, dtype=bf16), 0), (z(64, dtype=f16), 1), (z(64, dtype=torch.int16), 0), (z(64, dtype=torch.int16), 1), (z(64, dtype=torch.uint16), 1)):
+        run(w, kind)  # (patterns of 16 bits may be either)
+    assert len(calls) == 5
+    for w, kind in ((z(64, dtype=bf16), 1), (z(64, dtype=f16), 0)):
+        with pytest.raises(ValueError):
+            run(w, kind)
+    assert len(calls) == 5
