@@ -178,12 +178,14 @@ class QlinError(RuntimeError):
 
 _lib = None
 _F32 = _I32 = _U32 = _U8 = None  # torch's types
-_LORA_TYPES, _NOT_NORM_TYPE = {}, {}
+_BF16 = _F16 = None
+_LORA_TYPES = {}
+_current_device = None
 
 
 def lib() -> C.CDLL:
     """Loads the HIP library; raises if it has not been built (no fallback path exists)."""
-    global _lib, _F32, _I32, _U32, _U8, _LORA_TYPES, _NOT_NORM_TYPE
+    global _lib, _F32, _I32, _U32, _U8, _BF16, _F16, _LORA_TYPES, _current_device
     if _lib is None:
         # torch ships its own HIP runtime (torch/lib/libamdhip64.so, soname libamdhip64.so.7).  Loaded
         # first, it satisfies this library's libamdhip64.so.7 dependency, so the process has one HIP
@@ -193,7 +195,9 @@ def lib() -> C.CDLL:
             import torch
             _F32, _I32, _U32, _U8 = torch.float32, torch.int32, torch.uint32, torch.uint8
             _LORA_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-            _NOT_NORM_TYPE = {torch.float16: 0, torch.bfloat16: 1}  # (whole numbers are patterns of either type)
+            _BF16, _F16 = torch.bfloat16, torch.float16
+            # (what torch.cuda.current_device calls after its own look at whether the GPU has been met; a tensor there has)
+            _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -559,8 +563,9 @@ def _values_of(t, n, dtype, name, device):
 
 def _table_of(t, n, width, dtype, name, device):
     """The address of n rows of width values of dtype that stand one after the other: [>= n, width] (or a flat buffer of them)."""
-    if t.dtype is not dtype or t.numel() < n * width or n > 1 and width and t.dim() > 1 and t.shape[-1] != width or not t.is_contiguous() or (
-            t.get_device() != device):
+    shape = t.shape
+    if t.dtype is not dtype or shape != (n, width) and (t.numel() < n * width or n > 1 and width and len(shape) > 1 and shape[-1] != width) or (
+            not t.is_contiguous() or t.get_device() != device):
         raise _not(t, f"contiguous {dtype} [{n}, {width}]", name, device)
     return t.data_ptr()
 
@@ -580,6 +585,8 @@ def _device_of(t, name):
     device = t.get_device()
     if device < 0:
         raise ValueError(f"{name} is on {t.device}, not on a GPU")
+    if device != _current_device():  # (a launch goes to the current device)
+        raise ValueError(f"{name} is on {t.device}, not on the current device {_current_device()}")
     return device
 
 
@@ -593,14 +600,14 @@ def add_rms_norm(x, delta, sum, weight, norm_type, eps, one_plus, *, normed=None
     are float32 [rows, hidden] with contiguous rows; delta and sum may be None, sum may be x or delta."""
     library, device, shape = _lib or lib(), _device_of(x, "x"), x.shape
     rows, hidden = shape
-    p_x, n_x = _rows_of(x, shape, "x", device)
+    p_x, n_x = (x.data_ptr(), hidden) if x.dtype is _F32 and x.is_contiguous() else _rows_of(x, shape, "x", device)
     p_delta, n_delta = (0, 0) if delta is None else _rows_of(delta, shape, "delta", device)
     p_sum, n_sum = (0, 0) if sum is None else _rows_of(sum, shape, "sum", device)
     p_normed, n_normed = (0, 0) if normed is None else _rows_of(normed, shape, "normed", device)
     if weight.element_size() != 2 or weight.numel() != hidden and (weight.numel() < hidden or weight.dim() > 1) or not weight.is_contiguous() or (
             weight.get_device() != device):
         raise ValueError(f"weight: {tuple(weight.shape)} of {weight.dtype} on {weight.device}, not {hidden} contiguous values of 16 bits")
-    if _NOT_NORM_TYPE.get(weight.dtype) == norm_type:
+    if weight.dtype is (_BF16 if norm_type else _F16):  # (whole numbers are patterns of either type)
         raise ValueError(f"weight: {weight.dtype} with norm_type {norm_type} (0 bfloat16, 1 float16)")
     p_q8 = 0 if q8_1 is None else _bytes_of(q8_1, q8_1_bytes(hidden, rows, mmq), "q8_1", device)
     rc = library.qlin_launch_add_rms_norm(p_x, n_x, p_delta, n_delta, p_sum, n_sum, weight.data_ptr(), norm_type, eps, int(one_plus),
@@ -693,7 +700,8 @@ def moe_route(how, logits, ids, weights):
     weights float32, both [tokens, k] and contiguous."""
     library, device = _lib or lib(), _device_of(logits, "logits")
     tokens, n_experts = logits.shape
-    p_logits, stride = _rows_of(logits, logits.shape, "logits", device)
+    contiguous = logits.dtype is _F32 and logits.is_contiguous()
+    p_logits, stride = (logits.data_ptr(), n_experts) if contiguous else _rows_of(logits, logits.shape, "logits", device)
     shape = ids.shape
     k = shape[1]
     if how.bias is not None:
@@ -734,7 +742,8 @@ def verify_drafts(target, drafts, uniform, tokens, accepted, *, draft_logits=Non
     library, device, shape = _lib or lib(), _device_of(target, "target"), target.shape
     n, rows, vocab = shape
     d = rows - 1
-    p_target, target_stride = _logits_of(target, shape, "target", device)
+    contiguous = target.dtype is _F32 and target.is_contiguous()
+    p_target, target_stride = (target.data_ptr(), vocab) if contiguous else _logits_of(target, shape, "target", device)
     p_draft = draft_stride = p_ws = ws_bytes = 0
     if draft_logits is not None:
         p_draft, draft_stride = _logits_of(draft_logits, (n, d, vocab), "draft_logits", device)

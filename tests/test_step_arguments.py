@@ -117,3 +117,22 @@ def test_add_rms_norm_refuses_weights_of_the_other_type(calls):
         with pytest.raises(ValueError):
             run(w, kind)
     assert len(calls) == 5
+
+
+def test_tensors_of_another_device_than_the_current_one(calls, monkeypatch):
+    monkeypatch.undo()
+    qlin.lib()
+    monkeypatch.setattr(qlin, "_current_device", lambda: 0, raising=False)
+
+    class There:
+        device = "cuda"
+
+        def __init__(self, at):
+            self.at = at
+
+        def get_device(self):
+            return self.at
+    assert qlin._device_of(There(0), "x") == 0
+    for at in (1, -1):
+        with pytest.raises(ValueError):
+            qlin._device_of(There(at), "x")
