@@ -216,6 +216,8 @@ class Qwen2Decoder:
             raise ValueError("slot: a number, or int32 [1] on the decoder's device")
         self.adapters = dict(layers=layers, slot=slot, ids=ids, ranks=ranks, scales=scales,
                              ws=torch.empty(need, dtype=torch.uint8, device="cuda"))
+        # (a call on another stream than this one waits for nothing here: the slot is written, and what had the memory before is done)
+        torch.cuda.current_stream().synchronize()
 
     def _adapt(self, layer, x, rows, outs):
         """Adds the layer's adapters of the linears in outs (name: output), which read x."""
@@ -381,9 +383,11 @@ class Qwen2Decoder:
             raise ValueError(f"{n} drafted tokens: at most {min(self.max_prompt, qlin.KV8_BLOCK) - 1}")
         f = lambda *shape: torch.zeros(*shape, dtype=torch.float32, device=dev)
         i = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)
-        return dict(drafts=i(1, n), uniform=f(1, n + 1), n_drafts=torch.full((1,), n, dtype=torch.int32, device=dev), temperature=f(1),
-                    tokens=i(1, n + 1), accepted=i(1), logprobs=f(1, n + 1), rates=f(1, n), logits=f(1, n + 1, c.vocab),
-                    ws=torch.empty(max(16, qlin.verify_drafts_workspace_bytes(1, n, c.vocab)), dtype=torch.uint8, device=dev))
+        d = dict(drafts=i(1, n), uniform=f(1, n + 1), n_drafts=torch.full((1,), n, dtype=torch.int32, device=dev), temperature=f(1),
+                 tokens=i(1, n + 1), accepted=i(1), logprobs=f(1, n + 1), rates=f(1, n), logits=f(1, n + 1, c.vocab),
+                 ws=torch.empty(max(16, qlin.verify_drafts_workspace_bytes(1, n, c.vocab)), dtype=torch.uint8, device=dev))
+        torch.cuda.current_stream().synchronize()  # (as set_adapters)
+        return d
 
     def step_drafts(self, d: dict, draft_logits=None) -> None:
         """Decode tokens by drafts (of self.drafts(n)): the next token and the n drafted ones after it in one pass, those
