@@ -197,7 +197,7 @@ class Qwen2Decoder:
             raise ValueError(f"adapters for {len(layers)} layers of {c.layers}")
         dims = {"wq": (c.hidden, c.q_dim), "wk": (c.hidden, c.kv_dim), "wv": (c.hidden, c.kv_dim), "wo": (c.q_dim, c.hidden),
                 "wd": (c.ffn, c.hidden)}
-        need = 16
+        forms = set()
         for L in layers:
             for name, w in L.items():
                 if name not in dims or (w.in_dim, w.out_dim) != dims[name]:
@@ -206,9 +206,9 @@ class Qwen2Decoder:
                 there = [L[n] for n in names if n in L]
                 if any(w.like != there[0].like for w in there):
                     raise ValueError("the adapters of wq, wk and wv have one type, number of slots and rank")
-                # (also for fewer rows, which can take more workspace)
-                need = max([need] + [qlin.lora_workspace_bytes(rows, len(there), *w.like[1:]) for w in there[:1]
-                                     for rows in range(1, self.max_prompt + 1)])
+                forms.update((len(there), *w.like[1:]) for w in there[:1])
+        # (also for fewer rows, which can take more workspace)
+        need = max([16] + [qlin.lora_workspace_bytes(rows, *form) for form in forms for rows in range(1, self.max_prompt + 1)])
         ids = torch.empty(self.max_prompt, dtype=torch.int32, device="cuda")
         if not torch.is_tensor(slot):
             slot = torch.full((1,), slot, dtype=torch.int32, device="cuda")

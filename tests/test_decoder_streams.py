@@ -68,3 +68,21 @@ def test_set_up_on_another_stream():
             assert torch.equal(x, y), turn
         del held
     qlin.set_stream(torch.cuda.current_stream())
+
+
+def test_adapters_workspace(monkeypatch):
+    """Enough for every number of rows and linear, asked for once for layers that are alike."""
+    torch = _env()
+    from gpu_util import banner
+    from blog_amd.decoder import Qwen2Decoder, make_weights
+    banner("the adapters' workspace")
+    cfg = _config(vocab=200, layers=6)
+    dec = Qwen2Decoder(torch, cfg, make_weights(torch, cfg, seed=5), max_seq=96, max_prompt=80)
+    layers = _loras(torch, cfg, 1)
+    layers[3] = {"wq": layers[3]["wq"], "wv": qlin.Lora(torch.zeros(3, 8, cfg.hidden, device="cuda"), torch.zeros(3, cfg.kv_dim, 8, device="cuda"))}
+    asked, real = [], qlin.lora_workspace_bytes
+    monkeypatch.setattr(qlin, "lora_workspace_bytes", lambda *a: asked.append(a) or real(*a))
+    dec.set_adapters(layers, 1)
+    forms = {(len(ws), ws[0].like) for L in layers for names in dec.LINEARS if (ws := [L[n] for n in names if n in L])}
+    want = max(real(rows, n, *like[1:]) for n, like in forms for rows in range(1, 81))
+    assert len(forms) == 4 and dec.adapters["ws"].numel() == want and len(asked) <= len(forms) * 80
