@@ -12,9 +12,10 @@
 //
 // Products are exact.  bf16 and f16 weights go to v_mfma_f32_16x16x32_bf16: an f16 weight is the sum of two bf16 values, and
 // 2^26 v of an f32 value v is the sum of three (8 bits each; with the factor, which leaves with the sum, all parts of any v are
-// normal numbers).  Where a |v| is 2^60 or more (or infinite) these would overflow, and what is left goes to
-// v_mfma_f32_16x16x4_f32, a uniform and rare branch; f32 weights go there always.  (All types there: 613 rows of 18944 to 3584
-// with 8 adapters of rank 64 in f16 63.3 and 57.4 us in the two launches, where they take 25.3 and 14.0.)
+// normal numbers).  Where a |v| is 2^60 or more (or infinite) these would overflow: such values of x, and the rows of z that have
+// one, go to v_mfma_f32_16x16x4_f32 after the others, a uniform and rare branch, so that no row's result depends on the rows beside
+// it; f32 weights go there always.  (All types there: 613 rows of 18944 to 3584 with 8 adapters of rank 64 in f16 63.3 and 57.4 us
+// in the two launches, where they take 25.3 and 14.0.)
 //
 // Few rows are bound by latency: one row of 896 to 896, 128 and 128 at rank 16 takes 9.7 us in a graph, 48 rows of 3584 to 3584,
 // 512 and 512 with 15 adapters of rank 32 15.8.  Many are bound by memory in the second launch (2011 rows of 4096 to 14336 at rank
@@ -359,7 +360,11 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
     static_assert(H * 16 * NT <= kDownRows && 16 * RT <= kDownRows, "");
     char *mine = lds + wave * (kDownRows * kRowBytes);
     const int n = lane & 15, g = lane >> 4;
-    auto multiply = [&](Step &s, int at, auto wide) {
+    // How a step is taken: on bf16 products all values (not done, and false, where one is kWide or more) or those below kWide; on f32
+    // products the other ones, of f32 weights all.
+    constexpr int kAll = 0, kSmall = 1, kLarge = 2;
+    auto multiply = [&](Step &s, int at, auto how) {
+        constexpr int HOW = decltype(how)::value;
         if (K * at + K > a.in_dim) {  // uniform
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -385,7 +390,18 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
         for (int i = 0; i < RT; ++i)
             if (i < tiles) put_rows(mine + 16 * i * kRowBytes, s.w[i], lane);
         wave_sync();
-        if constexpr (decltype(wide)::value) {
+        if constexpr (HOW != kAll && T != 2) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float f = v[h][j][e >> 2][e & 3];
+                        v[h][j][e >> 2][e & 3] = (fabsf(f) < kWide) == (HOW == kSmall) ? f : 0.0f;
+                    }
+        }
+        if constexpr (HOW == kLarge) {
 #pragma unroll
             for (int i = 0; i < RT; ++i)
                 if (i < tiles) {
@@ -399,14 +415,16 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
                 }
             return true;
         } else {
-            float top = 0.0f;
+            if constexpr (HOW == kAll) {
+                float top = 0.0f;
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                    for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) top = max3_abs(v[h][j][e >> 2][e & 3], v[h][j][e >> 2][(e & 3) + 1], top);
-            if (__any(!(top < kWide))) return false;
+                        for (int e = 0; e < 8; e += 2) top = max3_abs(v[h][j][e >> 2][e & 3], v[h][j][e >> 2][(e & 3) + 1], top);
+                if (__any(!(top < kWide))) return false;
+            }
             u32x4 hi[H][NT], mid[H][NT], lo[H][NT];
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -437,25 +455,33 @@ __device__ __forceinline__ void down(const LoraArgs &a, const Group &t, const R 
         while (at < to) {
             Step now = s;
             if (at + 1 < to) load(s, at + 1);
-            fits = multiply(now, at, std::false_type());
-            if (!fits) break;  // uniform: a value that is too large
+            fits = multiply(now, at, std::integral_constant<int, kAll>());
+            if (!fits) break;  // uniform
             ++at;
+        }
+        // from the first step with a large value on: the small ones as before, in the same order, and the large ones after them, so that a row
+        // without any has the same sum
+        const int first_large = at;
+#pragma unroll 1
+        for (; at < to; ++at) {
+            load(s, at);
+            multiply(s, at, std::integral_constant<int, kSmall>());
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] *= kDown;
 #pragma unroll 1
-        for (; at < to; ++at) {
+        for (at = first_large; at < to; ++at) {
             load(s, at);
-            multiply(s, at, std::true_type());
+            multiply(s, at, std::integral_constant<int, kLarge>());
         }
     } else {
 #pragma unroll 1
         for (; at < to; ++at) {
             Step now = s;
             if (at + 1 < to) load(s, at + 1);
-            multiply(now, at, std::true_type());
+            multiply(now, at, std::integral_constant<int, kLarge>());
         }
     }
     __syncthreads();  // (the waves' rows are read)
@@ -534,7 +560,6 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 // scale z of a tile in LDS: the three bf16 parts of 2^26 of it (Z of bf16 and f16 weights), or f32 values; 0 past the rank.
 struct Staged {
     int stride, part;  // bytes from a row to the next one, and from a part
-    bool wide;
 };
 
 // y of 16 NT rows of a tile from its row `from` on, 32 outputs at a time: a line of each row.
@@ -546,7 +571,7 @@ struct Up {
     const qlin_lora &m;
     const float *base[2 * NT];
     float *y[2 * NT];
-    bool there[2 * NT];
+    bool there[2 * NT];  // rows to be stored
     f32x4 was[2 * NT];
     u32x4 ahead[4];  // the first line of weights of the next outputs
     const char *b;
@@ -563,6 +588,14 @@ struct Up {
             there[j] = at < t.count;
             base[j] = m.base + row * m.base_stride + 4 * (lane & 7);
             y[j] = m.y + row * m.y_stride + 4 * (lane & 7);
+        }
+    }
+    // Only the tile's rows in the mask are stored.
+    __device__ __forceinline__ void choose(uint64_t mask, int from, int count) {
+#pragma unroll
+        for (int j = 0; j < 2 * NT; ++j) {
+            const int at = from + 8 * j + (lane >> 3);
+            there[j] = at < count && (mask >> at & 1);
         }
     }
     // Weights come before the base: loads arrive in order, and the products can go ahead of it.
@@ -676,7 +709,7 @@ constexpr int kUpBytes = 32 * kRowBytes;  // of a wave
 
 // One run of outputs of one tile, by N threads.  s_z: the waves' own rows, then z of at most M rows.
 template <int T, int N, int M, class R>
-__device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &rows, int run, char *s_z, int &s_wide) {
+__device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &rows, int run, char *s_z, uint32_t (&s_wide)[2]) {
     int mat = 0;
     while (run >= a.chunks[mat]) ++mat;
     if (mat > 0) run -= a.chunks[mat - 1];
@@ -728,12 +761,11 @@ __device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &r
         }
     };
     // (rows 16 bytes more than a multiple of 64 apart: 16 lanes meet 16 times 4 banks)
-    Staged z = {2 * width + 16, M * (2 * width + 16), T == 2};
     if constexpr (T != 2) {
-        bool wide = false;
+        const Staged z = {2 * width + 16, M * (2 * width + 16)};
         each([&](int r, int row, int k) {
             const f32x4 v = z_of(row, k);
-            wide |= !(max3_abs(v[0], v[1], fmaxf(fabsf(v[2]), fabsf(v[3]))) < kWide);
+            if (!(max3_abs(v[0], v[1], fmaxf(fabsf(v[2]), fabsf(v[3]))) < kWide)) atomicOr(&s_wide[r >> 5], 1u << (r & 31));
             uint2 h, m, l;
             split3(v[0] * kUp, v[1] * kUp, h.x, m.x, l.x);
             split3(v[2] * kUp, v[3] * kUp, h.y, m.y, l.y);
@@ -742,24 +774,21 @@ __device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &r
             *reinterpret_cast<uint2 *>(at + z.part) = m;
             *reinterpret_cast<uint2 *>(at + 2 * z.part) = l;
         });
-        if (wide) s_wide = 1;
         __syncthreads();
-        z.wide = s_wide != 0;
-    }
-    if (z.wide) {  // uniform
-        z.stride = 4 * width + 16;
-        if (T != 2) __syncthreads();
-        each([&](int r, int row, int k) { *reinterpret_cast<f32x4 *>(s_parts + r * z.stride + 4 * k) = z_of(row, k); });
-        __syncthreads();
-    }
-    const char *rows_z = s_parts + from * z.stride;
-    if constexpr (T != 2) {
-        if (!z.wide) {  // uniform
+        const uint64_t apart = static_cast<uint64_t>(s_wide[1]) << 32 | s_wide[0];  // rows with a value that the parts cannot hold
+        if (apart) up.choose(~apart, from, t.count);  // uniform
+        const char *rows_z = s_parts + from * z.stride;
 #pragma unroll 1
-            for (int i = 0; i < passes; ++i) up.template add<false>(at(i), i + 1 < passes ? at(i + 1) : -1, z, rows_z);
-            return;
-        }
+        for (int i = 0; i < passes; ++i) up.template add<false>(at(i), i + 1 < passes ? at(i + 1) : -1, z, rows_z);
+        if (!apart) return;  // uniform
+        up.choose(apart, from, t.count);
+        if (passes > 0) up.load(at(0));
+        __syncthreads();  // (the parts are read)
     }
+    const Staged z = {4 * width + 16, 0};
+    each([&](int r, int row, int k) { *reinterpret_cast<f32x4 *>(s_parts + r * z.stride + 4 * k) = z_of(row, k); });
+    __syncthreads();
+    const char *rows_z = s_parts + from * z.stride;
 #pragma unroll 1
     for (int i = 0; i < passes; ++i) up.template add<true>(at(i), i + 1 < passes ? at(i + 1) : -1, z, rows_z);
 }
@@ -767,13 +796,13 @@ __device__ __forceinline__ void up(const LoraArgs &a, const Group &t, const R &r
 template <int T, bool FEW>
 __global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel(LoraArgs a) {
     extern __shared__ __attribute__((aligned(16))) char s_z[];
-    __shared__ int s_wide;
+    __shared__ uint32_t s_wide[2];  // of a tile's rows
     const int runs = a.chunks[a.n_mats - 1];
     if constexpr (FEW) {
         LaneRows rows;
         const Group t = find_tile(a, blockIdx.x / runs, rows);
         if (t.count == 0) return;  // uniform
-        if (threadIdx.x == 0) s_wide = 0;
+        if (threadIdx.x < 2) s_wide[threadIdx.x] = 0;
         __syncthreads();
         up<T, kThreads, 16>(a, t, rows, blockIdx.x % runs, s_z, s_wide);
     } else {
@@ -783,7 +812,7 @@ __global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel
             __syncthreads();  // (the tile of before is read)
             const Group of = tile_at(a, item / runs, s_rows);
             if (of.count == 0) break;  // uniform
-            if (threadIdx.x == 0) s_wide = 0;
+            if (threadIdx.x < 2) s_wide[threadIdx.x] = 0;
             __syncthreads();
             up<T, kUpThreads, kTile>(a, of, rows, item % runs, s_z, s_wide);
         }

@@ -200,7 +200,8 @@ typedef struct qlin_logits_controls {
  * much of a slot counts: the rest is not used, whatever it holds.  scales [n_adapters] or NULL (1).
  * Accuracy: exact products, sums in f32; A x is held in f32, then multiplied by the scale, and base is added to the sum in one
  * step.  bf16 and f16 weights are below 2^30 in magnitude, and sums of |A x| and |B z| below 2^100 (f32 weights, or an x or z of 2^60
- * or more: as far as f32 holds); an infinite weight gives NaN.  Infinities and NaN of x stay in their rows.
+ * or more: as far as f32 holds); an infinite weight gives NaN.  Infinities and NaN of x stay in their rows; a
+ * row's result has the same bits whatever the others hold and wherever it stands among as many.
  * n_adapters >= 1, in_dim and max_rank are multiples of 8, from 8 on (else QLIN_ERR_SHAPE), max_rank <= 256, n_adapters <= 1024 and rows <= 65536 (else
  * QLIN_ERR_LIMIT); a and b 16-byte aligned, the rest 4-byte (else QLIN_ERR_ALIGN).  Strides in floats, >= the row.
  * workspace: qlin_lora_workspace_bytes(...) bytes, 16-byte aligned, used by nothing else while the launches run (calls
