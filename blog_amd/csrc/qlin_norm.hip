@@ -191,11 +191,15 @@ hipStream_t current_stream() { return static_cast<hipStream_t>(qlin_get_stream()
 bool al(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 template <int W, int U>
-void launch(const NormArgs &a) {
+int launch(const NormArgs &a) {
     constexpr int R = W < 4 ? 4 / W : 1;
-    const dim3 grid((a.rows + R - 1) / R), block(W < 4 ? 256 : 64 * W);
+    const dim3 block(W < 4 ? 256 : 64 * W);
+    const int64_t groups = (static_cast<int64_t>(a.rows) + R - 1) / R;
+    if (groups * block.x > UINT32_MAX) return QLIN_ERR_LIMIT;
+    const dim3 grid(static_cast<unsigned>(groups));
     if (streamed(static_cast<int64_t>(a.rows) * a.hidden)) hipLaunchKernelGGL((add_rms_norm_kernel<W, U, true>), grid, block, 0, current_stream(), a);
     else hipLaunchKernelGGL((add_rms_norm_kernel<W, U, false>), grid, block, 0, current_stream(), a);
+    return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -224,16 +228,15 @@ int qlin_launch_add_rms_norm(const float *x, size_t x_stride, const float *delta
     const int unit = !q8_1 ? 1 : mmq ? 128 : 32;
     qlin::NormArgs a = {x, delta, sum, normed, q8_1, weight, x_stride, delta_stride, sum_stride, normed_stride, norm_type,
                         one_plus, rows, hidden, (hidden + unit - 1) / unit * unit, mmq != 0, raw_sum != 0, eps};
-    if (a.padded <= 256) qlin::launch<1, 1>(a);
-    else if (a.padded <= 1024) qlin::launch<4, 1>(a);
-    else if (a.padded <= 2048 && rows < 512) qlin::launch<8, 1>(a);
-    else if (a.padded <= 2048) qlin::launch<4, 2>(a);
-    else if (a.padded <= 4096 && rows < 512) qlin::launch<16, 1>(a);
-    else if (a.padded <= 4096) qlin::launch<4, 4>(a);
-    else if (a.padded <= 8192) qlin::launch<16, 2>(a);
-    else if (a.padded <= 16384) qlin::launch<16, 4>(a);
-    else qlin::launch<16, 0>(a);
-    return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;
+    if (a.padded <= 256) return qlin::launch<1, 1>(a);
+    if (a.padded <= 1024) return qlin::launch<4, 1>(a);
+    if (a.padded <= 2048 && rows < 512) return qlin::launch<8, 1>(a);
+    if (a.padded <= 2048) return qlin::launch<4, 2>(a);
+    if (a.padded <= 4096 && rows < 512) return qlin::launch<16, 1>(a);
+    if (a.padded <= 4096) return qlin::launch<4, 4>(a);
+    if (a.padded <= 8192) return qlin::launch<16, 2>(a);
+    if (a.padded <= 16384) return qlin::launch<16, 4>(a);
+    return qlin::launch<16, 0>(a);
 }
 
 int qlin_launch_dequantize_q8_1(const uint8_t *x_q8_1, float *x, int in_dim, int m, int mmq) {

@@ -152,8 +152,10 @@ extern "C" int qlin_launch_moe_route(const qlin_moe_routing *how, const float *r
     for (const void *p : {static_cast<const void *>(h.bias), static_cast<const void *>(router_logits),
                           static_cast<const void *>(expert_ids), static_cast<const void *>(weights)})
         if (!qlin::al4(p)) return QLIN_ERR_ALIGN;
+    const int64_t groups = (static_cast<int64_t>(tokens) + qlin::kWaves - 1) / qlin::kWaves;
+    if (groups * 64 * qlin::kWaves > UINT32_MAX) return QLIN_ERR_LIMIT;
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((tokens + qlin::kWaves - 1) / qlin::kWaves), dim3(64 * qlin::kWaves), 0,
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(64 * qlin::kWaves), 0,
                            static_cast<hipStream_t>(qlin_get_stream()), h, router_logits, logits_stride, expert_ids, weights,
                            tokens, n_experts, k);
         return hipGetLastError() == hipSuccess ? QLIN_OK : QLIN_ERR_LAUNCH;

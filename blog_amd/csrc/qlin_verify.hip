@@ -550,7 +550,7 @@ int qlin_launch_verify_drafts(const float *target, size_t target_stride, const f
     if (max_drafts == 0) draft = nullptr;
     const qlin::Layout l = qlin::layout_of(n_seqs, max_drafts, vocab);
     const int64_t grid = static_cast<int64_t>(n_seqs) * (max_drafts + 1 + (draft ? max_drafts : 0)) * l.slices;
-    if (grid > (1 << 23)) return QLIN_ERR_LIMIT;
+    if (grid > (1 << 23) || static_cast<int64_t>(n_seqs) * qlin::kDecideThreads > UINT32_MAX) return QLIN_ERR_LIMIT;
     if (!workspace) return QLIN_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(workspace) & 15u) return QLIN_ERR_ALIGN;
     if (workspace_bytes < l.bytes) return QLIN_ERR_LIMIT;

@@ -218,8 +218,8 @@ int qlin_launch_moe_router_topk(const float *router_logits, int *top_idx, float 
  * and one with such a logit or with a c that is -inf or NaN (a bias of -inf switches an expert off) is not picked: where
  * none is left the picks are -1 with weight 0, which the routed products skip.  So the picks go straight into
  * qlin_moe_routed_decode_indexed and qlin_moe_routed_decode_grouped.
- * logits_stride: floats from a token's logits to the next one's, >= n_experts.  n_experts <= 1024, n_groups <= 64 and
- * k <= 64 (else QLIN_ERR_LIMIT); n_groups divides n_experts, 1 <= top_groups <= n_groups, and k is at most the number of
+ * logits_stride: floats from a token's logits to the next one's, >= n_experts.  n_experts <= 1024, n_groups <= 64,
+ * k <= 64 and tokens < 1 << 26 (else QLIN_ERR_LIMIT); n_groups divides n_experts, 1 <= top_groups <= n_groups, and k is at most the number of
  * experts in top_groups groups (else QLIN_ERR_SHAPE). */
 typedef struct qlin_moe_routing {
     const float *bias; /* [n_experts], or NULL */

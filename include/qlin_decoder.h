@@ -185,7 +185,8 @@ typedef struct qlin_logits_controls {
  *   with a value that is not finite has scale NaN and codes 0.
  * normed or q8_1 or both.  *_stride: floats from a row to the next one, >= hidden.  sum may be x or delta (same pointer and
  * stride: the residual stream in place), and normed may be x or delta where sum is not; else outputs overlap nothing.
- * Norm weights 2-byte aligned, q8_1 and the rest 4-byte (else QLIN_ERR_ALIGN).
+ * Norm weights 2-byte aligned, q8_1 and the rest 4-byte (else QLIN_ERR_ALIGN).  hidden <= 1 << 24, and rows < 1 << 22 (up to hidden
+ * 4096 rows < 1 << 24) as what a launch holds (else QLIN_ERR_LIMIT).
  */
 
 /* ---- low-rank adapters of many requests beside a shared projection -------------------------------
@@ -237,7 +238,7 @@ typedef struct qlin_lora {
  * below 1; NaN: 0).  A logit that is NaN counts as -inf; tokens at +inf share a row's probability.  A row without any
  * logit above -inf accepts nothing; where y would come from it, y is 0 with logprob -inf.  A drafted token outside
  * [0, vocab) is not accepted (and by lookup takes nothing from p).
- * vocab <= 1 << 21 and max_drafts <= 63 (else QLIN_ERR_LIMIT).  Pointers 4-byte aligned, the workspace 16-byte
+ * vocab <= 1 << 21, max_drafts <= 63, n_seqs < 1 << 22 and what the launches hold, 1 << 23 slices of rows (else QLIN_ERR_LIMIT).  Pointers 4-byte aligned, the workspace 16-byte
  * (qlin_verify_drafts_workspace_bytes(...) bytes; rules as qlin_launch_lora_add's).
  */
 
