@@ -319,7 +319,7 @@ def graphs_us_interleaved(torch, qlin, fns, reps, rounds=5):
 
 
 def cpu_threads():
-    """The process's CPU thread share: OMP_NUM_THREADS (16 per GPU job on the GPU boxes), else every
+    """The process's CPU thread share: OMP_NUM_THREADS (as a job is given it), else every
     CPU it may run on."""
     return int(os.environ.get("OMP_NUM_THREADS", "0") or 0) or host_cpu()["cpus_allowed"]
 

@@ -21,7 +21,7 @@ SOURCES = ["qlin_gemv.hip", "qlin_q4k_stream.hip", "qlin_mfma_gemv.hip", "qlin_q
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
     f"-I{os.path.join(ROOT, 'include')}", f"-I{CSRC}",
-    # packed-FP32 VALU forms have produced silent wrong results on this pool: never emit them
+    # packed-FP32 VALU forms have given silent wrong results: never emit them
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # keep every IEEE operation as written (bit-exact dequant); explicit fmaf() calls still fuse
     "-ffp-contract=off",

@@ -14,8 +14,8 @@
 // 2^26 v of an f32 value v is the sum of three (8 bits each; with the factor, which leaves with the sum, all parts of any v are
 // normal numbers).  Where a |v| is 2^60 or more (or infinite) these would overflow: such values of x, and the rows of z that have
 // one, go to v_mfma_f32_16x16x4_f32 after the others, a uniform and rare branch, so that no row's result depends on the rows beside
-// it; f32 weights go there always.  (All types there: 613 rows of 18944 to 3584 with 8 adapters of rank 64 in f16 63.3 and 57.4 us
-// in the two launches, where they take 25.3 and 14.0.)
+// it; f32 weights go there always: 613 rows of 18944 to 3584 with 8 adapters of rank 64 51 us in a graph, of f16 42 and of bf16
+// 35; 2011 of 4096 to 14336 with 3 97, 76 and 68.
 //
 // Few rows are bound by latency: one row of 896 to 896, 128 and 128 at rank 16 takes 9.7 us in a graph, 48 rows of 3584 to 3584,
 // 512 and 512 with 15 adapters of rank 32 15.8.  Many are bound by memory in the second launch (2011 rows of 4096 to 14336 at rank
@@ -822,6 +822,7 @@ __global__ __launch_bounds__(FEW ? kThreads : kUpThreads, 2) void lora_up_kernel
 bool al(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Whether each wave groups the rows: what that takes grows with the adapters in use, 64 rows at a time, a launch for it takes 4 us.
+// (How many are in use stands on the device alone; there are no more than slots.)
 bool few_of(int rows, int n_adapters) { return rows <= 64 || (rows <= kFewRows && n_adapters < 32); }
 
 struct Layout {

@@ -1,8 +1,8 @@
 // qlin_norm.hip -- the residual's addition, the RMSNorm and its result in f32 and in Q8_1 blocks in one pass, and Q8_1
 // blocks read back as the values they stand for (qlin_launch_add_rms_norm, qlin_launch_dequantize_q8_1), gfx950.
 //
-// Mathematics (qlin_decoder.h): s = x + delta, y = s (mean s^2 + eps)^(-1/2) w, blocks of 32 values as codes rint(y / d),
-// d = amax / 127.  The sum of squares, the root and the product are in f64: y then is the same f32 value whatever the order of
+// Mathematics (qlin_decoder.h): s = x + delta, y = s (mean s^2 + eps)^(-1/2) w, blocks of 32 values as codes rint(y (1 / d)),
+// d = amax (1 / 127).  The sum of squares, the root and the product are in f64: y then is the same f32 value whatever the order of
 // the sum, and so are the codes (an f64 operation takes an f32 one's time here).
 //
 // A row is taken by W waves, 4 consecutive values a lane and U such runs in registers, so that x is read once; 8 lanes hold
@@ -10,7 +10,8 @@
 // that outputs may take the inputs' place.  Many rows are bound by HBM: 2011 rows of 4096 with their sum and blocks of 128 and
 // the blocks read back, 150 MB, take 35.1 us in a graph (4.3 TB/s; 8 waves of 2 runs 35.5, 16 of one 37.3), 42 with f32 results
 // through the caches: from 16 MB on they leave as streaming stores.  Few rows are bound by latency: 16 waves take a row of 3584 in
-// 4.4 us, 4 waves in 6.4; 48 rows of 2048 with f32 results and blocks take 4.0 by 8 waves each, 5.0 by 4.
+// 4.4 us, 4 waves in 6.4; 48 rows of 2048 with f32 results and blocks take 4.0 by 8 waves each, 5.0 by 4.  Wider rows take 16
+// waves however many they are: 2011 rows of 8192 49 us in a graph, by 8 waves of 4 runs 53; of 16384 95, by 8 of 8 runs 102.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

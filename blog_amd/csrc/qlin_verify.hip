@@ -13,8 +13,9 @@
 // 3. With draft logits: verify_rest_kernel sums max(p - q, 0) over each slice of the one row where a draft was rejected,
 //    verify_draw_kernel draws, also from p alone (in 2., a draw that a few sequences wait for cost all of them 4 us).
 //
-// 24 sequences of 4 drafts with their logits, 216 rows of 151936, take 51 us in a graph: 30.8 of the first launch, bound by HBM
-// (131 MB, 4.3 TB/s in the trace), and 5.1, 8.7 and 6.2 of chains of dependent loads, sums and barriers.  One sequence of 4
+// 24 sequences of 4 drafts with their logits, 216 rows of 151936, take 51 us in a graph: 30.8 of the first launch, bound by
+// its vector work (25 instructions a logit, which issue in 85% of its busy cycles; 131 MB at 4.3 TB/s beside), and 5.1, 8.7 and 6.2
+// of chains of dependent loads, sums and barriers.  One sequence of 4
 // drafts by lookup takes 9.8 us, 40 draws of 102400 without drafts 13.4: latency but for 3.2 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
